@@ -364,6 +364,195 @@ typedef struct mfa_merge_params {
 int mfa_merge(const mfa_merge_params* params, void* stream);
 int mfa_merge_params_size(void);
 
+/*
+ * Paged 4-bit K/V cache.  No counterpart in the reference.
+ *
+ * K and V are pools of pages, [num_pages, page_block_size, heads_kv, ...], held
+ * as code and scale bytes: a row of one head has head_dim / 2 code bytes and
+ * head_dim / 32 scale bytes, both contiguous.  32 consecutive elements share the
+ * power of two 2^(s - 127) of their scale byte s (255: all NaN); element 2i is
+ * the low half and element 2i + 1 the high half of code byte i, each a 4-bit
+ * float with a sign bit, two exponent bits and one mantissa bit (magnitudes 0,
+ * 0.5, 1, 1.5, 2, 3, 4, 6).  Page, row and head strides are in bytes, any order,
+ * row and head strides >= 0 (each head's rows of a page side by side read
+ * fastest); codes start at 16-byte aligned addresses with strides that are
+ * multiples of 16 bytes, scales have none to keep.
+ * Row j of sequence b is row j % page_block_size of page
+ * block_table[b * block_table_batch_stride + j / page_block_size];
+ * page_block_size is a multiple of 64, and max_pages the columns of the table.
+ * Page ids are read on the device: an id outside [0, num_pages) reads as zeros
+ * and drops what is written, never out of bounds.
+ */
+typedef struct mfa_kv4_pool {
+    uint8_t* codes;
+    uint8_t* scales;
+    int64_t code_page_stride, code_row_stride, code_head_stride;
+    int64_t scale_page_stride, scale_row_stride, scale_head_stride;
+} mfa_kv4_pool;
+typedef struct mfa_kv4_cache {
+    mfa_kv4_pool k, v;
+    const int32_t* block_table;
+    int64_t block_table_batch_stride;
+    int32_t max_pages, page_block_size, num_pages;
+    int32_t reserved;
+} mfa_kv4_cache;
+
+/*
+ * New rows into the cache.  k and v are [total, heads_kv, head_dim] of `dtype`
+ * (16-byte aligned, strides multiples of 16 bytes, head dim contiguous); token t
+ * of sequence b, cu_seqlens[b] <= t < cu_seqlens[b + 1], becomes row
+ * cache_seqlens[b] + t - cu_seqlens[b].  A row outside the table, or whose page
+ * id is outside the pool, is dropped, as are tokens of no sequence; two tokens
+ * must not share a row.  The scale of 32 elements is the smallest power of two
+ * (2^-127 at least) that leaves them within 7 times it, so that none is off by
+ * more than half a step; elements are rounded to the nearest value, ties to the
+ * even code, and a group that holds an infinity or NaN becomes NaN.
+ * k_values / v_values (optional, both or none): what the cache now holds for
+ * every token, contiguous [total, heads_kv, head_dim] of `dtype`.
+ * head_dim: a multiple of 32 up to MFA_MAX_HEAD_DIM.  One kernel; never
+ * synchronizes, never allocates.
+ */
+typedef struct mfa_kv4_append_params {
+    mfa_kv4_cache cache;
+    const void* k;
+    const void* v;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride; /* elements */
+    void* k_values;
+    void* v_values;
+    const int32_t* cu_seqlens;    /* [batch + 1] */
+    const int32_t* cache_seqlens; /* [batch], rows already held */
+    int32_t batch, total, heads_kv, head_dim;
+    int32_t dtype; /* MFA_DTYPE_* of k, v and the values */
+} mfa_kv4_append_params;
+int mfa_kv4_append(const mfa_kv4_append_params* params, void* stream);
+int mfa_kv4_append_params_size(void);
+
+/*
+ * Attention over the cache: the forward of mfa_fwd (masks, soft-cap, ALiBi,
+ * grouped-query heads and softmax_lse as there) with K and V from the cache.
+ * Sequence b has min(cache_seqlens[b], max_seqlen_k, what the table can name)
+ * keys, read on the device; max_seqlen_k 0 leaves the bound out.  Queries: q
+ * [batch, seqlen_q, heads_q, head_dim], or with cu_seqlens_q q [total_q, heads_q,
+ * head_dim], sequence b owning tokens [cu_seqlens_q[b], cu_seqlens_q[b + 1])
+ * (tokens of no sequence are left unwritten).  The query rows are the last
+ * positions of their sequence.  q and o: fp16 or bf16, 16-byte aligned, strides
+ * multiples of 8 elements.  head_dim: 32, 64, 96 or 128.
+ * Enqueues one or two kernels; never synchronizes, never allocates.  The results
+ * do not depend on the workspace's address or content; they may differ in the
+ * last bit with the batch a sequence stands in (its keys are dealt over
+ * workgroups with the others').
+ */
+typedef struct mfa_kv4_fwd_params {
+    mfa_kv4_cache cache;
+    const void* q;
+    void* o;
+    int64_t q_batch_stride, q_seq_stride, q_head_stride;
+    int64_t o_batch_stride, o_seq_stride, o_head_stride;
+    float* softmax_lse; /* NULL = not written; layout as in mfa_fwd_params */
+    int64_t lse_batch_stride, lse_head_stride;
+    const int32_t* cu_seqlens_q; /* NULL = seqlen_q rows per sequence */
+    const int32_t* cache_seqlens;
+    const float* alibi_slopes;
+    int32_t alibi_batch_stride;
+    int32_t batch, seqlen_q, total_q, heads_q, heads_kv, head_dim, max_seqlen_k;
+    float scale, softcap;
+    int32_t window_left, window_right, causal;
+    int32_t dtype;
+} mfa_kv4_fwd_params;
+int64_t mfa_kv4_fwd_workspace_bytes(const mfa_kv4_fwd_params* params);
+int mfa_kv4_fwd(const mfa_kv4_fwd_params* params, void* workspace, int64_t workspace_bytes, void* stream);
+int mfa_kv4_fwd_params_size(void);
+
+/*
+ * Pages copied inside pools: page src[i] to page dst[i] of every pool, i < pairs
+ * (a forked sequence's last page, compaction).  No counterpart in the reference.
+ * A pool is `page_bytes` contiguous bytes per page, `page_stride` bytes apart.
+ * Pairs with an id outside [0, num_pages) are skipped.  The destinations have to
+ * differ from each other and from every source: pairs are copied in no order.
+ * One kernel; never synchronizes, never allocates.
+ */
+#define MFA_COPY_MAX_POOLS 64
+typedef struct mfa_copy_pool {
+    void* base;
+    int64_t page_stride, page_bytes;
+} mfa_copy_pool;
+typedef struct mfa_copy_pages_params {
+    mfa_copy_pool pool[MFA_COPY_MAX_POOLS];
+    const int32_t* src;
+    const int32_t* dst;
+    int32_t pools, pairs, num_pages;
+    int32_t reserved;
+} mfa_copy_pages_params;
+int mfa_copy_pages(const mfa_copy_pages_params* params, void* stream);
+int mfa_copy_pages_params_size(void);
+
+/*
+ * RMS norm of every query and key head and the rotation of its position, in one
+ * pass.  No counterpart in the reference.  For a row x of head_dim elements at
+ * position pos:
+ *   n = x / sqrt(mean(x^2) + eps), y = n * weight (q_weight / k_weight, NULL: 1),
+ *   out_a = y_a cos - y_b sin, out_b = y_b cos + y_a sin
+ * for each pair i < rotary_dim / 2 with cos[pos][i], sin[pos][i]: elements (a, b)
+ * = (i, i + rotary_dim / 2), or (2i, 2i + 1) with `interleaved`; elements from
+ * rotary_dim on are y.  fp32 arithmetic, one rounding.  A position outside
+ * [0, table_rows) gives NaN in the rotated elements, never a read out of bounds.
+ * q [batch, seqlen, heads_q, head_dim], k [batch, seqlen, heads_kv, head_dim] by
+ * element strides (head dim contiguous); outputs and gradients are contiguous.
+ * positions: [batch, seqlen] int32 or int64 (positions_64) with
+ * positions_batch_stride (0: one row for the batch) and unit stride inside, NULL:
+ * 0, 1, 2, ...  cos / sin: [table_rows, rotary_dim / 2], rows table_stride
+ * elements apart.  head_dim up to MFA_MAX_HEAD_DIM, rotary_dim even, 0 <=
+ * rotary_dim <= head_dim.  One kernel; never synchronizes, never allocates.
+ */
+typedef struct mfa_norm_rope_params {
+    const void* q;
+    const void* k;
+    void* q_out;
+    void* k_out;
+    int64_t q_batch_stride, q_seq_stride, q_head_stride;
+    int64_t k_batch_stride, k_seq_stride, k_head_stride;
+    const void* q_weight;
+    const void* k_weight;
+    const void* cos;
+    const void* sin;
+    int64_t table_stride;
+    const void* positions;
+    int64_t positions_batch_stride;
+    int32_t batch, seqlen, heads_q, heads_kv, head_dim, rotary_dim, table_rows;
+    int32_t positions_64, interleaved;
+    int32_t dtype;        /* of q, k and the outputs */
+    int32_t dtype_weight; /* of the weights and their gradients */
+    int32_t dtype_table;  /* of cos and sin */
+    float eps;
+} mfa_norm_rope_params;
+int mfa_norm_rope(const mfa_norm_rope_params* params, void* stream);
+int mfa_norm_rope_params_size(void);
+
+/*
+ * Backward of mfa_norm_rope (fwd.q_out / k_out unused): with g the rotation of
+ * dq_out turned back, h = g * weight,
+ *   dq = (h - n mean(h n)) / sqrt(mean(x^2) + eps),  dq_weight = sum over rows g n
+ * and the same for k.  dq / dk are contiguous.  Weight gradients (dtype_weight)
+ * where the weight is set and the pointer is not NULL: summed in fp32, in an
+ * order that the sizes alone decide.  `workspace`: 256-byte aligned, at least
+ * mfa_norm_rope_bwd_workspace_bytes bytes.  One or two kernels; never
+ * synchronizes, never allocates.
+ */
+typedef struct mfa_norm_rope_bwd_params {
+    mfa_norm_rope_params fwd;
+    const void* dq_out;
+    const void* dk_out;
+    int64_t dqo_batch_stride, dqo_seq_stride, dqo_head_stride;
+    int64_t dko_batch_stride, dko_seq_stride, dko_head_stride;
+    void* dq;
+    void* dk;
+    void* dq_weight;
+    void* dk_weight;
+} mfa_norm_rope_bwd_params;
+int64_t mfa_norm_rope_bwd_workspace_bytes(const mfa_norm_rope_bwd_params* params);
+int mfa_norm_rope_bwd(const mfa_norm_rope_bwd_params* params, void* workspace, int64_t workspace_bytes, void* stream);
+int mfa_norm_rope_bwd_params_size(void);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,19 +18,25 @@ paged K/V cache (`block_table`, CUDA flash-attn's layout), and
 softmax log-sum-exp, which `merge_attention_partials` uses to combine attention
 over disjoint key sets (context-parallel shards, cache + new tokens).
 
+Around the attention call: `qk_norm_rope` (RMS norm and rotation of the query
+and key heads in one pass, differentiable), and a paged K/V cache held in 4 bits
+(`kv4_cache`, `kv4_append`, `flash_attn_kv4_func`, `flash_attn_varlen_kv4_func`,
+`copy_cache_pages`).
+
 Every call runs the gfx950 HIP kernels of libmtlfa_hip.so on the tensors'
 ROCm device; there is no CPU path.
 """
 from __future__ import annotations
 
 import math
-import os
 
 import torch
 
 from . import _kernel
 from ._kernel import MAX_HEAD_DIM, flash_attn_forward, forward_bshd, forward_varlen
 from ._version import __version__
+from .kv4 import copy_cache_pages, flash_attn_kv4_func, flash_attn_varlen_kv4_func, kv4_append, kv4_cache
+from .norm_rope import qk_norm_rope
 
 __all__ = [
     "flash_attn_func",
@@ -43,6 +49,12 @@ __all__ = [
     "flash_attn_func_with_lse",
     "flash_attn_varlen_func_with_lse",
     "merge_attention_partials",
+    "qk_norm_rope",
+    "kv4_cache",
+    "kv4_append",
+    "flash_attn_kv4_func",
+    "flash_attn_varlen_kv4_func",
+    "copy_cache_pages",
     "__version__",
 ]
 
@@ -53,19 +65,7 @@ def _check_supported(q, k, v, dropout_p, window_size, softcap, alibi_slopes, det
     """Error contract of metal_flash_attn/__init__.py:28-59, checked in the same order."""
     if dropout_p:
         raise NotImplementedError("mtlflashattn_amd: dropout_p > 0 not supported (inference-only)")
-    if (
-        not isinstance(window_size, (tuple, list))
-        or len(window_size) != 2
-        or any(not isinstance(w, int) or isinstance(w, bool) or w < -1 for w in window_size)
-    ):
-        raise ValueError(
-            "mtlflashattn_amd: window_size must be a (left, right) pair of ints >= -1 "
-            "(-1 = unbounded on that side)"
-        )
-    if softcap < 0:
-        raise ValueError("mtlflashattn_amd: softcap must be >= 0 (0 disables capping)")
-    if alibi_slopes is not None and not torch.is_tensor(alibi_slopes):
-        raise TypeError("mtlflashattn_amd: alibi_slopes must be a tensor of per-head slopes")
+    _kernel._check_options(window_size, softcap, alibi_slopes)
     if deterministic:
         raise NotImplementedError("mtlflashattn_amd: deterministic not supported")
     if return_attn_probs:
@@ -303,7 +303,7 @@ def _check_block_table(block_table, lens_k, page, num_pages):
                          f"{max(need)} needed for {max(lens_k)} keys")
     if not need or max(need) == 0:
         return
-    if os.environ.get("MTLFLASHATTN_CHECK_PAGES", "").lower() not in ("1", "on", "true", "yes"):
+    if not _kernel._check_pages_enabled():
         return
     used = torch.arange(block_table.shape[1]).unsqueeze(0) < torch.tensor(need).unsqueeze(1)
     ids = block_table.cpu()[used]

@@ -106,6 +106,95 @@ class MfaMergeParams(ctypes.Structure):
     ]
 
 
+class MfaKv4Pool(ctypes.Structure):
+    """Mirror of `mfa_kv4_pool` (include/mfa.h)."""
+
+    _fields_ = [
+        ("codes", _c_ptr), ("scales", _c_ptr),
+        ("code_page_stride", _c_i64), ("code_row_stride", _c_i64), ("code_head_stride", _c_i64),
+        ("scale_page_stride", _c_i64), ("scale_row_stride", _c_i64), ("scale_head_stride", _c_i64),
+    ]
+
+
+class MfaKv4Cache(ctypes.Structure):
+    """Mirror of `mfa_kv4_cache` (include/mfa.h)."""
+
+    _fields_ = [
+        ("k", MfaKv4Pool), ("v", MfaKv4Pool), ("block_table", _c_ptr), ("block_table_batch_stride", _c_i64),
+        ("max_pages", _c_i32), ("page_block_size", _c_i32), ("num_pages", _c_i32), ("reserved", _c_i32),
+    ]
+
+
+class MfaKv4AppendParams(ctypes.Structure):
+    """Mirror of `mfa_kv4_append_params` (include/mfa.h)."""
+
+    _fields_ = [
+        ("cache", MfaKv4Cache), ("k", _c_ptr), ("v", _c_ptr),
+        ("k_token_stride", _c_i64), ("k_head_stride", _c_i64), ("v_token_stride", _c_i64), ("v_head_stride", _c_i64),
+        ("k_values", _c_ptr), ("v_values", _c_ptr), ("cu_seqlens", _c_ptr), ("cache_seqlens", _c_ptr),
+        ("batch", _c_i32), ("total", _c_i32), ("heads_kv", _c_i32), ("head_dim", _c_i32), ("dtype", _c_i32),
+    ]
+
+
+class MfaKv4FwdParams(ctypes.Structure):
+    """Mirror of `mfa_kv4_fwd_params` (include/mfa.h)."""
+
+    _fields_ = [
+        ("cache", MfaKv4Cache), ("q", _c_ptr), ("o", _c_ptr),
+        ("q_batch_stride", _c_i64), ("q_seq_stride", _c_i64), ("q_head_stride", _c_i64),
+        ("o_batch_stride", _c_i64), ("o_seq_stride", _c_i64), ("o_head_stride", _c_i64),
+        ("softmax_lse", _c_ptr), ("lse_batch_stride", _c_i64), ("lse_head_stride", _c_i64),
+        ("cu_seqlens_q", _c_ptr), ("cache_seqlens", _c_ptr), ("alibi_slopes", _c_ptr), ("alibi_batch_stride", _c_i32),
+        ("batch", _c_i32), ("seqlen_q", _c_i32), ("total_q", _c_i32), ("heads_q", _c_i32), ("heads_kv", _c_i32),
+        ("head_dim", _c_i32), ("max_seqlen_k", _c_i32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+        ("window_left", _c_i32), ("window_right", _c_i32), ("causal", _c_i32), ("dtype", _c_i32),
+    ]
+
+
+MFA_COPY_MAX_POOLS = 64
+
+
+class MfaCopyPool(ctypes.Structure):
+    """Mirror of `mfa_copy_pool` (include/mfa.h)."""
+
+    _fields_ = [("base", _c_ptr), ("page_stride", _c_i64), ("page_bytes", _c_i64)]
+
+
+class MfaCopyPagesParams(ctypes.Structure):
+    """Mirror of `mfa_copy_pages_params` (include/mfa.h)."""
+
+    _fields_ = [
+        ("pool", MfaCopyPool * MFA_COPY_MAX_POOLS), ("src", _c_ptr), ("dst", _c_ptr),
+        ("pools", _c_i32), ("pairs", _c_i32), ("num_pages", _c_i32), ("reserved", _c_i32),
+    ]
+
+
+class MfaNormRopeParams(ctypes.Structure):
+    """Mirror of `mfa_norm_rope_params` (include/mfa.h)."""
+
+    _fields_ = [
+        ("q", _c_ptr), ("k", _c_ptr), ("q_out", _c_ptr), ("k_out", _c_ptr),
+        ("q_batch_stride", _c_i64), ("q_seq_stride", _c_i64), ("q_head_stride", _c_i64),
+        ("k_batch_stride", _c_i64), ("k_seq_stride", _c_i64), ("k_head_stride", _c_i64),
+        ("q_weight", _c_ptr), ("k_weight", _c_ptr), ("cos", _c_ptr), ("sin", _c_ptr), ("table_stride", _c_i64),
+        ("positions", _c_ptr), ("positions_batch_stride", _c_i64),
+        ("batch", _c_i32), ("seqlen", _c_i32), ("heads_q", _c_i32), ("heads_kv", _c_i32), ("head_dim", _c_i32),
+        ("rotary_dim", _c_i32), ("table_rows", _c_i32), ("positions_64", _c_i32), ("interleaved", _c_i32),
+        ("dtype", _c_i32), ("dtype_weight", _c_i32), ("dtype_table", _c_i32), ("eps", ctypes.c_float),
+    ]
+
+
+class MfaNormRopeBwdParams(ctypes.Structure):
+    """Mirror of `mfa_norm_rope_bwd_params` (include/mfa.h)."""
+
+    _fields_ = [
+        ("fwd", MfaNormRopeParams), ("dq_out", _c_ptr), ("dk_out", _c_ptr),
+        ("dqo_batch_stride", _c_i64), ("dqo_seq_stride", _c_i64), ("dqo_head_stride", _c_i64),
+        ("dko_batch_stride", _c_i64), ("dko_seq_stride", _c_i64), ("dko_head_stride", _c_i64),
+        ("dq", _c_ptr), ("dk", _c_ptr), ("dq_weight", _c_ptr), ("dk_weight", _c_ptr),
+    ]
+
+
 class MfaLaunchInfo(ctypes.Structure):
     """Mirror of `mfa_launch_info` (include/mfa.h)."""
 
@@ -119,6 +208,15 @@ class MfaLaunchInfo(ctypes.Structure):
 class HipLibraryError(RuntimeError):
     """The HIP kernel library is missing, stale or failed a call."""
 
+
+# entry points of one parameter struct: (name, struct, takes a workspace)
+_SIMPLE_CALLS = (
+    ("mfa_norm_rope", MfaNormRopeParams, False),
+    ("mfa_norm_rope_bwd", MfaNormRopeBwdParams, True),
+    ("mfa_kv4_append", MfaKv4AppendParams, False),
+    ("mfa_kv4_fwd", MfaKv4FwdParams, True),
+    ("mfa_copy_pages", MfaCopyPagesParams, False),
+)
 
 _lock = threading.Lock()
 _lib = None
@@ -199,6 +297,21 @@ def load():
                 f"mtlflashattn_amd: mfa_fwd_params is {lib.mfa_params_size()} bytes in {path} but "
                 f"{ctypes.sizeof(MfaFwdParams)} in the ctypes mirror; rebuild it"
             )
+        for name, struct, takes_workspace in _SIMPLE_CALLS:
+            if not hasattr(lib, name):
+                raise HipLibraryError(f"mtlflashattn_amd: {path} has no {name}; rebuild it")
+            fn = getattr(lib, name)
+            fn.restype = ctypes.c_int
+            fn.argtypes = [ctypes.POINTER(struct), *([_c_ptr, ctypes.c_int64] if takes_workspace else []), _c_ptr]
+            if takes_workspace:
+                need = getattr(lib, name + "_workspace_bytes")
+                need.restype, need.argtypes = ctypes.c_int64, [ctypes.POINTER(struct)]
+            size = getattr(lib, name + "_params_size")()
+            if size != ctypes.sizeof(struct):
+                raise HipLibraryError(
+                    f"mtlflashattn_amd: {name}_params is {size} bytes in {path} but "
+                    f"{ctypes.sizeof(struct)} in the ctypes mirror; rebuild it"
+                )
         _lib = lib
         return lib
 
@@ -278,6 +391,40 @@ def merge(params: MfaMergeParams, stream: int) -> None:
     rc = lib.mfa_merge(ctypes.byref(params), _c_ptr(stream))
     if rc != MFA_OK:
         raise HipLibraryError(lib.mfa_last_error().decode(errors="replace") or f"mfa_merge failed ({rc})")
+
+
+def _checked(name: str, rc: int) -> int:
+    if rc < 0:
+        raise HipLibraryError(load().mfa_last_error().decode(errors="replace") or f"{name} failed ({rc})")
+    return rc
+
+
+def norm_rope(params: MfaNormRopeParams, stream: int) -> None:
+    _checked("mfa_norm_rope", load().mfa_norm_rope(ctypes.byref(params), stream))
+
+
+def norm_rope_bwd_workspace_bytes(params: MfaNormRopeBwdParams) -> int:
+    return _checked("mfa_norm_rope_bwd_workspace_bytes", load().mfa_norm_rope_bwd_workspace_bytes(ctypes.byref(params)))
+
+
+def norm_rope_bwd(params: MfaNormRopeBwdParams, workspace: int, workspace_bytes_: int, stream: int) -> None:
+    _checked("mfa_norm_rope_bwd", load().mfa_norm_rope_bwd(ctypes.byref(params), workspace, workspace_bytes_, stream))
+
+
+def kv4_append(params: MfaKv4AppendParams, stream: int) -> None:
+    _checked("mfa_kv4_append", load().mfa_kv4_append(ctypes.byref(params), stream))
+
+
+def kv4_fwd_workspace_bytes(params: MfaKv4FwdParams) -> int:
+    return _checked("mfa_kv4_fwd_workspace_bytes", load().mfa_kv4_fwd_workspace_bytes(ctypes.byref(params)))
+
+
+def kv4_fwd(params: MfaKv4FwdParams, workspace: int, workspace_bytes_: int, stream: int) -> None:
+    _checked("mfa_kv4_fwd", load().mfa_kv4_fwd(ctypes.byref(params), workspace, workspace_bytes_, stream))
+
+
+def copy_pages(params: MfaCopyPagesParams, stream: int) -> None:
+    _checked("mfa_copy_pages", load().mfa_copy_pages(ctypes.byref(params), stream))
 
 
 def launch_info(params: MfaFwdParams) -> MfaLaunchInfo:

@@ -145,6 +145,27 @@ def _alibi_arg(alibi_slopes, B, Hq, device):
     return s.to(device=device, dtype=torch.float32).contiguous(), bstride
 
 
+def _check_pages_enabled() -> bool:
+    return os.environ.get("MTLFLASHATTN_CHECK_PAGES", "").lower() in ("1", "on", "true", "yes")
+
+
+def _check_options(window_size, softcap, alibi_slopes):
+    """The window, soft-cap and ALiBi arguments (metal_flash_attn/__init__.py:31-46)."""
+    if (
+        not isinstance(window_size, (tuple, list))
+        or len(window_size) != 2
+        or any(not isinstance(w, int) or isinstance(w, bool) or w < -1 for w in window_size)
+    ):
+        raise ValueError(
+            "mtlflashattn_amd: window_size must be a (left, right) pair of ints >= -1 "
+            "(-1 = unbounded on that side)"
+        )
+    if softcap < 0:
+        raise ValueError("mtlflashattn_amd: softcap must be >= 0 (0 disables capping)")
+    if alibi_slopes is not None and not torch.is_tensor(alibi_slopes):
+        raise TypeError("mtlflashattn_amd: alibi_slopes must be a tensor of per-head slopes")
+
+
 def _check_qkv_shapes(q, k, v, h_axis, s_axis):
     """4-D q/k/v that agree on the batch size, k/v on head count and length,
     and a K/V head count that divides the query head count (CUDA flash-attn

@@ -1,0 +1,411 @@
+"""A paged K/V cache held in 4 bits: writing it, attention over it, and copies of
+its pages.  The reference has no cache (block_table raises,
+metal_flash_attn/__init__.py:130-131); here 16-bit pages are read by
+flash_attn_varlen_func and 4-bit pages, 17/64 of their size, by the functions of
+this module.
+
+Format (include/mfa.h): 32 consecutive elements of a head share one power-of-two
+scale byte and are 4-bit floats (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives).
+A cache of K or V is a pair (codes, scales) of uint8 tensors [num_pages,
+page_block_size, Hkv, D / 2] and [..., D / 32], as kv4_cache makes it.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _hip, _kernel
+from ._kernel import MAX_HEAD_DIM
+
+_ATTEND_DTYPES = (torch.float16, torch.bfloat16)
+
+# prepared parameters (everything but the data pointers) of a call's signature
+_plans = {}
+
+
+def _sig(t):
+    return (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _plan(key, make):
+    plan = _plans.get(key)
+    if plan is None:
+        plan = make()
+        if len(_plans) >= _kernel._PLANS_MAX:
+            _plans.clear()
+        _plans[key] = plan
+    return plan
+
+
+def kv4_cache(num_pages, page_block_size, num_heads_kv, head_dim, device="cuda"):
+    """An empty 4-bit cache of K or of V: (codes, scales).
+
+    codes: uint8 [num_pages, page_block_size, num_heads_kv, head_dim / 2], scales:
+    uint8 [..., head_dim / 32], zeroed (rows read as 0).  In memory each head's
+    rows of a page lie side by side (the heads-third shape is a view), which the
+    kernels read fastest; they take any other order too.  page_block_size: a
+    multiple of 64; head_dim: 32, 64, 96 or 128.
+    """
+    if page_block_size <= 0 or page_block_size % 64:
+        raise ValueError(f"mtlflashattn_amd: page_block_size {page_block_size} must be a positive multiple of 64")
+    if head_dim <= 0 or head_dim % 32 or head_dim > MAX_HEAD_DIM:
+        raise NotImplementedError(f"mtlflashattn_amd: head_dim {head_dim} of a 4-bit cache must be 32, 64, 96 or 128")
+    return tuple(torch.zeros(num_pages, num_heads_kv, page_block_size, n, dtype=torch.uint8, device=device).transpose(1, 2)
+                 for n in (head_dim // 2, head_dim // 32))
+
+
+def _check_tensors(*tensors):
+    """Before a call's signature is formed: everything in its place is a tensor."""
+    if not all(torch.is_tensor(t) for t in tensors):
+        raise ValueError("mtlflashattn_amd: tensors expected")
+
+
+def _check_pairs(k_cache, v_cache):
+    for what, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if not isinstance(c, (tuple, list)) or len(c) != 2 or not (torch.is_tensor(c[0]) and torch.is_tensor(c[1])):
+            raise ValueError(f"mtlflashattn_amd: {what} must be a pair (codes, scales), as kv4_cache makes it")
+
+
+def _check_cache(cache, D, Hkv, device, what):
+    codes, scales = cache
+    if codes.dim() != 4 or scales.dim() != 4 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError(f"mtlflashattn_amd: {what}: codes and scales must be 4-D uint8 tensors")
+    page = codes.shape[1]
+    if page == 0 or page % 64:
+        raise ValueError(f"mtlflashattn_amd: page_block_size {page} must be a positive multiple of 64")
+    if tuple(codes.shape[2:]) != (Hkv, D // 2) or tuple(scales.shape) != (*codes.shape[:3], D // 32):
+        raise ValueError(f"mtlflashattn_amd: {what}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not "
+                         f"hold {Hkv} heads of {D} elements")
+    for t, unit in ((codes, 16), (scales, 1)):
+        if t.device != device:
+            raise ValueError(f"mtlflashattn_amd: tensors on different devices ({device} vs {t.device})")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"mtlflashattn_amd: {what}: the last dimension must be contiguous")
+        if any(s % unit for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1):
+            raise ValueError(f"mtlflashattn_amd: {what}: code strides must be multiples of 16 bytes")
+
+
+def _check_table(block_table, batch, device):
+    if not torch.is_tensor(block_table) or block_table.dim() != 2 or block_table.dtype != torch.int32:
+        raise ValueError("mtlflashattn_amd: block_table must be an int32 [batch, max_pages] tensor")
+    if block_table.shape[0] != batch:
+        raise ValueError(f"mtlflashattn_amd: block_table has {block_table.shape[0]} rows for {batch} sequences")
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        raise ValueError("mtlflashattn_amd: block_table must have contiguous rows")
+    if block_table.device != device:
+        raise ValueError(f"mtlflashattn_amd: tensors on different devices ({device} vs {block_table.device})")
+
+
+def _check_ints(t, n, device, what):
+    if not torch.is_tensor(t) or t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (n,):
+        raise ValueError(f"mtlflashattn_amd: {what} must be an int32 tensor of {n} elements")
+    if t.device != device:
+        raise ValueError(f"mtlflashattn_amd: tensors on different devices ({device} vs {t.device})")
+
+
+def _cache_struct(c, k_cache, v_cache, block_table):
+    """The strides and sizes of a cache."""
+    for pool, (codes, scales) in ((c.k, k_cache), (c.v, v_cache)):
+        pool.code_page_stride, pool.code_row_stride, pool.code_head_stride = (
+            s if n > 1 else 0 for s, n in zip(codes.stride()[:3], codes.shape[:3]))
+        pool.scale_page_stride, pool.scale_row_stride, pool.scale_head_stride = (
+            s if n > 1 else 0 for s, n in zip(scales.stride()[:3], scales.shape[:3]))
+    c.num_pages, c.page_block_size = k_cache[0].shape[:2]
+    c.max_pages = block_table.shape[1]
+    c.block_table_batch_stride = block_table.stride(0) if block_table.shape[0] > 1 else 0
+
+
+def _cache_pointers(c, k_cache, v_cache, block_table):
+    ck, cv = c.k, c.v
+    ck.codes, ck.scales = k_cache[0].data_ptr(), k_cache[1].data_ptr()
+    cv.codes, cv.scales = v_cache[0].data_ptr(), v_cache[1].data_ptr()
+    c.block_table = block_table.data_ptr()
+
+
+def _i32(t):
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+def _check_pages(block_table, lens, page, num_pages):
+    """With MTLFLASHATTN_CHECK_PAGES=1: the page ids that `lens` rows use, on the host."""
+    if not _kernel._check_pages_enabled():
+        return
+    lens = lens.clamp(min=0).cpu()
+    used = torch.arange(block_table.shape[1]).unsqueeze(0) < ((lens + page - 1) // page).unsqueeze(1)
+    if lens.numel() and int(lens.max()) > block_table.shape[1] * page:
+        raise ValueError(f"mtlflashattn_amd: block_table has {block_table.shape[1]} pages per sequence, "
+                         f"too few for {int(lens.max())} rows")
+    ids = block_table.cpu()[used]
+    if ids.numel() and (int(ids.min()) < 0 or int(ids.max()) >= num_pages):
+        raise ValueError(f"mtlflashattn_amd: block_table holds page ids outside [0, {num_pages})")
+
+
+def kv4_append(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, return_values=False):
+    """Write new rows into a paged 4-bit cache, in one launch.
+
+    k, v: [total, Hkv, D] fp16 / bf16 / fp32 rows packed without padding (views are
+    read in place); cu_seqlens: int32 [B + 1], sequence b owning tokens
+    [cu_seqlens[b], cu_seqlens[b + 1]); cache_seqlens: int32 [B], the rows each
+    sequence holds already.  Token t of sequence b becomes row cache_seqlens[b] + t -
+    cu_seqlens[b], which is row j % page_block_size of page block_table[b, j //
+    page_block_size].  cache_seqlens is not changed.  All of them are read on the
+    device (no synchronisation): a row behind the last column of the table or on a
+    page id outside the pool is dropped, as are tokens of no sequence.  No two
+    tokens may land on one row: a page that forked sequences share is copied
+    (copy_cache_pages) before one of them writes to it.
+
+    Each 32 elements take the smallest power-of-two scale that leaves them within 7
+    times it; elements are rounded to the nearest 4-bit value, ties to the even
+    code.  A group with an infinity or a NaN is held as NaN.
+
+    return_values=True returns (k', v') [total, Hkv, D] in k.dtype: the rows as the
+    cache now holds them, for attention over a prompt that later steps will read
+    back from the cache (flash_attn_varlen_func(q, k', v', ...)).  Not
+    differentiable: inputs that require grad raise.
+    """
+    def make():
+        if k.dim() != 3 or v.dim() != 3 or k.shape != v.shape:
+            raise ValueError(f"mtlflashattn_amd: expected k and v [total,H,D], got {tuple(k.shape)} and {tuple(v.shape)}")
+        _kernel._check_device(k, v)
+        if k.dtype not in _kernel._SUPPORTED_DTYPES or v.dtype != k.dtype:
+            raise NotImplementedError(f"mtlflashattn_amd: dtype {k.dtype} (k/v must match, fp16/bf16/fp32)")
+        total, Hkv, D = k.shape
+        if D == 0 or D % 32 or D > MAX_HEAD_DIM:
+            raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} of a 4-bit cache must be 32, 64, 96 or 128")
+        _check_cache(k_cache, D, Hkv, k.device, "k_cache")
+        _check_cache(v_cache, D, Hkv, k.device, "v_cache")
+        if k_cache[0].shape != v_cache[0].shape:
+            raise ValueError("mtlflashattn_amd: k_cache and v_cache differ in pages")
+        batch = cache_seqlens.shape[0] if torch.is_tensor(cache_seqlens) and cache_seqlens.dim() == 1 else 0
+        _check_ints(cache_seqlens, batch, k.device, "cache_seqlens")
+        _check_ints(cu_seqlens, batch + 1, k.device, "cu_seqlens")
+        _check_table(block_table, batch, k.device)
+        p = _hip.MfaKv4AppendParams()
+        _cache_struct(p.cache, k_cache, v_cache, block_table)
+        p.batch, p.total, p.heads_kv, p.head_dim = batch, total, Hkv, D
+        p.dtype = _hip.DTYPE_CODES[k.dtype]
+        return p
+
+    _check_tensors(k, v, cu_seqlens, cache_seqlens, block_table)
+    _check_pairs(k_cache, v_cache)
+    if _kernel._needs_grad(k, v):
+        raise NotImplementedError("mtlflashattn_amd: kv4_append is not differentiable; run it under torch.no_grad() or on "
+                                  "detached rows")
+    key = ("append", _sig(k), _sig(v), *(_sig(t) for c in (k_cache, v_cache) for t in c), _sig(cu_seqlens),
+           _sig(cache_seqlens), _sig(block_table))
+    p = _hip.MfaKv4AppendParams.from_buffer_copy(_plan(key, make))
+    kk, vv, cu, lens = _kernel._abi_operand(k), _kernel._abi_operand(v), _i32(cu_seqlens), _i32(cache_seqlens)
+    _check_pages(block_table, lens + (cu[1:] - cu[:-1]) if _kernel._check_pages_enabled() else lens, k_cache[0].shape[1],
+                 k_cache[0].shape[0])
+    p.k, p.v = kk.data_ptr(), vv.data_ptr()
+    p.k_token_stride, p.k_head_stride = (s if n > 1 else 0 for s, n in zip(kk.stride()[:2], kk.shape[:2]))
+    p.v_token_stride, p.v_head_stride = (s if n > 1 else 0 for s, n in zip(vv.stride()[:2], vv.shape[:2]))
+    _cache_pointers(p.cache, k_cache, v_cache, block_table)
+    p.cu_seqlens, p.cache_seqlens = cu.data_ptr(), lens.data_ptr()
+    values = None
+    if return_values:
+        values = tuple(torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
+        p.k_values, p.v_values = values[0].data_ptr(), values[1].data_ptr()
+    with _kernel._on(k.device):
+        _hip.kv4_append(p, torch._C._cuda_getCurrentRawStream(k.device.index))
+    return values
+
+
+def flash_attn_kv4_func(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale=None, causal=False,
+                        window_size=(-1, -1), softcap=0.0, alibi_slopes=None, max_seqlen_k=None,
+                        return_softmax_lse=False):
+    """Attention of [B, Lq, Hq, D] queries over a paged 4-bit cache.
+
+    q: fp16 or bf16, the last Lq positions of each sequence (Lq = 1: a decoding
+    step; a few: drafted tokens; many: a chunk of a prompt whose rows kv4_append has
+    written).  k_cache, v_cache: (codes, scales) pairs; cache_seqlens: int32 [B], the
+    rows of each sequence in the cache, the queries' own included; block_table: int32
+    [B, max_pages].  Masks, soft-cap, ALiBi, grouped-query heads as in
+    flash_attn_func; rows with no valid key give 0.  Returns [B, Lq, Hq, D] in q.dtype,
+    with return_softmax_lse=True also the log-sum-exp [B, Hq, Lq] fp32.
+
+    Lengths and page ids are read on the device (no synchronisation: a call can be
+    captured into a graph and replayed as the sequences grow).  A sequence has at
+    most max_seqlen_k keys (None: as many as the table names); a tight bound keeps
+    the workspace and the grid small.  A page id outside the pool reads as zeros and
+    its keys are not masked; MTLFLASHATTN_CHECK_PAGES=1 checks the ids on the host.
+    Forward only: a query that requires grad raises.
+    """
+    if torch.is_tensor(q) and q.dim() != 4:
+        raise ValueError(f"mtlflashattn_amd: expected q [B,Lq,H,D], got {q.dim()}-D")
+    return _attend(q, k_cache, v_cache, None, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap,
+                   alibi_slopes, max_seqlen_k, return_softmax_lse)
+
+
+def flash_attn_varlen_kv4_func(q, k_cache, v_cache, cu_seqlens_q, cache_seqlens, block_table, softmax_scale=None,
+                               causal=False, window_size=(-1, -1), softcap=0.0, alibi_slopes=None, max_seqlen_k=None,
+                               return_softmax_lse=False):
+    """flash_attn_kv4_func for sequences of different query counts (a serving step
+    that mixes prompt chunks and decoding sequences).
+
+    q: [total, Hq, D] packed without padding, sequence b owning rows
+    [cu_seqlens_q[b], cu_seqlens_q[b + 1]) (int32 [B + 1], read on the device; it must
+    be non-decreasing).  Rows of no sequence come back as 0.  Returns [total, Hq, D]
+    and, if asked, the log-sum-exp [Hq, total].
+    """
+    if torch.is_tensor(q) and q.dim() != 3:
+        raise ValueError(f"mtlflashattn_amd: expected q [total,H,D], got {q.dim()}-D")
+    return _attend(q, k_cache, v_cache, cu_seqlens_q, cache_seqlens, block_table, softmax_scale, causal, window_size,
+                   softcap, alibi_slopes, max_seqlen_k, return_softmax_lse)
+
+
+def _attend(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap, alibi_slopes,
+            max_seqlen_k, return_lse):
+    _check_tensors(q, cache_seqlens, block_table)
+    _check_pairs(k_cache, v_cache)
+    varlen = q.dim() == 3
+    if varlen:
+        _check_tensors(cu_q)
+
+    def make():
+        _kernel._check_device(q)
+        if q.dtype not in _ATTEND_DTYPES:
+            raise NotImplementedError(f"mtlflashattn_amd: dtype {q.dtype} (queries over a 4-bit cache are fp16 or bf16)")
+        Hq, D = q.shape[-2:]
+        if D not in (32, 64, 96, 128):
+            raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} of a 4-bit cache must be 32, 64, 96 or 128")
+        Hkv = k_cache[0].shape[2] if k_cache[0].dim() == 4 else 0
+        _check_cache(k_cache, D, Hkv, q.device, "k_cache")
+        _check_cache(v_cache, D, Hkv, q.device, "v_cache")
+        if k_cache[0].shape != v_cache[0].shape:
+            raise ValueError("mtlflashattn_amd: k_cache and v_cache differ in pages or heads")
+        if Hkv == 0 or Hq == 0 or Hq % Hkv:
+            raise ValueError(f"mtlflashattn_amd: num_heads_kv ({Hkv}) must divide num_heads_q ({Hq})")
+        if varlen:
+            batch = cache_seqlens.shape[0] if torch.is_tensor(cache_seqlens) and cache_seqlens.dim() == 1 else 0
+            _check_ints(cu_q, batch + 1, q.device, "cu_seqlens_q")
+        else:
+            batch = q.shape[0]
+        _check_ints(cache_seqlens, batch, q.device, "cache_seqlens")
+        _check_table(block_table, batch, q.device)
+        if max_seqlen_k is not None and max_seqlen_k < 0:
+            raise ValueError("mtlflashattn_amd: max_seqlen_k must be >= 0")
+        _kernel._alibi_arg(alibi_slopes, batch, Hq, q.device)
+        p = _hip.MfaKv4FwdParams()
+        _cache_struct(p.cache, k_cache, v_cache, block_table)
+        p.batch, p.heads_q, p.heads_kv, p.head_dim = batch, Hq, Hkv, D
+        if varlen:
+            p.total_q = q.shape[0]
+            p.o_seq_stride, p.o_head_stride = Hq * D, D
+            p.lse_head_stride = q.shape[0]
+        else:
+            p.seqlen_q = q.shape[1]
+            p.o_batch_stride, p.o_seq_stride, p.o_head_stride = q.shape[1] * Hq * D, Hq * D, D
+            p.lse_batch_stride, p.lse_head_stride = Hq * q.shape[1], q.shape[1]
+        cap = block_table.shape[1] * k_cache[0].shape[1]
+        p.max_seqlen_k = cap if max_seqlen_k is None else min(int(max_seqlen_k), cap)
+        if p.max_seqlen_k == 0:  # (0 means no bound to the library)
+            p.cache.max_pages = 0
+        p.scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
+        p.softcap = softcap
+        p.window_left, p.window_right = window_size
+        p.causal = int(bool(causal))
+        p.dtype = _hip.DTYPE_CODES[q.dtype]
+        # placeholders: sizing the workspace reads no tensor
+        p.q = p.o = p.cache_seqlens = p.cache.block_table = 256
+        p.cache.k.codes = p.cache.k.scales = p.cache.v.codes = p.cache.v.scales = 256
+        p.cu_seqlens_q = 256 if varlen else None
+        with _kernel._on(q.device):
+            return p, _hip.kv4_fwd_workspace_bytes(p)
+
+    if _kernel._needs_grad(q):
+        raise NotImplementedError("mtlflashattn_amd: attention over a 4-bit cache is forward-only; run it under "
+                                  "torch.no_grad() or without inputs that require grad")
+    _kernel._check_options(window_size, softcap, alibi_slopes)
+    window_size = tuple(window_size)
+    key = ("attend", _sig(q), *(_sig(t) for c in (k_cache, v_cache) for t in c), cu_q is not None and _sig(cu_q),
+           _sig(cache_seqlens), _sig(block_table), alibi_slopes is not None and _sig(alibi_slopes), softmax_scale,
+           bool(causal), window_size, softcap, max_seqlen_k)
+    template, nbytes = _plan(key, make)
+    if _kernel._trace_enabled():
+        _kernel._record_trace(q.dtype, q.shape[-1], q.shape[0 if varlen else 1], template.max_seqlen_k, causal, "hip-kv4")
+    p = _hip.MfaKv4FwdParams.from_buffer_copy(template)
+    device, qq, lens = q.device, _kernel._abi_operand(q), _i32(cache_seqlens)
+    _check_pages(block_table, lens.clamp(max=template.max_seqlen_k) if _kernel._check_pages_enabled() else lens,
+                 k_cache[0].shape[1], k_cache[0].shape[0])
+    strides = [s if n > 1 else 0 for s, n in zip(qq.stride(), qq.shape)]
+    if varlen:
+        cu = _i32(cu_q)
+        p.cu_seqlens_q = cu.data_ptr()
+        p.q_seq_stride, p.q_head_stride = strides[:2]
+        # (rows of no sequence: the kernels leave them)
+        out = torch.zeros(q.shape, dtype=q.dtype, device=device)
+        lse = torch.full((q.shape[1], q.shape[0]), float("-inf"), device=device) if return_lse else None
+    else:
+        p.q_batch_stride, p.q_seq_stride, p.q_head_stride = strides[:3]
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=device) if return_lse else None
+    p.q, p.o = qq.data_ptr(), out.data_ptr()
+    if lse is not None:
+        p.softmax_lse = lse.data_ptr()
+    if alibi_slopes is not None:
+        slopes, p.alibi_batch_stride = _kernel._alibi_arg(alibi_slopes, p.batch, p.heads_q, device)
+        p.alibi_slopes = slopes.data_ptr()
+    p.cache_seqlens = lens.data_ptr()
+    _cache_pointers(p.cache, k_cache, v_cache, block_table)
+    with _kernel._on(device):
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+        _hip.kv4_fwd(p, ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(device.index))
+    return (out, lse) if return_lse else out
+
+
+def copy_cache_pages(pools, src, dst):
+    """Copy page src[i] to page dst[i] in every pool, in one launch per 64 pools.
+
+    pools: tensors [num_pages, ...] of any dtype that hold one page after another:
+    16-bit K and V pools, (codes, scales) of 4-bit caches, of one layer or many; each
+    page dense in memory (any order of its dimensions).  src, dst: int32 [n] page ids,
+    read on the device (no synchronisation); a pair with an id outside the pools is
+    skipped, so -1 pads a list.  This is what forked sequences (the shared last page is
+    copied before one of them writes to it) and compaction (pages move into free ones)
+    need.  The destinations have to differ from each other and from every source; pairs
+    are copied in no order.  MTLFLASHATTN_CHECK_PAGES=1 checks that on the host and raises
+    ValueError.
+    """
+    pools = list(pools)
+    if not pools:
+        return
+    if not all(torch.is_tensor(t) and t.dim() >= 1 for t in pools):
+        raise ValueError("mtlflashattn_amd: pools must be tensors [num_pages, ...]")
+    _kernel._check_device(*pools)
+    device, num_pages = pools[0].device, pools[0].shape[0]
+    if not torch.is_tensor(src) or src.dim() != 1:
+        raise ValueError("mtlflashattn_amd: src must be an int32 [n] tensor of page ids")
+    _check_ints(src, src.shape[0], device, "src")
+    _check_ints(dst, src.shape[0], device, "dst")
+    if any(t.requires_grad for t in pools) and torch.is_grad_enabled():
+        raise NotImplementedError("mtlflashattn_amd: copy_cache_pages is not differentiable")
+    sizes = []
+    for t in pools:
+        if t.shape[0] != num_pages:
+            raise ValueError(f"mtlflashattn_amd: pools of {num_pages} and {t.shape[0]} pages")
+        n = 1
+        for size, stride in sorted(zip(t.shape[1:], t.stride()[1:]), key=lambda x: x[1]):
+            if size > 1 and stride != n:
+                raise ValueError("mtlflashattn_amd: the pages of a pool must be dense in memory")
+            n *= size
+        if num_pages > 1 and n and t.stride(0) < n:
+            raise ValueError("mtlflashattn_amd: the pages of a pool must not overlap")
+        sizes.append(n * t.element_size())
+    src, dst = _i32(src), _i32(dst)
+    if _kernel._check_pages_enabled():
+        pairs = [(a, b) for a, b in zip(src.tolist(), dst.tolist()) if 0 <= a < num_pages and 0 <= b < num_pages and a != b]
+        to = [b for _, b in pairs]
+        if len(set(to)) != len(to) or set(to) & {a for a, _ in pairs}:
+            raise ValueError("mtlflashattn_amd: copy_cache_pages: a destination is given twice or is a source too")
+    with _kernel._on(device):
+        stream = torch._C._cuda_getCurrentRawStream(device.index)
+        for first in range(0, len(pools), _hip.MFA_COPY_MAX_POOLS):
+            p = _hip.MfaCopyPagesParams()
+            part = pools[first:first + _hip.MFA_COPY_MAX_POOLS]
+            for i, t in enumerate(part):
+                p.pool[i] = (t.data_ptr(), t.stride(0) * t.element_size() if num_pages > 1 else 0, sizes[first + i])
+            p.src, p.dst = src.data_ptr(), dst.data_ptr()
+            p.pools, p.pairs, p.num_pages = len(part), src.shape[0], num_pages
+            _hip.copy_pages(p, stream)

@@ -1,0 +1,194 @@
+"""RMS norm of query and key heads and the rotation of their positions in one HIP
+pass (mfa_norm_rope), with its backward.  The reference has no counterpart: its
+callers normalise and rotate with elementwise framework ops before the attention
+call."""
+from __future__ import annotations
+
+import torch
+
+from . import _hip, _kernel
+from ._kernel import MAX_HEAD_DIM
+
+_DTYPES = _kernel._SUPPORTED_DTYPES
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, interleaved=False):
+    """Norm and rotation of every query and key head, in one launch.
+
+    q: [B, L, Hq, D] (or packed [T, Hq, D]), k: [B, L, Hkv, D] ([T, Hkv, D]),
+    fp16 / bf16 / fp32, any strides (views of a packed projection are read in
+    place).  Returns (q', k'), contiguous, in the same dtype:
+
+      n = x / sqrt(mean(x^2) + eps),  y = n * weight
+      y_a cos - y_b sin, y_b cos + y_a sin    for each pair (a, b) of the rotated part
+
+    q_weight, k_weight: [D] of any of the three dtypes (the same one), or None (1).
+    cos, sin: [rows, rotary_dim / 2] tables in q.dtype or fp32; the pairs are
+    (i, i + rotary_dim / 2) of the first rotary_dim <= D elements, or (2i, 2i + 1)
+    with interleaved=True; the elements behind are normalised only.
+    positions: int32 / int64 rows of the tables, [B, L] ([T]) or [L]; None: 0, 1,
+    2, ... in each sequence.  They are read on the device: a position outside the
+    tables gives NaN in the rotated elements (never a read out of bounds).
+    Arithmetic is fp32, rounded once.  Differentiable in q, k and the weights
+    (weight gradients are summed in fp32 in a fixed order: the same bits every
+    time); cos and sin are constants.
+    """
+    template = _signature(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    if _kernel._needs_grad(q, k) or (torch.is_grad_enabled() and any(
+            w is not None and w.requires_grad for w in (q_weight, k_weight))):
+        return _QkNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    return _forward(template, q, k, q_weight, k_weight, cos, sin, positions)
+
+
+# prepared parameters (everything but the data pointers) of a call's signature
+_plans = {}
+
+
+def _sig(t):
+    try:
+        return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+    except AttributeError:
+        raise ValueError(f"mtlflashattn_amd: a tensor expected, got {type(t).__name__}") from None
+
+
+def _signature(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    """The parameter template of a call, its arguments checked at their first use."""
+    if cos is None or sin is None or q is None or k is None:
+        raise ValueError("mtlflashattn_amd: q, k, cos and sin are required")
+    key = (_sig(q), _sig(k), _sig(q_weight), _sig(k_weight), _sig(cos), _sig(sin), _sig(positions), eps, interleaved)
+    template = _plans.get(key)
+    if template is None:
+        template = _prepare(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+        if len(_plans) >= _kernel._PLANS_MAX:
+            _plans.clear()
+        _plans[key] = template
+    if cos.requires_grad or sin.requires_grad:
+        raise NotImplementedError("mtlflashattn_amd: cos and sin are constants (no gradient)")
+    return template
+
+
+def _check(q, k, q_weight, k_weight, cos, sin, positions, eps):
+    if q.dim() not in (3, 4) or k.dim() != q.dim():
+        raise ValueError(f"mtlflashattn_amd: expected q and k [B,L,H,D] or [T,H,D], got {q.dim()}-D and {k.dim()}-D")
+    _kernel._check_device(q, k)
+    if q.dtype not in _DTYPES or k.dtype != q.dtype:
+        raise NotImplementedError(f"mtlflashattn_amd: dtype {q.dtype} (q/k must match, fp16/bf16/fp32)")
+    D = q.shape[-1]
+    if D > MAX_HEAD_DIM or D == 0:
+        raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} outside [1, {MAX_HEAD_DIM}]")
+    if k.shape[-1] != D or k.shape[:-2] != q.shape[:-2]:
+        raise ValueError(f"mtlflashattn_amd: q {tuple(q.shape)} and k {tuple(k.shape)} differ in tokens or head_dim")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    for w in weights:
+        if tuple(w.shape) != (D,) or w.dtype not in _DTYPES or w.dtype != weights[0].dtype:
+            raise ValueError(f"mtlflashattn_amd: norm weights must be [{D}] tensors of one fp16/bf16/fp32 dtype")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.dtype not in (q.dtype, torch.float32):
+        raise ValueError("mtlflashattn_amd: cos and sin must be [rows, rotary_dim / 2] tables in q.dtype or fp32")
+    if 2 * cos.shape[1] > D:
+        raise ValueError(f"mtlflashattn_amd: rotary_dim {2 * cos.shape[1]} > head_dim {D}")
+    if positions is not None:
+        if not torch.is_tensor(positions) or positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError("mtlflashattn_amd: positions must be an int32 or int64 tensor")
+        if positions.shape not in (q.shape[:-2], q.shape[-3:-2]):
+            raise ValueError(f"mtlflashattn_amd: positions {tuple(positions.shape)} must be {tuple(q.shape[:-2])} or "
+                             f"{tuple(q.shape[-3:-2])}")
+    if not eps >= 0:
+        raise ValueError("mtlflashattn_amd: eps must be >= 0")
+    _kernel._check_device(q, *weights, cos, sin, *([positions] if positions is not None else []))
+
+
+def _strides(t):
+    """(batch, token, head) element strides of [B, L, H, D] or [T, H, D]; 0 for size-1 dims."""
+    st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
+    return (0, st[0], st[1]) if len(st) == 3 else tuple(st[:3])
+
+
+def _rows(t):
+    """t with a contiguous last dim."""
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _prepare(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    _check(q, k, q_weight, k_weight, cos, sin, positions, eps)
+    p = _hip.MfaNormRopeParams()
+    q, k, cos, sin, positions = (_rows(t) for t in (q, k, cos, sin, positions))
+    p.q_batch_stride, p.q_seq_stride, p.q_head_stride = _strides(q)
+    p.k_batch_stride, p.k_seq_stride, p.k_head_stride = _strides(k)
+    if cos.stride(0) != sin.stride(0):
+        cos, sin = cos.contiguous(), sin.contiguous()
+    p.table_stride = cos.stride(0) if cos.shape[0] > 1 else 0
+    p.batch, p.seqlen = (q.shape[0], q.shape[1]) if q.dim() == 4 else (1, q.shape[0])
+    p.heads_q, p.heads_kv, p.head_dim = q.shape[-2], k.shape[-2], q.shape[-1]
+    p.rotary_dim, p.table_rows = 2 * cos.shape[1], cos.shape[0]
+    if positions is not None:
+        p.positions_64 = int(positions.dtype == torch.int64)
+        p.positions_batch_stride = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
+    p.interleaved = int(bool(interleaved))
+    p.dtype = _hip.DTYPE_CODES[q.dtype]
+    w = q_weight if q_weight is not None else k_weight
+    p.dtype_weight = _hip.DTYPE_CODES[w.dtype if w is not None else q.dtype]
+    p.dtype_table = _hip.DTYPE_CODES[cos.dtype]
+    p.eps = eps
+    return p
+
+
+def _fill(p, q, k, q_weight, k_weight, cos, sin, positions):
+    """Sets the data pointers; returns the tensors they point into."""
+    held = tuple(_rows(t) for t in (q, k, q_weight, k_weight, cos, sin, positions))
+    q, k, q_weight, k_weight, cos, sin, positions = held
+    if cos.stride(0) != sin.stride(0):
+        cos, sin = cos.contiguous(), sin.contiguous()
+    p.q, p.k = q.data_ptr(), k.data_ptr()
+    p.q_weight = None if q_weight is None else q_weight.data_ptr()
+    p.k_weight = None if k_weight is None else k_weight.data_ptr()
+    p.cos, p.sin = cos.data_ptr(), sin.data_ptr()
+    p.positions = None if positions is None else positions.data_ptr()
+    return held, cos, sin
+
+
+def _forward(template, q, k, q_weight, k_weight, cos, sin, positions):
+    p = _hip.MfaNormRopeParams.from_buffer_copy(template)
+    held = _fill(p, q, k, q_weight, k_weight, cos, sin, positions)  # noqa: F841 (kept until the launch)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    p.q_out, p.k_out = q_out.data_ptr(), k_out.data_ptr()
+    with _kernel._on(q.device):
+        _hip.norm_rope(p, torch._C._cuda_getCurrentRawStream(q.device.index))
+    return q_out, k_out
+
+
+class _QkNormRopeFn(torch.autograd.Function):
+    """qk_norm_rope with the HIP backward, which forms the statistics again from
+    q and k (nothing but the inputs is kept)."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+        template = _signature(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.template = template
+        return _forward(template, q, k, q_weight, k_weight, cos, sin, positions)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+        b = _hip.MfaNormRopeBwdParams()
+        b.fwd = ctx.template
+        held = _fill(b.fwd, q, k, q_weight, k_weight, cos, sin, positions)  # noqa: F841 (kept until the launch)
+        dq_out, dk_out = _rows(dq_out.to(q.dtype)), _rows(dk_out.to(k.dtype))
+        b.dq_out, b.dk_out = dq_out.data_ptr(), dk_out.data_ptr()
+        b.dqo_batch_stride, b.dqo_seq_stride, b.dqo_head_stride = _strides(dq_out)
+        b.dko_batch_stride, b.dko_seq_stride, b.dko_head_stride = _strides(dk_out)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        b.dq, b.dk = dq.data_ptr(), dk.data_ptr()
+        dw = [None, None]
+        for i, w in enumerate((q_weight, k_weight)):
+            if w is not None and ctx.needs_input_grad[2 + i]:
+                dw[i] = torch.empty(w.shape, dtype=w.dtype, device=w.device)
+        b.dq_weight, b.dk_weight = (None if d is None else d.data_ptr() for d in dw)
+        with _kernel._on(q.device):
+            nbytes = _hip.norm_rope_bwd_workspace_bytes(b)
+            ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=q.device)
+            _hip.norm_rope_bwd(b, ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(q.device.index))
+        return dq, dk, dw[0], dw[1], None, None, None, None, None
