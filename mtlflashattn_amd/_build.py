@@ -28,6 +28,7 @@ SRCS = [
     (os.path.join(PKG_DIR, "csrc", "mfa_norm_rope.hip"), []),
     (os.path.join(PKG_DIR, "csrc", "mfa_kv4.hip"), []),
     (os.path.join(PKG_DIR, "csrc", "mfa_kv4_attend.hip"), ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]),
+    (os.path.join(PKG_DIR, "csrc", "mfa_kv4_tile.hip"), ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]),
     (os.path.join(PKG_DIR, "csrc", "mfa_pages.hip"), []),
 ]
 INCLUDE = os.path.join(REPO_DIR, "include")

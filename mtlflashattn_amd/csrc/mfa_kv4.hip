@@ -159,9 +159,10 @@ int mfa_kv4_check_cache(const mfa_kv4_cache* c, int head_dim, const char* who) {
             return aerr(MFA_ERR_INVALID, "%s: code strides must be multiples of 16 bytes", who);
         if (p->code_row_stride < 0 || p->code_head_stride < 0 || p->scale_row_stride < 0 || p->scale_head_stride < 0)
             return aerr(MFA_ERR_INVALID, "%s: row and head strides must be >= 0", who);
-        // (32-key blocks are addressed with 32-bit byte offsets)
-        if (31 * p->code_row_stride + head_dim >= (1LL << 31) || 31 * p->scale_row_stride + head_dim >= (1LL << 31))
-            return aerr(MFA_ERR_INVALID, "%s: 32 rows must span less than 2 GiB", who);
+        // (a page's rows are addressed with 32-bit byte offsets)
+        if (c->page_block_size * p->code_row_stride + head_dim >= (1LL << 31) ||
+            c->page_block_size * p->scale_row_stride + head_dim >= (1LL << 31))
+            return aerr(MFA_ERR_INVALID, "%s: the rows of a page must span less than 2 GiB", who);
     }
     return MFA_OK;
 }
