@@ -434,10 +434,10 @@ int mfa_kv4_append_params_size(void);
  * keys, read on the device; max_seqlen_k 0 leaves the bound out.  Queries: q
  * [batch, seqlen_q, heads_q, head_dim], or with cu_seqlens_q q [total_q, heads_q,
  * head_dim], sequence b owning tokens [cu_seqlens_q[b], cu_seqlens_q[b + 1])
- * (tokens of no sequence are left unwritten).  The query rows are the last
+ * (tokens of no sequence get 0, lse -inf).  The query rows are the last
  * positions of their sequence.  q and o: fp16 or bf16, 16-byte aligned, strides
  * multiples of 8 elements.  head_dim: 32, 64, 96 or 128.
- * Enqueues one or two kernels; never synchronizes, never allocates.  The results
+ * Enqueues up to three kernels; never synchronizes, never allocates.  The results
  * do not depend on the workspace's address or content; they may differ in the
  * last bit with the batch a sequence stands in (its keys are dealt over
  * workgroups with the others').

@@ -13,6 +13,12 @@ constexpr int kThreads4 = 256;
 constexpr int kChunk4 = 128;  // keys per chunk, the unit of dealt work
 constexpr float kLn2f = 0.6931471805599453f;
 
+// What the merge kernel adds for workgroup w: the parts of workgroups w - 1 to w1
+// (-1: nothing) of a unit, whose first part is in slot0.
+struct Merge4 {
+    int32_t w1, slot0, b, q0, hkv, col0, ncol, pad;
+};
+
 struct K4Args {
     const char* q;
     char* o;
@@ -37,14 +43,15 @@ struct K4Args {
     int32_t min_cols, max_cols;  // a sequence with fewer or more columns is another launch's
     float* ws_o;     // [G][2][cols][D]
     float* ws_ml;    // [G][2][cols][2] exponent reference, sum of p
+    Merge4* ws_merge;  // [G], NULL: no unit is walked by more than one workgroup
 };
 
 // The kernels read their arguments where they need them, through a pointer that
 // the compiler cannot see through: all of them in scalar registers at once are
 // more than there are, and the spills land in the inner loop.
 typedef const __attribute__((address_space(4))) K4Args K4Const;
-__device__ __forceinline__ K4Const& args4() {
-    K4Const* p = (K4Const*)__builtin_amdgcn_kernarg_segment_ptr();
+__device__ __forceinline__ K4Const& args4(int which = 0) {
+    K4Const* p = (K4Const*)__builtin_amdgcn_kernarg_segment_ptr() + which;
     asm volatile("" : "+s"(p));
     return *p;
 }
@@ -117,9 +124,34 @@ struct Walk4 {
     int b, before;  // sequence of item x, items before that sequence
     Seq4 sq;
 
-    // false: no items
+    // of this workgroup; false: no items
     __device__ __forceinline__ bool start() {
         K4Const& a = args4();
+        w = blockIdx.x;
+        if (a.xcds > 1) w = (w % a.xcds) * (a.G / a.xcds) + w / a.xcds;  // (neighbours share an XCD)
+        const bool some = find(a);
+        if (a.ws_merge && threadIdx.x == 0) {
+            // the unit of the first item is merged here where it began in the
+            // walk of the workgroup before
+            Merge4 g{-1, 0, 0, 0, 0, 0, 0, 0};
+            if (some && w > 0) {
+                const int off = x - before, unit = off / sq.chunks, x0 = before + unit * sq.chunks;
+                const int first = first_item(w - 1, C, G);
+                if (x0 < x && wg_of_item(x0, C, G) == w - 1) {
+                    g.w1 = wg_of_item(x0 + sq.chunks - 1, C, G);
+                    g.slot0 = first >= x0 ? 0 : 1;
+                    g.b = b;
+                    g.q0 = sq.q0;
+                    g.hkv = unit / sq.tiles;
+                    g.col0 = (unit - g.hkv * sq.tiles) * a.cols;
+                    g.ncol = min(a.cols, sq.Lq * a.R - g.col0);
+                }
+            }
+            a.ws_merge[w] = g;
+        }
+        return some;
+    }
+    __device__ __forceinline__ bool find(K4Const& a) {
         const int lane = threadIdx.x & 63, B = a.B;
         // (one pass where the sequences fit a wavefront)
         Seq4 s{0, 0, 0, 0, 1};
@@ -131,8 +163,6 @@ struct Walk4 {
             C += __builtin_amdgcn_readlane(scan64(y), 63);
         }
         G = min(a.G, C);  // (every workgroup below G has an item: the merge reads them all)
-        w = blockIdx.x;
-        if (a.xcds > 1) w = (w % a.xcds) * (a.G / a.xcds) + w / a.xcds;  // (neighbours share an XCD)
         if (w >= G) return false;
         xbeg = x = first_item(w, C, G);
         xend = first_item(w + 1, C, G);

@@ -104,6 +104,26 @@ __device__ __forceinline__ void load_block4(Block4<DP>& w, const __amdgpu_buffer
     }
 }
 
+// Query rows of no sequence (varlen): 0 and -inf.
+template <int DP>
+__device__ __forceinline__ void clear_rest() {
+    K4Const& a = args4();
+    if (!a.cu_q) return;
+    const int rows = a.rows_q, first = min(max(a.cu_q[0], 0), rows), end = min(max(a.cu_q[a.B], 0), rows);
+    for (int r = 0; r < rows; ++r) {
+        if (r >= first && r < end) {
+            r = end - 1;
+            continue;
+        }
+        for (int x = threadIdx.x; x < a.Hq * (DP / 8); x += kThreads4) {
+            const int h = x / (DP / 8), d = 8 * (x - h * (DP / 8));
+            *reinterpret_cast<u32x4_t*>(a.o + (r * a.os + h * a.oh + d) * 2) = u32x4_t{0, 0, 0, 0};
+        }
+        if (a.lse)
+            for (int h = threadIdx.x; h < a.Hq; h += kThreads4) a.lse[r + h * a.lse_h] = -INFINITY;
+    }
+}
+
 #ifndef MFA_KV4_NT
 #define MFA_KV4_NT 0
 #endif
@@ -132,6 +152,7 @@ mfa_kv4_kernel(K4Args) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, grp = lane >> 4;
+    if (blockIdx.x == gridDim.x - 1) clear_rest<DP>();
     Walk4 wk;
     if (!wk.start()) return;
 
@@ -453,98 +474,92 @@ mfa_kv4_kernel(K4Args) {
     }
 }
 
-// Sum of a row's parts in the order of its keys, one wavefront per (row, query
-// head): 32 lanes hold four elements each, and the halves take every other part.
+// The parts of a unit that several workgroups walked, added in the order of its
+// keys: block (w, z) takes kMergeCols columns of the unit whose walk workgroup w is
+// the first to go on with.  Up to two launches' units in one (blocks of the first,
+// then of the second); a thread holds four elements of a column, and where there
+// are few of them (one or a few columns) groups of threads take every P-th part.
+// Bound by the latency of its loads: a part's reference, sum and elements are
+// loaded at once (no pass for the largest reference first), N parts at a time.
+constexpr int kMergeCols = 8;
 template <int DP, bool IS_BF16>
-__global__ void __launch_bounds__(64) mfa_kv4_merge_kernel(K4Args) {
-    K4Const& a = args4();
-    const int lane = threadIdx.x, half = lane >> 5, d = 4 * (lane & 31);
-    const int row = blockIdx.x / a.Hq, h = blockIdx.x - row * a.Hq;
-    const int hkv = h / a.R, B = a.B;
-    int b, i;
-    if (a.cu_q) {
-        // the sequence of this row: the last whose rows begin at or before it
-        b = -1;
-        for (int b0 = 0; b0 < B; b0 += 64) {
-            const uint64_t at = __ballot(b0 + lane < B && a.cu_q[min(b0 + lane, B - 1)] <= row);
-            if (!at) break;
-            b = b0 + 63 - __builtin_clzll(at);
-        }
-        b = __builtin_amdgcn_readfirstlane(b);
-        if (b < 0) return;
-        i = row - a.cu_q[b];
-    } else {
-        b = row / a.Lq;
-        i = row - b * a.Lq;
-    }
-    // its unit's items, of all
-    int C = 0, before = 0;
-    Seq4 sq;
-    for (int b0 = 0; b0 < B; b0 += 64) {
-        Seq4 s{0, 0, 0, 0, 1};
-        if (b0 + lane < B) s = seq4(a, b0 + lane);
-        const int n = s.items(a.Hkv), inc = scan64(n);
-        if (b >= b0 && b < b0 + 64) {
-            sq = lane_seq4(s, b - b0);
-            before = C + __builtin_amdgcn_readlane(inc - n, b - b0);
-        }
-        C += __builtin_amdgcn_readlane(inc, 63);
-    }
-    if (i < 0 || i >= sq.Lq || sq.tiles == 0) return;  // (rows of no sequence, or of another launch's)
-    const int G = min(a.G, C);
-    const int col = i * a.R + h - hkv * a.R, tile = col / a.cols;
-    const int x0 = before + (hkv * sq.tiles + tile) * sq.chunks;
-    const int w0 = wg_of_item(x0, C, G), w1 = wg_of_item(x0 + sq.chunks - 1, C, G);
-    if (w0 == w1) return;  // (stored by the workgroup that walked it)
-    const int cc = col - tile * a.cols;
-    // the part of workgroup w: its first unit, unless it began before this one
-    const int slot0 = first_item(w0, C, G) >= x0 ? 0 : 1;
-    auto at = [&](int w) { return ((int64_t)w * 2 + (w == w0 ? slot0 : 0)) * a.cols + cc; };
-    float m = -INFINITY;
-    for (int w = w0 + lane; w <= w1; w += 64) m = fmax_nn(m, a.ws_ml[2 * at(w)]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmax_nn(m, __shfl_xor(m, o));
+__global__ void __launch_bounds__(kThreads4) mfa_kv4_merge_kernel(K4Args, K4Args) {
+    __shared__ f32x4_t o_s[kThreads4];
+    __shared__ float2 ml_s[kThreads4];
+    const int tid = threadIdx.x;
+    const int first = args4(0).ws_merge ? args4(0).G * (args4(0).cols / kMergeCols) : 0;
+    const int which = __builtin_amdgcn_readfirstlane((int)blockIdx.x >= first);
+    K4Const& a = args4(which);
+    const int cols = a.cols, blk = blockIdx.x - (which ? first : 0), w = blk / (cols / kMergeCols);
+    const int cbeg = (blk - w * (cols / kMergeCols)) * kMergeCols;  // first of this block's columns
+    const Merge4 g4 = a.ws_merge[w];
+    const int w0 = w - 1, w1 = g4.w1, ncol = min(kMergeCols, g4.ncol - cbeg), items = ncol * (DP / 4);
+    if (w1 < 0 || ncol <= 0) return;
+    // the part of workgroup v: its first unit, unless it began before this one
+    auto at = [&](int v) { return ((int64_t)v * 2 + (v == w0 ? g4.slot0 : 0)) * cols + cbeg; };
+    const int P = items <= 32 ? 8 : items <= 64 ? 4 : items <= 128 ? 2 : 1, S = kThreads4 / P;
+    const int g = tid / S, it = tid - g * S;  // (a round holds every item)
+    const bool in = it < items;
+    const int r = in ? it / (DP / 4) : 0, d = in ? 4 * (it - r * (DP / 4)) : 0;
+    const float* ws_o = a.ws_o;
+    const float* ws_ml = a.ws_ml;
+    float m = -INFINITY, l = 0.f;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    const bool in = d < DP;
-    // (eight parts' loads in flight)
-    for (int v0 = w0; v0 <= w1; v0 += 16) {
-        float2 ml[8];
-        f32x4_t y[8];
+    auto add = [&](float mw, float lw, const f32x4_t& y) {
+        const float mn = fmax_nn(m, mw), e0 = pow2_diff(m, mn), e1 = pow2_diff(mw, mn);
+        l = fmaf(lw, e1, l * e0);
 #pragma unroll
-        for (int z = 0; z < 8; ++z) {
-            const int64_t r = at(min(v0 + 2 * z + half, w1));
-            ml[z] = *reinterpret_cast<const float2*>(a.ws_ml + 2 * r);
-            y[z] = *reinterpret_cast<const f32x4_t*>(a.ws_o + r * DP + (in ? d : 0));
-        }
+        for (int k = 0; k < 4; ++k) acc[k] = fmaf(y[k], e1, acc[k] * e0);
+        m = mn;
+    };
+    auto walk = [&](auto ahead) {
+        constexpr int N = decltype(ahead)::value;
+        for (int v0 = w0 + g; v0 <= w1; v0 += P * N) {
+            float2 ml[N];
+            f32x4_t y[N];
 #pragma unroll
-        for (int z = 0; z < 8; ++z) {
-            if (v0 + 2 * z + half <= w1) {
-                const float e = pow2_diff(ml[z].x, m);
-                l = fmaf(ml[z].y, e, l);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[k] = fmaf(y[z][k], e, acc[k]);
+            for (int z = 0; z < N; ++z) {
+                const int64_t row = at(min(v0 + P * z, w1)) + r;
+                ml[z] = *reinterpret_cast<const float2*>(ws_ml + 2 * row);
+                y[z] = *reinterpret_cast<const f32x4_t*>(ws_o + row * DP + d);
             }
-        }
-    }
-    l = sum_halves(l);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] = sum_halves(acc[k]);
-    if (in && half == 0) store_row4<IS_BF16>(a.o + row_off4(a.cu_q != nullptr, b, sq.q0, i, h, a.ob, a.os, a.oh) * 2, d, acc, l);
-    if (lane == 0) store_lse4(a, b, sq.q0, i, h, m, l);
+            for (int z = 0; z < N; ++z)
+                if (v0 + P * z <= w1) add(ml[z].x, ml[z].y, y[z]);
+        }
+    };
+    if (w1 - w0 + 1 <= 2 * P)
+        walk(std::integral_constant<int, 2>{});
+    else
+        walk(std::integral_constant<int, 8>{});
+    if (P > 1) {
+        o_s[tid] = acc;
+        ml_s[tid] = make_float2(m, l);
+        __syncthreads();
+        if (g > 0) return;
+        for (int z = 1; z < P; ++z) add(ml_s[tid + z * S].x, ml_s[tid + z * S].y, o_s[tid + z * S]);
+    }
+    if (in) {
+        const int col = g4.col0 + cbeg + r, i = (int)div4(col, a.by_r), h = g4.hkv * a.R + col - i * a.R;
+        store_row4<IS_BF16>(a.o + row_off4(a.cu_q != nullptr, g4.b, g4.q0, i, h, a.ob, a.os, a.oh) * 2, d, acc, l);
+        if (d == 0) store_lse4(a, g4.b, g4.q0, i, h, m, l);
+    }
 }
+static_assert(kMergeCols * (MFA_MAX_HEAD_DIM / 4) <= kThreads4, "a thread per four elements");
 
 typedef void (*k4_fn)(K4Args);
 #ifndef MFA_KV4_WGS
 #define MFA_KV4_WGS 2
 #endif
+typedef void (*k4_merge_fn)(K4Args, K4Args);
 struct K4Kernels {
-    k4_fn attend, merge;
+    k4_fn attend;
+    k4_merge_fn merge;
 };
 // cols: columns of a unit, 16, 32 or kTileCols4
 template <int DP, bool IS_BF16>
 K4Kernels kernels4(int cols, bool bias) {
-    const k4_fn merge = mfa_kv4_merge_kernel<DP, IS_BF16>;
+    const k4_merge_fn merge = mfa_kv4_merge_kernel<DP, IS_BF16>;
     if (cols == 16) return {mfa_kv4_kernel<DP, 1, IS_BF16>, merge};
     if (cols == 32) return {mfa_kv4_kernel<DP, 2, IS_BF16>, merge};
     return {(k4_fn)mfa_kv4_tile_kernel_of(DP, IS_BF16, bias), merge};
@@ -575,10 +590,14 @@ struct K4Launch {
     K4Args a;
     int64_t parts;  // rows of its partial results, 0: no merge
 };
+// workspace of a launch: parts, their references and sums, what is merged
+int64_t part_bytes(const K4Launch& l, int D) {
+    return l.parts ? (l.parts * (D * 4 + 8) + (int64_t)l.a.G * sizeof(Merge4) + 255) / 256 * 256 : 0;
+}
 struct K4Plan {
     K4Launch l[2];
     int n = 0;
-    int64_t rows = 0, ws_bytes = 0;
+    int64_t ws_bytes = 0;
 };
 
 int k4_plan(const mfa_kv4_fwd_params* p, K4Plan* plan, int cus) {
@@ -653,7 +672,6 @@ int k4_plan(const mfa_kv4_fwd_params* p, K4Plan* plan, int cus) {
     // 16 columns, another the longer ones.
     const int64_t cols = (varlen ? rows : p->seqlen_q) * (int64_t)a.R;
     plan->n = varlen && cols > 16 ? 2 : 1;
-    plan->rows = rows;
     const int64_t chunks = std::max<int64_t>(1, ((int64_t)a.max_k + kChunk4 - 1) / kChunk4);
     for (int i = 0; i < plan->n; ++i) {
         K4Launch& l = plan->l[i];
@@ -671,7 +689,7 @@ int k4_plan(const mfa_kv4_fwd_params* p, K4Plan* plan, int cus) {
         // (neighbouring tiles of a K/V head share its rows in their XCD's L2)
         l.a.xcds = l.a.cols == kTileCols4 && l.a.G % 8 == 0 ? 8 : 1;
         l.parts = chunks > 1 ? (int64_t)l.a.G * 2 * l.a.cols : 0;
-        plan->ws_bytes += (l.parts * (D * 4 + 8) + 255) / 256 * 256;
+        plan->ws_bytes += part_bytes(l, D);
     }
     return MFA_OK;
 }
@@ -703,16 +721,22 @@ int mfa_kv4_fwd(const mfa_kv4_fwd_params* p, void* workspace, int64_t workspace_
     }
     const hipStream_t st = static_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
+    K4Kernels k{};
+    int merge = 0;
     for (int i = 0; i < plan.n; ++i) {
         K4Launch& l = plan.l[i];
-        const bool a_bias = l.a.bias != 0;
-        const K4Kernels k = p->dtype == MFA_DTYPE_BF16 ? kernels4<true>(p->head_dim, l.a.cols, a_bias) : kernels4<false>(p->head_dim, l.a.cols, a_bias);
-        l.a.ws_o = reinterpret_cast<float*>(ws);
-        l.a.ws_ml = l.a.ws_o + l.parts * p->head_dim;
-        ws += (l.parts * (p->head_dim * 4 + 8) + 255) / 256 * 256;
+        const bool bias = l.a.bias != 0;
+        k = p->dtype == MFA_DTYPE_BF16 ? kernels4<true>(p->head_dim, l.a.cols, bias) : kernels4<false>(p->head_dim, l.a.cols, bias);
+        if (l.parts) {
+            l.a.ws_o = reinterpret_cast<float*>(ws);
+            l.a.ws_ml = l.a.ws_o + l.parts * p->head_dim;
+            l.a.ws_merge = reinterpret_cast<Merge4*>(l.a.ws_ml + l.parts * 2);
+            ws += part_bytes(l, p->head_dim);
+            merge += l.a.G * (l.a.cols / kMergeCols);
+        }
         hipLaunchKernelGGL(k.attend, dim3(l.a.G), dim3(kThreads4), 0, st, l.a);
-        if (l.parts) hipLaunchKernelGGL(k.merge, dim3((unsigned)(plan.rows * l.a.Hq)), dim3(64), 0, st, l.a);
     }
+    if (merge) hipLaunchKernelGGL(k.merge, dim3(merge), dim3(kThreads4), 0, st, plan.l[0].a, plan.l[plan.n - 1].a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return k4err(MFA_ERR_LAUNCH, "mfa_kv4_fwd: launch failed: %s", hipGetErrorString(e));
     return MFA_OK;

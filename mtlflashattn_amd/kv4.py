@@ -334,9 +334,12 @@ def _attend(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale
         cu = _i32(cu_q)
         p.cu_seqlens_q = cu.data_ptr()
         p.q_seq_stride, p.q_head_stride = strides[:2]
-        # (rows of no sequence: the kernels leave them)
-        out = torch.zeros(q.shape, dtype=q.dtype, device=device)
-        lse = torch.full((q.shape[1], q.shape[0]), float("-inf"), device=device) if return_lse else None
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=device) if return_lse else None
+        if p.batch == 0:  # (nothing is launched)
+            out.zero_()
+            if return_lse:
+                lse.fill_(float("-inf"))
     else:
         p.q_batch_stride, p.q_seq_stride, p.q_head_stride = strides[:3]
         out = torch.empty(q.shape, dtype=q.dtype, device=device)
