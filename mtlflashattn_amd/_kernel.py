@@ -401,12 +401,25 @@ def _prepare(q, k, v, out, batch, Hq, Hkv, Lq, Lk, Dp, varlen, scale, causal, so
     return p, chunk, nbytes
 
 
+_NO_CONTEXT = contextlib.nullcontext()
+
+
 def _on(device):
     """Context with `device`, a call's, as the current one: the library plans for
     the current device's CU count."""
     if device.type != "cuda" or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _NO_CONTEXT
     return torch.cuda.device(device)
+
+
+def _launch_on(device, launch, p, *workspace):
+    """launch(p, *workspace, stream) on `device` and its current stream."""
+    idx = device.index
+    if device.type == "cuda" and idx != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            launch(p, *workspace, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        launch(p, *workspace, torch._C._cuda_getCurrentRawStream(idx))
 
 
 def _split_and_workspace(p, dtype, hint, device):

@@ -6,7 +6,10 @@
 // wavefronts owns 32 columns; 64 keys at a time, the workgroup turns the codes of
 // K and V into 16-bit rows in LDS once for all of them (a thread takes one
 // 32-element scale group of each: 16 conversions, exact in bf16 and saturating in
-// fp16), while the codes of the next 64 keys are on their way into registers.
+// fp16), while the codes of the next 64 keys are on their way into registers (one
+// tile of each in LDS: two measured the same, 343 and 338 us for 1024 rows over
+// 16384 keys, Hq=32 Hkv=8 D=128 bf16, as the other workgroup of the CU computes
+// meanwhile).
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16: a lane owns a column, its
 // probabilities go from the accumulators into the second product as they are, and
 // V is read transposed (ds_read_b64_tr_b16).  Exponent references are integers
@@ -21,17 +24,27 @@ namespace {
 
 constexpr int kTK = 64;  // keys per block
 
+// A row of the V tile is not padded: 16-byte chunk c of row r is in slot c ^
+// vswz<DP>(r), which spreads the stores of 16 lanes (a scale group each, the same
+// chunk of it) and the transposing reads' four rows over the 16 slots of 256 bytes.
+template <int DP>
+__device__ __forceinline__ int vswz4(int r) {
+    return DP == 128 ? 5 * (r & 3) : DP == 64 ? 4 * ((r >> 1) & 1) + ((r >> 1) & 3) : DP == 96 ? r & 3 : (r >> 2) & 3;
+}
+
 template <int DP, bool IS_BF16, bool BIAS>
 __global__ void __launch_bounds__(kThreads4) __attribute__((amdgpu_waves_per_eu(2)))
 mfa_kv4_tile_kernel(K4Args) {
     typedef typename std::conditional<IS_BF16, bf16x8_t, f16x8_t>::type op_t;
     constexpr int DS = DP / 16, DB = DP / 32, GPR = DP / 32, CPR = DP / 8;
-    constexpr int KST = DP + 8, VST = DP + 32;  // LDS rows (elements), padded against bank conflicts
+    constexpr int KST = DP + 8, VST = DP;       // LDS rows (elements); K's padded against bank conflicts
     constexpr int K_ELEMS = kTK * KST, V_ELEMS = kTK * VST;
     constexpr int GROUPS = 2 * kTK * GPR;       // scale groups of a block, K's then V's
     constexpr int NG = (GROUPS + kThreads4 - 1) / kThreads4;
-    static_assert(4 * 32 * KST <= 2 * (K_ELEMS + V_ELEMS), "the tiles hold every wavefront's result rows");
-    __shared__ __attribute__((aligned(16))) uint16_t smem[2 * (K_ELEMS + V_ELEMS)];
+    constexpr int R_ELEMS = 4 * 32 * KST;       // the wavefronts' result rows, in the tiles' place
+    __shared__ __attribute__((aligned(16))) uint16_t smem[R_ELEMS > K_ELEMS + V_ELEMS ? R_ELEMS : K_ELEMS + V_ELEMS];
+    uint16_t* const ktile = smem;
+    uint16_t* const vtile = smem + K_ELEMS;
 
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -40,7 +53,7 @@ mfa_kv4_tile_kernel(K4Args) {
 
     // this thread's groups of a block: wavefront-uniform choice of K or V
     bool gv[NG];
-    int glds[NG];
+    int glds[NG], gsw[NG];
     uint32_t goff[NG], gsoff[NG];
     {
         K4Const& a = args4();
@@ -53,7 +66,9 @@ mfa_kv4_tile_kernel(K4Args) {
             const bool in = g < GROUPS;
             goff[i] = in ? (uint32_t)(row * (int)(gv[i] ? a.v.cr : a.k.cr) + grp * 16) : 0x80000000u;
             gsoff[i] = in ? (uint32_t)(row * (int)(gv[i] ? a.v.sr : a.k.sr) + grp) : 0x80000000u;
-            glds[i] = (gv[i] ? 2 * K_ELEMS + row * VST : row * KST) + 32 * grp;
+            // (chunk e of the group: + 8 (e ^ gsw))
+            glds[i] = gv[i] ? K_ELEMS + row * VST + ((32 * grp) ^ ((vswz4<DP>(row) & ~3) << 3)) : row * KST + 32 * grp;
+            gsw[i] = gv[i] ? vswz4<DP>(row) & 3 : 0;
         }
     }
 
@@ -109,15 +124,15 @@ mfa_kv4_tile_kernel(K4Args) {
                 gs[i] = __builtin_amdgcn_raw_buffer_load_b8(gv[i] ? pg.rs[3] : pg.rs[1], gsoff[i] + (uint32_t)(row * pg.rstride[x + 1]), 0, 0);
             }
         };
-        auto swrite = [&](int buf) {
+        auto swrite = [&]() {
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
                 if (GROUPS % kThreads4 == 0 || tid + kThreads4 * i < GROUPS) {
-                    uint16_t* p = smem + glds[i] + buf * (gv[i] ? V_ELEMS : K_ELEMS);
+                    uint16_t* p = smem + glds[i];
                     const float s = kv4_scale(gs[i]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        *reinterpret_cast<u32x4_t*>(p + 8 * e) = IS_BF16 ? kv4_bf16x8(gc[i][e], s) : kv4_f16x8(gc[i][e], s);
+                        *reinterpret_cast<u32x4_t*>(p + 8 * (e ^ gsw[i])) = IS_BF16 ? kv4_bf16x8(gc[i][e], s) : kv4_f16x8(gc[i][e], s);
                 }
             }
         };
@@ -135,10 +150,12 @@ mfa_kv4_tile_kernel(K4Args) {
             else
                 return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, acc, 0, 0, 0);
         };
-        const int tr_row = 4 * half + ((lane & 15) >> 2), tr_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-        auto load_vf = [&](const uint16_t* vbuf, int db, int kb, int st) -> op_t {
-            const uint16_t* p0 = vbuf + (32 * kb + 16 * st + tr_row) * VST + 32 * db + tr_col;
-            const uint16_t* p1 = p0 + 8 * VST;
+        const int tr_row = 4 * half + ((lane & 15) >> 2), tr_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        auto load_vf = [&](int db, int kb, int st) -> op_t {
+            // (rows 16 apart have the same swizzle)
+            auto at = [&](int r) { return r * VST + (((4 * db + tr_chunk) ^ vswz4<DP>(r)) << 3) + 4 * (lane & 1); };
+            const uint16_t* p0 = vtile + (32 * kb + 16 * st) * VST + at(tr_row);
+            const uint16_t* p1 = vtile + (32 * kb + 16 * st) * VST + at(tr_row + 8);
             if constexpr (IS_BF16) {
                 typedef __attribute__((__vector_size__(4 * sizeof(__bf16)))) __bf16 v4;
                 typedef __attribute__((address_space(3))) v4* lp;
@@ -154,7 +171,7 @@ mfa_kv4_tile_kernel(K4Args) {
             }
         };
 
-        auto block = [&](bool masked, const uint16_t* kbuf, const uint16_t* vbuf, int j) {
+        auto block = [&](bool masked, int j) {
             f32x16_t s[2];
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -163,7 +180,7 @@ mfa_kv4_tile_kernel(K4Args) {
                 for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
 #pragma unroll
                 for (int t = 0; t < DS; ++t)
-                    s[kb] = mfma(*reinterpret_cast<const op_t*>(kbuf + (32 * kb + l32) * KST + 16 * t + 8 * half), qf[t], s[kb]);
+                    s[kb] = mfma(*reinterpret_cast<const op_t*>(ktile + (32 * kb + l32) * KST + 16 * t + 8 * half), qf[t], s[kb]);
             }
             __builtin_amdgcn_s_setprio(0);
             // register r of s[kb] is key j + 32 kb + 4 half + acc_row(r)
@@ -218,11 +235,12 @@ mfa_kv4_tile_kernel(K4Args) {
                 m = mn;
             }
             const float mu = m == -INFINITY ? 0.f : m;
-            // probabilities rounded to 16 bits; l adds them as rounded
-            u32x4_t pw[2][2];
+            // probabilities rounded to 16 bits; l adds them as rounded.  The second 32
+            // keys' are formed while the first's products run.
             float acc[2] = {0.f, 0.f};
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < 2; ++kb) {
+                u32x4_t pw[2];
 #pragma unroll
                 for (int st = 0; st < 2; ++st)
 #pragma unroll
@@ -232,23 +250,22 @@ mfa_kv4_tile_kernel(K4Args) {
                         if constexpr (IS_BF16) {
                             const k4_bf16x2_t pk = {(__bf16)p0, (__bf16)p1}, one = {(__bf16)1.f, (__bf16)1.f};
                             acc[w & 1] = __builtin_amdgcn_fdot2_f32_bf16(pk, one, acc[w & 1], false);
-                            pw[kb][st][w] = __builtin_bit_cast(uint32_t, pk);
+                            pw[st][w] = __builtin_bit_cast(uint32_t, pk);
                         } else {
                             const k4_f16x2_t pk = {(_Float16)p0, (_Float16)p1}, one = {(_Float16)1.f, (_Float16)1.f};
                             acc[w & 1] = __builtin_amdgcn_fdot2(pk, one, acc[w & 1], false);
-                            pw[kb][st][w] = __builtin_bit_cast(uint32_t, pk);
+                            pw[st][w] = __builtin_bit_cast(uint32_t, pk);
                         }
                     }
-            l += acc[0] + acc[1];
-            __builtin_amdgcn_s_setprio(1);
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int db = 0; db < DB; ++db)
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int db = 0; db < DB; ++db)
 #pragma unroll
                     for (int st = 0; st < 2; ++st)
-                        o[db] = mfma(load_vf(vbuf, db, kb, st), __builtin_bit_cast(op_t, pw[kb][st]), o[db]);
-            __builtin_amdgcn_s_setprio(0);
+                        o[db] = mfma(load_vf(db, kb, st), __builtin_bit_cast(op_t, pw[st]), o[db]);
+                __builtin_amdgcn_s_setprio(0);
+            }
+            l += acc[0] + acc[1];
         };
 
         if (jbeg < jend) gload(jbeg);
@@ -256,20 +273,11 @@ mfa_kv4_tile_kernel(K4Args) {
 #pragma unroll
         for (int s = 0; s < DS; ++s) pin(qf[s]);
         pin(slope);
-        if (jbeg < jend) {
-            swrite(0);
-            if (jbeg + kTK < jend) gload(jbeg + kTK);
-        }
-        __syncthreads();
-        int buf = 0;
-        for (int j = jbeg; j < jend; j += kTK, buf ^= 1) {
-            const uint16_t* kbuf = smem + buf * K_ELEMS;
-            const uint16_t* vbuf = smem + 2 * K_ELEMS + buf * V_ELEMS;
-            if (live && j <= w_hi && j + kTK - 1 >= w_lo) block(j < f_lo || j + kTK - 1 > f_hi, kbuf, vbuf, j);
-            if (j + kTK < jend) {
-                swrite(buf ^ 1);
-                if (j + 2 * kTK < jend) gload(j + 2 * kTK);
-            }
+        for (int j = jbeg; j < jend; j += kTK) {
+            swrite();
+            if (j + kTK < jend) gload(j + kTK);
+            __syncthreads();
+            if (live && j <= w_hi && j + kTK - 1 >= w_lo) block(j < f_lo || j + kTK - 1 > f_hi, j);
             __syncthreads();
         }
 

@@ -25,7 +25,13 @@
 namespace {
 
 constexpr int kNThreads = 256;
-constexpr int kNMaxBlocks = 1024;  // workgroups of the backward per tensor (partial weight sums)
+#ifndef MFA_NORM_BLOCKS
+#define MFA_NORM_BLOCKS 1024
+#endif
+#ifndef MFA_NORM_FWD
+#define MFA_NORM_FWD 16
+#endif
+constexpr int kNMaxBlocks = MFA_NORM_BLOCKS;  // workgroups of the backward per tensor (partial weight sums)
 enum { kHalf = 0, kInterleaved = 1, kAny = 2 };
 
 struct NTensor {
@@ -251,32 +257,46 @@ __device__ __forceinline__ Row row_of(const NArgs& a, const NTensor& t, int64_t 
     return w;
 }
 
+// rows of a lane group whose loads are in flight together
+#ifndef MFA_NORM_ROWS
+#define MFA_NORM_ROWS 2
+#endif
 template <int DT, int MODE, int LPR>
 __global__ void __launch_bounds__(kNThreads) mfa_norm_rope_kernel(NArgs a) {
     constexpr int ES = DT == MFA_DTYPE_F32 ? 4 : 2;
+    constexpr int kRows = MODE == kAny ? 1 : MFA_NORM_ROWS;
     const Lane<MODE, LPR> ln(a);
     const int which = blockIdx.x >= (unsigned)a.blocks[0];
     const NTensor& t = a.t[which];
     const int64_t blk = blockIdx.x - (which ? a.blocks[0] : 0);
     float w[8];
     ln.weights(a, t.w, w);
-    for (int64_t r = blk * (kNThreads / LPR) + threadIdx.x / LPR; r < t.rows; r += (int64_t)a.blocks[which] * (kNThreads / LPR)) {
-        const Row row = row_of(a, t, r);
-        float x[8], c[4], s[4];
-        ln.template load<DT>(a, t.x + (row.b * t.xb + row.i * t.xs + row.h * t.xh) * ES, x);
-        ln.angles(a, row.pos, c, s);
-        float sq[8];
+    const int64_t step = (int64_t)a.blocks[which] * (kNThreads / LPR);
+    for (int64_t r0 = blk * (kNThreads / LPR) + threadIdx.x / LPR; r0 < t.rows; r0 += kRows * step) {
+        float x[kRows][8], c[kRows][4], s[kRows][4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sq[i] = x[i] * x[i];
-        const float rs = rsqrtf(fmaf(row_sum<LPR>(sum8(sq)), a.inv_d, a.eps));
-        float y[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float u = x[i] * rs * w[i], v = x[4 + i] * rs * w[4 + i];
-            y[i] = u * c[i] - v * s[i];
-            y[4 + i] = v * c[i] + u * s[i];
+        for (int u = 0; u < kRows; ++u) {
+            const int64_t r = min(r0 + u * step, t.rows - 1);
+            const Row row = row_of(a, t, r);
+            ln.template load<DT>(a, t.x + (row.b * t.xb + row.i * t.xs + row.h * t.xh) * ES, x[u]);
+            ln.angles(a, row.pos, c[u], s[u]);
         }
-        ln.template store<DT>(a, t.out + r * a.D * ES, y);
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            float sq[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sq[i] = x[u][i] * x[u][i];
+            const float rs = rsqrtf(fmaf(row_sum<LPR>(sum8(sq)), a.inv_d, a.eps));
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = x[u][i] * rs * w[i], q = x[u][4 + i] * rs * w[4 + i];
+                y[i] = p * c[u][i] - q * s[u][i];
+                y[4 + i] = q * c[u][i] + p * s[u][i];
+            }
+            const int64_t r = r0 + u * step;
+            if (u == 0 || r < t.rows) ln.template store<DT>(a, t.out + r * a.D * ES, y);
+        }
     }
 }
 
@@ -284,6 +304,7 @@ template <int DT, int MODE, int LPR>
 __global__ void __launch_bounds__(kNThreads) mfa_norm_rope_bwd_kernel(NArgs a) {
     constexpr int ES = DT == MFA_DTYPE_F32 ? 4 : 2;
     constexpr int RPB = kNThreads / LPR;
+    constexpr int kRows = MODE == kAny ? 1 : MFA_NORM_ROWS;
     __shared__ float sh[4][128];
     const Lane<MODE, LPR> ln(a);
     const int which = blockIdx.x >= (unsigned)a.blocks[0];
@@ -293,34 +314,46 @@ __global__ void __launch_bounds__(kNThreads) mfa_norm_rope_bwd_kernel(NArgs a) {
     ln.weights(a, t.w, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[i] = 0.f;
-    for (int64_t r = blk * RPB + threadIdx.x / LPR; r < t.rows; r += (int64_t)a.blocks[which] * RPB) {
-        const Row row = row_of(a, t, r);
-        float x[8], g[8], c[4], s[4];
-        ln.template load<DT>(a, t.x + (row.b * t.xb + row.i * t.xs + row.h * t.xh) * ES, x);
-        ln.template load<DT>(a, t.g + (row.b * t.gb + row.i * t.gs + row.h * t.gh) * ES, g);
-        ln.angles(a, row.pos, c, s);
-        float sq[8];
+    const int64_t step = (int64_t)a.blocks[which] * RPB;
+    for (int64_t r0 = blk * RPB + threadIdx.x / LPR; r0 < t.rows; r0 += kRows * step) {
+        float xs[kRows][8], gs[kRows][8], cs[kRows][4], ss[kRows][4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sq[i] = x[i] * x[i];
-        const float rs = rsqrtf(fmaf(row_sum<LPR>(sum8(sq)), a.inv_d, a.eps));
-        float hn[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {  // g turned back, then g w n
-            const float u = g[i] * c[i] + g[4 + i] * s[i], v = g[4 + i] * c[i] - g[i] * s[i];
-            g[i] = u;
-            g[4 + i] = v;
+        for (int u = 0; u < kRows; ++u) {
+            const int64_t r = min(r0 + u * step, t.rows - 1);
+            const Row row = row_of(a, t, r);
+            ln.template load<DT>(a, t.x + (row.b * t.xb + row.i * t.xs + row.h * t.xh) * ES, xs[u]);
+            ln.template load<DT>(a, t.g + (row.b * t.gb + row.i * t.gs + row.h * t.gh) * ES, gs[u]);
+            ln.angles(a, row.pos, cs[u], ss[u]);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[i] *= rs;
-            dw[i] = fmaf(g[i], x[i], dw[i]);
-            g[i] *= w[i];
-            hn[i] = g[i] * x[i];
-        }
-        const float mean = row_sum<LPR>(sum8(hn)) * a.inv_d;
+        for (int u = 0; u < kRows; ++u) {
+            float(&x)[8] = xs[u];
+            float(&g)[8] = gs[u];
+            const int64_t r = r0 + u * step;
+            const bool in = u == 0 || r < t.rows;
+            float sq[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = rs * fmaf(-x[i], mean, g[i]);
-        ln.template store<DT>(a, t.out + r * a.D * ES, x);
+            for (int i = 0; i < 8; ++i) sq[i] = x[i] * x[i];
+            const float rs = rsqrtf(fmaf(row_sum<LPR>(sum8(sq)), a.inv_d, a.eps));
+            float hn[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // g turned back, then g w n
+                const float p = g[i] * cs[u][i] + g[4 + i] * ss[u][i], q = g[4 + i] * cs[u][i] - g[i] * ss[u][i];
+                g[i] = p;
+                g[4 + i] = q;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] *= rs;
+                if (in) dw[i] = fmaf(g[i], x[i], dw[i]);
+                g[i] *= w[i];
+                hn[i] = g[i] * x[i];
+            }
+            const float mean = row_sum<LPR>(sum8(hn)) * a.inv_d;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = rs * fmaf(-x[i], mean, g[i]);
+            if (in) ln.template store<DT>(a, t.out + r * a.D * ES, x);
+        }
     }
     if (!a.dw[which]) return;
     // the workgroup's sums: over the rows of a wavefront, then over wavefronts
@@ -352,8 +385,10 @@ __global__ void __launch_bounds__(kNThreads) mfa_norm_rope_dw_kernel(NArgs a) {
     if (!a.dw[which]) return;
     const float* ws = a.ws + (which ? (int64_t)a.blocks[0] * a.D : 0);
     float sum = 0.f;
-    if (d < a.D)
+    if (d < a.D) {
+#pragma unroll 8
         for (int r = threadIdx.x / kRCols; r < a.blocks[which]; r += kNThreads / kRCols) sum += ws[(int64_t)r * a.D + d];
+    }
     sh[threadIdx.x] = sum;
     __syncthreads();
     for (int n = kNThreads / 2; n >= kRCols; n >>= 1) {
@@ -476,7 +511,7 @@ int n_plan(const mfa_norm_rope_params* p, const mfa_norm_rope_bwd_params* b, NPl
     plan->lpr = plan->mode == kAny ? 16 : p->head_dim <= 32 ? 4 : p->head_dim <= 64 ? 8 : 16;
     // forward: a row per lane group, up to 16 workgroups per CU, then a walk;
     // backward: fewer workgroups, each one partial sum of the weight gradients
-    const int64_t rpb = kNThreads / plan->lpr, most = b ? kNMaxBlocks : (int64_t)cus * 16;
+    const int64_t rpb = kNThreads / plan->lpr, most = b ? kNMaxBlocks : (int64_t)cus * MFA_NORM_FWD;
     for (int i = 0; i < 2; ++i) a.blocks[i] = (int32_t)std::min<int64_t>((a.t[i].rows + rpb - 1) / rpb, most);
     if (b) {
         a.dw[0] = p->q_weight ? static_cast<char*>(b->dq_weight) : nullptr;
@@ -485,10 +520,13 @@ int n_plan(const mfa_norm_rope_params* p, const mfa_norm_rope_bwd_params* b, NPl
     return MFA_OK;
 }
 
+// (by the sizes alone, also where alignment decides the lanes per row)
 int64_t n_ws_bytes(const NPlan& plan) {
     const NArgs& a = plan.a;
     if (!a.dw[0] && !a.dw[1]) return 0;
-    return ((int64_t)a.blocks[0] + a.blocks[1]) * a.D * 4;
+    int64_t blocks = 0;
+    for (const NTensor& t : a.t) blocks += std::min<int64_t>((t.rows + kNThreads / 16 - 1) / (kNThreads / 16), kNMaxBlocks);
+    return blocks * a.D * 4;
 }
 
 void n_launch(const NPlan& plan, bool bwd, int dtype, hipStream_t st) {

@@ -24,18 +24,19 @@ _ATTEND_DTYPES = (torch.float16, torch.bfloat16)
 _plans = {}
 
 
-def _sig(t):
-    return (t.shape, t.stride(), t.dtype, t.device)
-
-
-def _plan(key, make):
-    plan = _plans.get(key)
-    if plan is None:
-        plan = make()
-        if len(_plans) >= _kernel._PLANS_MAX:
-            _plans.clear()
-        _plans[key] = plan
+def _remember(key, plan):
+    if len(_plans) >= _kernel._PLANS_MAX:
+        _plans.clear()
+    _plans[key] = plan
     return plan
+
+
+def _not_tensors(k_cache, v_cache):
+    """The error for arguments of which no signature can be formed."""
+    for what, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if not isinstance(c, (tuple, list)) or len(c) != 2 or not (torch.is_tensor(c[0]) and torch.is_tensor(c[1])):
+            return ValueError(f"mtlflashattn_amd: {what} must be a pair (codes, scales), as kv4_cache makes it")
+    return ValueError("mtlflashattn_amd: tensors expected")
 
 
 def kv4_cache(num_pages, page_block_size, num_heads_kv, head_dim, device="cuda"):
@@ -53,18 +54,6 @@ def kv4_cache(num_pages, page_block_size, num_heads_kv, head_dim, device="cuda")
         raise NotImplementedError(f"mtlflashattn_amd: head_dim {head_dim} of a 4-bit cache must be 32, 64, 96 or 128")
     return tuple(torch.zeros(num_pages, num_heads_kv, page_block_size, n, dtype=torch.uint8, device=device).transpose(1, 2)
                  for n in (head_dim // 2, head_dim // 32))
-
-
-def _check_tensors(*tensors):
-    """Before a call's signature is formed: everything in its place is a tensor."""
-    if not all(torch.is_tensor(t) for t in tensors):
-        raise ValueError("mtlflashattn_amd: tensors expected")
-
-
-def _check_pairs(k_cache, v_cache):
-    for what, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if not isinstance(c, (tuple, list)) or len(c) != 2 or not (torch.is_tensor(c[0]) and torch.is_tensor(c[1])):
-            raise ValueError(f"mtlflashattn_amd: {what} must be a pair (codes, scales), as kv4_cache makes it")
 
 
 def _check_cache(cache, D, Hkv, device, what):
@@ -116,10 +105,11 @@ def _cache_struct(c, k_cache, v_cache, block_table):
     c.block_table_batch_stride = block_table.stride(0) if block_table.shape[0] > 1 else 0
 
 
-def _cache_pointers(c, k_cache, v_cache, block_table):
-    ck, cv = c.k, c.v
-    ck.codes, ck.scales = k_cache[0].data_ptr(), k_cache[1].data_ptr()
-    cv.codes, cv.scales = v_cache[0].data_ptr(), v_cache[1].data_ptr()
+def _cache_pointers(c, kc, ks, vc, vs, block_table):
+    pool = c.k
+    pool.codes, pool.scales = kc.data_ptr(), ks.data_ptr()
+    pool = c.v
+    pool.codes, pool.scales = vc.data_ptr(), vs.data_ptr()
     c.block_table = block_table.data_ptr()
 
 
@@ -128,10 +118,8 @@ def _i32(t):
 
 
 def _check_pages(block_table, lens, page, num_pages):
-    """With MTLFLASHATTN_CHECK_PAGES=1: the page ids that `lens` rows use, on the host."""
-    if not _kernel._check_pages_enabled():
-        return
-    lens = lens.clamp(min=0).cpu()
+    """The page ids that `lens` rows use, on the host (MTLFLASHATTN_CHECK_PAGES=1)."""
+    lens = lens.clamp(min=0).cpu().long()
     used = torch.arange(block_table.shape[1]).unsqueeze(0) < ((lens + page - 1) // page).unsqueeze(1)
     if lens.numel() and int(lens.max()) > block_table.shape[1] * page:
         raise ValueError(f"mtlflashattn_amd: block_table has {block_table.shape[1]} pages per sequence, "
@@ -164,52 +152,71 @@ def kv4_append(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, r
     back from the cache (flash_attn_varlen_func(q, k', v', ...)).  Not
     differentiable: inputs that require grad raise.
     """
-    def make():
-        if k.dim() != 3 or v.dim() != 3 or k.shape != v.shape:
-            raise ValueError(f"mtlflashattn_amd: expected k and v [total,H,D], got {tuple(k.shape)} and {tuple(v.shape)}")
-        _kernel._check_device(k, v)
-        if k.dtype not in _kernel._SUPPORTED_DTYPES or v.dtype != k.dtype:
-            raise NotImplementedError(f"mtlflashattn_amd: dtype {k.dtype} (k/v must match, fp16/bf16/fp32)")
-        total, Hkv, D = k.shape
-        if D == 0 or D % 32 or D > MAX_HEAD_DIM:
-            raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} of a 4-bit cache must be 32, 64, 96 or 128")
-        _check_cache(k_cache, D, Hkv, k.device, "k_cache")
-        _check_cache(v_cache, D, Hkv, k.device, "v_cache")
-        if k_cache[0].shape != v_cache[0].shape:
-            raise ValueError("mtlflashattn_amd: k_cache and v_cache differ in pages")
-        batch = cache_seqlens.shape[0] if torch.is_tensor(cache_seqlens) and cache_seqlens.dim() == 1 else 0
-        _check_ints(cache_seqlens, batch, k.device, "cache_seqlens")
-        _check_ints(cu_seqlens, batch + 1, k.device, "cu_seqlens")
-        _check_table(block_table, batch, k.device)
-        p = _hip.MfaKv4AppendParams()
-        _cache_struct(p.cache, k_cache, v_cache, block_table)
-        p.batch, p.total, p.heads_kv, p.head_dim = batch, total, Hkv, D
-        p.dtype = _hip.DTYPE_CODES[k.dtype]
-        return p
-
-    _check_tensors(k, v, cu_seqlens, cache_seqlens, block_table)
-    _check_pairs(k_cache, v_cache)
+    try:
+        (kc, ks), (vc, vs) = k_cache, v_cache
+        key = ("append", k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
+               kc.shape, kc.stride(), kc.dtype, kc.device, ks.shape, ks.stride(), ks.dtype, ks.device,
+               vc.shape, vc.stride(), vc.dtype, vc.device, vs.shape, vs.stride(), vs.dtype, vs.device,
+               cu_seqlens.shape, cu_seqlens.stride(), cu_seqlens.dtype, cu_seqlens.device,
+               cache_seqlens.shape, cache_seqlens.stride(), cache_seqlens.dtype, cache_seqlens.device,
+               block_table.shape, block_table.stride(), block_table.dtype, block_table.device)
+    except (AttributeError, TypeError, ValueError):
+        raise _not_tensors(k_cache, v_cache) from None
     if _kernel._needs_grad(k, v):
         raise NotImplementedError("mtlflashattn_amd: kv4_append is not differentiable; run it under torch.no_grad() or on "
                                   "detached rows")
-    key = ("append", _sig(k), _sig(v), *(_sig(t) for c in (k_cache, v_cache) for t in c), _sig(cu_seqlens),
-           _sig(cache_seqlens), _sig(block_table))
-    p = _hip.MfaKv4AppendParams.from_buffer_copy(_plan(key, make))
-    kk, vv, cu, lens = _kernel._abi_operand(k), _kernel._abi_operand(v), _i32(cu_seqlens), _i32(cache_seqlens)
-    _check_pages(block_table, lens + (cu[1:] - cu[:-1]) if _kernel._check_pages_enabled() else lens, k_cache[0].shape[1],
-                 k_cache[0].shape[0])
-    p.k, p.v = kk.data_ptr(), vv.data_ptr()
-    p.k_token_stride, p.k_head_stride = (s if n > 1 else 0 for s, n in zip(kk.stride()[:2], kk.shape[:2]))
-    p.v_token_stride, p.v_head_stride = (s if n > 1 else 0 for s, n in zip(vv.stride()[:2], vv.shape[:2]))
-    _cache_pointers(p.cache, k_cache, v_cache, block_table)
-    p.cu_seqlens, p.cache_seqlens = cu.data_ptr(), lens.data_ptr()
+    plan = _plans.get(key) or _remember(key, _append_plan(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table))
+    template, direct = plan
+    p = _hip.MfaKv4AppendParams.from_buffer_copy(template)
+    kp, vp = k.data_ptr(), v.data_ptr()
+    if not direct or (kp | vp) & 15:
+        k_, v_, cu_seqlens, cache_seqlens = (_kernel._abi_operand(k), _kernel._abi_operand(v), _i32(cu_seqlens),
+                                             _i32(cache_seqlens))
+        kp, vp = k_.data_ptr(), v_.data_ptr()
+        p.k_token_stride, p.k_head_stride = _token_strides(k_)
+        p.v_token_stride, p.v_head_stride = _token_strides(v_)
+    if _kernel._check_pages_enabled():
+        _check_pages(block_table, cache_seqlens + (cu_seqlens[1:] - cu_seqlens[:-1]), kc.shape[1], kc.shape[0])
+    p.k, p.v, p.cu_seqlens, p.cache_seqlens = kp, vp, cu_seqlens.data_ptr(), cache_seqlens.data_ptr()
+    _cache_pointers(p.cache, kc, ks, vc, vs, block_table)
     values = None
     if return_values:
-        values = tuple(torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
+        values = k.new_empty(k.shape), v.new_empty(v.shape)
         p.k_values, p.v_values = values[0].data_ptr(), values[1].data_ptr()
-    with _kernel._on(k.device):
-        _hip.kv4_append(p, torch._C._cuda_getCurrentRawStream(k.device.index))
+    _kernel._launch_on(k.device, _hip.kv4_append, p)
     return values
+
+
+def _token_strides(x):
+    return tuple(s if n > 1 else 0 for s, n in zip(x.stride()[:2], x.shape[:2]))
+
+
+def _append_plan(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table):
+    """(parameters without data pointers, whether the tensors are used in place) of a kv4_append call."""
+    if k.dim() != 3 or v.dim() != 3 or k.shape != v.shape:
+        raise ValueError(f"mtlflashattn_amd: expected k and v [total,H,D], got {tuple(k.shape)} and {tuple(v.shape)}")
+    _kernel._check_device(k, v)
+    if k.dtype not in _kernel._SUPPORTED_DTYPES or v.dtype != k.dtype:
+        raise NotImplementedError(f"mtlflashattn_amd: dtype {k.dtype} (k/v must match, fp16/bf16/fp32)")
+    total, Hkv, D = k.shape
+    if D == 0 or D % 32 or D > MAX_HEAD_DIM:
+        raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} of a 4-bit cache must be 32, 64, 96 or 128")
+    _check_cache(k_cache, D, Hkv, k.device, "k_cache")
+    _check_cache(v_cache, D, Hkv, k.device, "v_cache")
+    if k_cache[0].shape != v_cache[0].shape:
+        raise ValueError("mtlflashattn_amd: k_cache and v_cache differ in pages")
+    batch = cache_seqlens.shape[0] if cache_seqlens.dim() == 1 else 0
+    _check_ints(cache_seqlens, batch, k.device, "cache_seqlens")
+    _check_ints(cu_seqlens, batch + 1, k.device, "cu_seqlens")
+    _check_table(block_table, batch, k.device)
+    p = _hip.MfaKv4AppendParams()
+    _cache_struct(p.cache, k_cache, v_cache, block_table)
+    p.k_token_stride, p.k_head_stride = _token_strides(k)
+    p.v_token_stride, p.v_head_stride = _token_strides(v)
+    p.batch, p.total, p.heads_kv, p.head_dim = batch, total, Hkv, D
+    p.dtype = _hip.DTYPE_CODES[k.dtype]
+    return p, (_kernel._fits_strides(k) and _kernel._fits_strides(v) and _i32(cu_seqlens) is cu_seqlens
+               and _i32(cache_seqlens) is cache_seqlens)
 
 
 def flash_attn_kv4_func(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale=None, causal=False,
@@ -257,105 +264,121 @@ def flash_attn_varlen_kv4_func(q, k_cache, v_cache, cu_seqlens_q, cache_seqlens,
 
 def _attend(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap, alibi_slopes,
             max_seqlen_k, return_lse):
-    _check_tensors(q, cache_seqlens, block_table)
-    _check_pairs(k_cache, v_cache)
-    varlen = q.dim() == 3
-    if varlen:
-        _check_tensors(cu_q)
-
-    def make():
-        _kernel._check_device(q)
-        if q.dtype not in _ATTEND_DTYPES:
-            raise NotImplementedError(f"mtlflashattn_amd: dtype {q.dtype} (queries over a 4-bit cache are fp16 or bf16)")
-        Hq, D = q.shape[-2:]
-        if D not in (32, 64, 96, 128):
-            raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} of a 4-bit cache must be 32, 64, 96 or 128")
-        Hkv = k_cache[0].shape[2] if k_cache[0].dim() == 4 else 0
-        _check_cache(k_cache, D, Hkv, q.device, "k_cache")
-        _check_cache(v_cache, D, Hkv, q.device, "v_cache")
-        if k_cache[0].shape != v_cache[0].shape:
-            raise ValueError("mtlflashattn_amd: k_cache and v_cache differ in pages or heads")
-        if Hkv == 0 or Hq == 0 or Hq % Hkv:
-            raise ValueError(f"mtlflashattn_amd: num_heads_kv ({Hkv}) must divide num_heads_q ({Hq})")
-        if varlen:
-            batch = cache_seqlens.shape[0] if torch.is_tensor(cache_seqlens) and cache_seqlens.dim() == 1 else 0
-            _check_ints(cu_q, batch + 1, q.device, "cu_seqlens_q")
-        else:
-            batch = q.shape[0]
-        _check_ints(cache_seqlens, batch, q.device, "cache_seqlens")
-        _check_table(block_table, batch, q.device)
-        if max_seqlen_k is not None and max_seqlen_k < 0:
-            raise ValueError("mtlflashattn_amd: max_seqlen_k must be >= 0")
-        _kernel._alibi_arg(alibi_slopes, batch, Hq, q.device)
-        p = _hip.MfaKv4FwdParams()
-        _cache_struct(p.cache, k_cache, v_cache, block_table)
-        p.batch, p.heads_q, p.heads_kv, p.head_dim = batch, Hq, Hkv, D
-        if varlen:
-            p.total_q = q.shape[0]
-            p.o_seq_stride, p.o_head_stride = Hq * D, D
-            p.lse_head_stride = q.shape[0]
-        else:
-            p.seqlen_q = q.shape[1]
-            p.o_batch_stride, p.o_seq_stride, p.o_head_stride = q.shape[1] * Hq * D, Hq * D, D
-            p.lse_batch_stride, p.lse_head_stride = Hq * q.shape[1], q.shape[1]
-        cap = block_table.shape[1] * k_cache[0].shape[1]
-        p.max_seqlen_k = cap if max_seqlen_k is None else min(int(max_seqlen_k), cap)
-        if p.max_seqlen_k == 0:  # (0 means no bound to the library)
-            p.cache.max_pages = 0
-        p.scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
-        p.softcap = softcap
-        p.window_left, p.window_right = window_size
-        p.causal = int(bool(causal))
-        p.dtype = _hip.DTYPE_CODES[q.dtype]
-        # placeholders: sizing the workspace reads no tensor
-        p.q = p.o = p.cache_seqlens = p.cache.block_table = 256
-        p.cache.k.codes = p.cache.k.scales = p.cache.v.codes = p.cache.v.scales = 256
-        p.cu_seqlens_q = 256 if varlen else None
-        with _kernel._on(q.device):
-            return p, _hip.kv4_fwd_workspace_bytes(p)
-
-    if _kernel._needs_grad(q):
+    _kernel._check_options(window_size, softcap, alibi_slopes)
+    try:
+        (kc, ks), (vc, vs) = k_cache, v_cache
+        varlen = q.dim() == 3
+        key = (q.shape, q.stride(), q.dtype, q.device, kc.shape, kc.stride(), kc.dtype, kc.device,
+               ks.shape, ks.stride(), ks.dtype, ks.device, vc.shape, vc.stride(), vc.dtype, vc.device,
+               vs.shape, vs.stride(), vs.dtype, vs.device,
+               cache_seqlens.shape, cache_seqlens.stride(), cache_seqlens.dtype, cache_seqlens.device,
+               block_table.shape, block_table.stride(), block_table.dtype, block_table.device,
+               varlen and (cu_q.shape, cu_q.stride(), cu_q.dtype, cu_q.device),
+               alibi_slopes is not None and (alibi_slopes.shape, alibi_slopes.device),
+               softmax_scale, causal, tuple(window_size), softcap, max_seqlen_k)
+    except (AttributeError, TypeError, ValueError):
+        raise _not_tensors(k_cache, v_cache) from None
+    if q.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("mtlflashattn_amd: attention over a 4-bit cache is forward-only; run it under "
                                   "torch.no_grad() or without inputs that require grad")
-    _kernel._check_options(window_size, softcap, alibi_slopes)
-    window_size = tuple(window_size)
-    key = ("attend", _sig(q), *(_sig(t) for c in (k_cache, v_cache) for t in c), cu_q is not None and _sig(cu_q),
-           _sig(cache_seqlens), _sig(block_table), alibi_slopes is not None and _sig(alibi_slopes), softmax_scale,
-           bool(causal), window_size, softcap, max_seqlen_k)
-    template, nbytes = _plan(key, make)
+    plan = _plans.get(key) or _remember(key, _attend_plan(
+        q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap, alibi_slopes,
+        max_seqlen_k))
+    template, nbytes, direct = plan
     if _kernel._trace_enabled():
         _kernel._record_trace(q.dtype, q.shape[-1], q.shape[0 if varlen else 1], template.max_seqlen_k, causal, "hip-kv4")
     p = _hip.MfaKv4FwdParams.from_buffer_copy(template)
-    device, qq, lens = q.device, _kernel._abi_operand(q), _i32(cache_seqlens)
-    _check_pages(block_table, lens.clamp(max=template.max_seqlen_k) if _kernel._check_pages_enabled() else lens,
-                 k_cache[0].shape[1], k_cache[0].shape[0])
-    strides = [s if n > 1 else 0 for s, n in zip(qq.stride(), qq.shape)]
+    device, qp = q.device, q.data_ptr()
+    if not direct or qp & 15:
+        q_, cache_seqlens = _kernel._abi_operand(q), _i32(cache_seqlens)
+        qp = q_.data_ptr()
+        strides = [s if n > 1 else 0 for s, n in zip(q_.stride(), q_.shape)]
+        p.q_batch_stride, p.q_seq_stride, p.q_head_stride = (0, *strides[:2]) if varlen else strides[:3]
+        if varlen:
+            cu_q = _i32(cu_q)
+    if _kernel._check_pages_enabled():
+        _check_pages(block_table, cache_seqlens.clamp(max=template.max_seqlen_k), kc.shape[1], kc.shape[0])
+    out, lse = q.new_empty(q.shape), None
+    if return_lse:
+        shape = (q.shape[1], q.shape[0]) if varlen else (q.shape[0], q.shape[2], q.shape[1])
+        lse = torch.empty(shape, dtype=torch.float32, device=device)
+        p.softmax_lse = lse.data_ptr()
     if varlen:
-        cu = _i32(cu_q)
-        p.cu_seqlens_q = cu.data_ptr()
-        p.q_seq_stride, p.q_head_stride = strides[:2]
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=device) if return_lse else None
+        p.cu_seqlens_q = cu_q.data_ptr()
         if p.batch == 0:  # (nothing is launched)
             out.zero_()
             if return_lse:
                 lse.fill_(float("-inf"))
-    else:
-        p.q_batch_stride, p.q_seq_stride, p.q_head_stride = strides[:3]
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=device) if return_lse else None
-    p.q, p.o = qq.data_ptr(), out.data_ptr()
-    if lse is not None:
-        p.softmax_lse = lse.data_ptr()
     if alibi_slopes is not None:
         slopes, p.alibi_batch_stride = _kernel._alibi_arg(alibi_slopes, p.batch, p.heads_q, device)
         p.alibi_slopes = slopes.data_ptr()
-    p.cache_seqlens = lens.data_ptr()
-    _cache_pointers(p.cache, k_cache, v_cache, block_table)
-    with _kernel._on(device):
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
-        _hip.kv4_fwd(p, ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(device.index))
+    p.q, p.o, p.cache_seqlens = qp, out.data_ptr(), cache_seqlens.data_ptr()
+    _cache_pointers(p.cache, kc, ks, vc, vs, block_table)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _kernel._launch_on(device, _hip.kv4_fwd, p, None if ws is None else ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
+
+
+def _attend_plan(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap,
+                 alibi_slopes, max_seqlen_k):
+    """(parameters without data pointers, workspace bytes, whether the tensors are used in place) of a call."""
+    varlen = q.dim() == 3
+    _kernel._check_device(q)
+    if q.dtype not in _ATTEND_DTYPES:
+        raise NotImplementedError(f"mtlflashattn_amd: dtype {q.dtype} (queries over a 4-bit cache are fp16 or bf16)")
+    Hq, D = q.shape[-2:]
+    if D not in (32, 64, 96, 128):
+        raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} of a 4-bit cache must be 32, 64, 96 or 128")
+    Hkv = k_cache[0].shape[2] if k_cache[0].dim() == 4 else 0
+    _check_cache(k_cache, D, Hkv, q.device, "k_cache")
+    _check_cache(v_cache, D, Hkv, q.device, "v_cache")
+    if k_cache[0].shape != v_cache[0].shape:
+        raise ValueError("mtlflashattn_amd: k_cache and v_cache differ in pages or heads")
+    if Hkv == 0 or Hq == 0 or Hq % Hkv:
+        raise ValueError(f"mtlflashattn_amd: num_heads_kv ({Hkv}) must divide num_heads_q ({Hq})")
+    if varlen:
+        batch = cache_seqlens.shape[0] if cache_seqlens.dim() == 1 else 0
+        _check_ints(cu_q, batch + 1, q.device, "cu_seqlens_q")
+    else:
+        batch = q.shape[0]
+    _check_ints(cache_seqlens, batch, q.device, "cache_seqlens")
+    _check_table(block_table, batch, q.device)
+    if max_seqlen_k is not None and max_seqlen_k < 0:
+        raise ValueError("mtlflashattn_amd: max_seqlen_k must be >= 0")
+    _kernel._alibi_arg(alibi_slopes, batch, Hq, q.device)
+    p = _hip.MfaKv4FwdParams()
+    _cache_struct(p.cache, k_cache, v_cache, block_table)
+    p.batch, p.heads_q, p.heads_kv, p.head_dim = batch, Hq, Hkv, D
+    strides = [s if n > 1 else 0 for s, n in zip(q.stride(), q.shape)]
+    if varlen:
+        p.total_q = q.shape[0]
+        p.q_seq_stride, p.q_head_stride = strides[:2]
+        p.o_seq_stride, p.o_head_stride = Hq * D, D
+        p.lse_head_stride = q.shape[0]
+    else:
+        p.seqlen_q = q.shape[1]
+        p.q_batch_stride, p.q_seq_stride, p.q_head_stride = strides[:3]
+        p.o_batch_stride, p.o_seq_stride, p.o_head_stride = q.shape[1] * Hq * D, Hq * D, D
+        p.lse_batch_stride, p.lse_head_stride = Hq * q.shape[1], q.shape[1]
+    cap = block_table.shape[1] * k_cache[0].shape[1]
+    p.max_seqlen_k = cap if max_seqlen_k is None else min(int(max_seqlen_k), cap)
+    if p.max_seqlen_k == 0:  # (0 means no bound to the library)
+        p.cache.max_pages = 0
+    p.scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
+    p.softcap = softcap
+    p.window_left, p.window_right = window_size
+    p.causal = int(bool(causal))
+    p.dtype = _hip.DTYPE_CODES[q.dtype]
+    # placeholders: sizing the workspace reads no tensor
+    sized = _hip.MfaKv4FwdParams.from_buffer_copy(p)
+    sized.q = sized.o = sized.cache_seqlens = sized.cache.block_table = 256
+    sized.cache.k.codes = sized.cache.k.scales = sized.cache.v.codes = sized.cache.v.scales = 256
+    sized.cu_seqlens_q = 256 if varlen else None
+    sized.q_batch_stride = sized.q_seq_stride = sized.q_head_stride = 0
+    with _kernel._on(q.device):
+        nbytes = _hip.kv4_fwd_workspace_bytes(sized)
+    return p, nbytes, (_kernel._fits_strides(q) and _i32(cache_seqlens) is cache_seqlens
+                       and (not varlen or _i32(cu_q) is cu_q))
 
 
 def copy_cache_pages(pools, src, dst):
@@ -374,41 +397,58 @@ def copy_cache_pages(pools, src, dst):
     pools = list(pools)
     if not pools:
         return
-    if not all(torch.is_tensor(t) and t.dim() >= 1 for t in pools):
-        raise ValueError("mtlflashattn_amd: pools must be tensors [num_pages, ...]")
-    _kernel._check_device(*pools)
-    device, num_pages = pools[0].device, pools[0].shape[0]
-    if not torch.is_tensor(src) or src.dim() != 1:
-        raise ValueError("mtlflashattn_amd: src must be an int32 [n] tensor of page ids")
-    _check_ints(src, src.shape[0], device, "src")
-    _check_ints(dst, src.shape[0], device, "dst")
-    if any(t.requires_grad for t in pools) and torch.is_grad_enabled():
+    try:
+        key = ("copy", src.shape, src.stride(), src.dtype, src.device, dst.shape, dst.stride(), dst.dtype, dst.device,
+               *[x for t in pools for x in (t.shape, t.stride(), t.dtype, t.device)])
+    except AttributeError:
+        raise ValueError("mtlflashattn_amd: pools, src and dst must be tensors") from None
+    if torch.is_grad_enabled() and any([t.requires_grad for t in pools]):
         raise NotImplementedError("mtlflashattn_amd: copy_cache_pages is not differentiable")
-    sizes = []
-    for t in pools:
-        if t.shape[0] != num_pages:
-            raise ValueError(f"mtlflashattn_amd: pools of {num_pages} and {t.shape[0]} pages")
-        n = 1
-        for size, stride in sorted(zip(t.shape[1:], t.stride()[1:]), key=lambda x: x[1]):
-            if size > 1 and stride != n:
-                raise ValueError("mtlflashattn_amd: the pages of a pool must be dense in memory")
-            n *= size
-        if num_pages > 1 and n and t.stride(0) < n:
-            raise ValueError("mtlflashattn_amd: the pages of a pool must not overlap")
-        sizes.append(n * t.element_size())
-    src, dst = _i32(src), _i32(dst)
+    plan = _plans.get(key) or _remember(key, _copy_plan(pools, src, dst))
+    templates, direct = plan
+    device = pools[0].device
+    if not direct:
+        src, dst = _i32(src), _i32(dst)
     if _kernel._check_pages_enabled():
+        num_pages = pools[0].shape[0]
         pairs = [(a, b) for a, b in zip(src.tolist(), dst.tolist()) if 0 <= a < num_pages and 0 <= b < num_pages and a != b]
         to = [b for _, b in pairs]
         if len(set(to)) != len(to) or set(to) & {a for a, _ in pairs}:
             raise ValueError("mtlflashattn_amd: copy_cache_pages: a destination is given twice or is a source too")
-    with _kernel._on(device):
-        stream = torch._C._cuda_getCurrentRawStream(device.index)
-        for first in range(0, len(pools), _hip.MFA_COPY_MAX_POOLS):
-            p = _hip.MfaCopyPagesParams()
-            part = pools[first:first + _hip.MFA_COPY_MAX_POOLS]
-            for i, t in enumerate(part):
-                p.pool[i] = (t.data_ptr(), t.stride(0) * t.element_size() if num_pages > 1 else 0, sizes[first + i])
-            p.src, p.dst = src.data_ptr(), dst.data_ptr()
-            p.pools, p.pairs, p.num_pages = len(part), src.shape[0], num_pages
-            _hip.copy_pages(p, stream)
+    first = 0
+    for template in templates:
+        p = _hip.MfaCopyPagesParams.from_buffer_copy(template)
+        pool = p.pool
+        for i in range(p.pools):
+            pool[i].base = pools[first + i].data_ptr()
+        first += p.pools
+        p.src, p.dst = src.data_ptr(), dst.data_ptr()
+        _kernel._launch_on(device, _hip.copy_pages, p)
+
+
+def _copy_plan(pools, src, dst):
+    """(parameters without data pointers of each launch, whether the ids are used in place)."""
+    _kernel._check_device(*pools)
+    if any(t.dim() < 1 for t in pools) or src.dim() != 1:
+        raise ValueError("mtlflashattn_amd: pools must be [num_pages, ...] tensors, src and dst int32 [n] page ids")
+    device, num_pages = pools[0].device, pools[0].shape[0]
+    _check_ints(src, src.shape[0], device, "src")
+    _check_ints(dst, src.shape[0], device, "dst")
+    templates = []
+    for first in range(0, len(pools), _hip.MFA_COPY_MAX_POOLS):
+        p = _hip.MfaCopyPagesParams()
+        part = pools[first:first + _hip.MFA_COPY_MAX_POOLS]
+        for i, t in enumerate(part):
+            if t.shape[0] != num_pages:
+                raise ValueError(f"mtlflashattn_amd: pools of {num_pages} and {t.shape[0]} pages")
+            n = 1
+            for size, stride in sorted(zip(t.shape[1:], t.stride()[1:]), key=lambda x: x[1]):
+                if size > 1 and stride != n:
+                    raise ValueError("mtlflashattn_amd: the pages of a pool must be dense in memory")
+                n *= size
+            if num_pages > 1 and n and t.stride(0) < n:
+                raise ValueError("mtlflashattn_amd: the pages of a pool must not overlap")
+            p.pool[i] = (None, t.stride(0) * t.element_size() if num_pages > 1 else 0, n * t.element_size())
+        p.pools, p.pairs, p.num_pages = len(part), src.shape[0], num_pages
+        templates.append(p)
+    return templates, _i32(src) is src and _i32(dst) is dst

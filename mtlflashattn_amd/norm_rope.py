@@ -33,38 +33,49 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, i
     (weight gradients are summed in fp32 in a fixed order: the same bits every
     time); cos and sin are constants.
     """
-    template = _signature(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-    if _kernel._needs_grad(q, k) or (torch.is_grad_enabled() and any(
-            w is not None and w.requires_grad for w in (q_weight, k_weight))):
-        return _QkNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-    return _forward(template, q, k, q_weight, k_weight, cos, sin, positions)
+    plan = _plan(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (
+            q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad)):
+        return _QkNormRopeFn.apply(plan, q, k, q_weight, k_weight, cos, sin, positions)
+    return _forward(plan, q, k, q_weight, k_weight, cos, sin, positions)
 
 
-# prepared parameters (everything but the data pointers) of a call's signature
+class _Plan:
+    """Of a call's signature: its parameters (everything but the data pointers),
+    whether the tensors are used in place, and the backward's workspace (bytes by
+    which weights have a gradient)."""
+
+    __slots__ = ("params", "direct", "ws")
+
+    def __init__(self, params, direct):
+        self.params, self.direct, self.ws = params, direct, {}
+
+
 _plans = {}
 
 
-def _sig(t):
+def _plan(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    """The plan of a call, its arguments checked at their first use."""
     try:
-        return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+        if cos.requires_grad or sin.requires_grad:
+            raise NotImplementedError("mtlflashattn_amd: cos and sin are constants (no gradient)")
+        key = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, cos.shape, cos.stride(),
+               cos.dtype, cos.device, sin.shape, sin.stride(), sin.dtype, sin.device, eps, interleaved,
+               q_weight is not None and (q_weight.shape, q_weight.stride(), q_weight.dtype, q_weight.device),
+               k_weight is not None and (k_weight.shape, k_weight.stride(), k_weight.dtype, k_weight.device),
+               positions is not None and (positions.shape, positions.stride(), positions.dtype, positions.device))
     except AttributeError:
-        raise ValueError(f"mtlflashattn_amd: a tensor expected, got {type(t).__name__}") from None
-
-
-def _signature(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-    """The parameter template of a call, its arguments checked at their first use."""
-    if cos is None or sin is None or q is None or k is None:
-        raise ValueError("mtlflashattn_amd: q, k, cos and sin are required")
-    key = (_sig(q), _sig(k), _sig(q_weight), _sig(k_weight), _sig(cos), _sig(sin), _sig(positions), eps, interleaved)
-    template = _plans.get(key)
-    if template is None:
-        template = _prepare(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+        raise ValueError("mtlflashattn_amd: q, k, cos and sin (and norm weights and positions, if given) must be "
+                         "tensors") from None
+    plan = _plans.get(key)
+    if plan is None:
+        tensors = (q, k, q_weight, k_weight, cos, sin, positions)
+        p = _prepare(*tensors, eps, interleaved)
+        plan = _Plan(p, all(t is _rows(t) for t in tensors) and cos.stride(0) == sin.stride(0))
         if len(_plans) >= _kernel._PLANS_MAX:
             _plans.clear()
-        _plans[key] = template
-    if cos.requires_grad or sin.requires_grad:
-        raise NotImplementedError("mtlflashattn_amd: cos and sin are constants (no gradient)")
-    return template
+        _plans[key] = plan
+    return plan
 
 
 def _check(q, k, q_weight, k_weight, cos, sin, positions, eps):
@@ -132,28 +143,28 @@ def _prepare(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
     return p
 
 
-def _fill(p, q, k, q_weight, k_weight, cos, sin, positions):
+def _fill(p, plan, q, k, q_weight, k_weight, cos, sin, positions):
     """Sets the data pointers; returns the tensors they point into."""
-    held = tuple(_rows(t) for t in (q, k, q_weight, k_weight, cos, sin, positions))
-    q, k, q_weight, k_weight, cos, sin, positions = held
-    if cos.stride(0) != sin.stride(0):
-        cos, sin = cos.contiguous(), sin.contiguous()
-    p.q, p.k = q.data_ptr(), k.data_ptr()
-    p.q_weight = None if q_weight is None else q_weight.data_ptr()
-    p.k_weight = None if k_weight is None else k_weight.data_ptr()
-    p.cos, p.sin = cos.data_ptr(), sin.data_ptr()
-    p.positions = None if positions is None else positions.data_ptr()
-    return held, cos, sin
+    if not plan.direct:
+        q, k, q_weight, k_weight, cos, sin, positions = (_rows(t) for t in (q, k, q_weight, k_weight, cos, sin, positions))
+        if cos.stride(0) != sin.stride(0):
+            cos, sin = cos.contiguous(), sin.contiguous()
+    p.q, p.k, p.cos, p.sin = q.data_ptr(), k.data_ptr(), cos.data_ptr(), sin.data_ptr()
+    if q_weight is not None:
+        p.q_weight = q_weight.data_ptr()
+    if k_weight is not None:
+        p.k_weight = k_weight.data_ptr()
+    if positions is not None:
+        p.positions = positions.data_ptr()
+    return q, k, q_weight, k_weight, cos, sin, positions
 
 
-def _forward(template, q, k, q_weight, k_weight, cos, sin, positions):
-    p = _hip.MfaNormRopeParams.from_buffer_copy(template)
-    held = _fill(p, q, k, q_weight, k_weight, cos, sin, positions)  # noqa: F841 (kept until the launch)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+def _forward(plan, q, k, q_weight, k_weight, cos, sin, positions):
+    p = _hip.MfaNormRopeParams.from_buffer_copy(plan.params)
+    held = _fill(p, plan, q, k, q_weight, k_weight, cos, sin, positions)  # noqa: F841 (kept until the launch)
+    q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
     p.q_out, p.k_out = q_out.data_ptr(), k_out.data_ptr()
-    with _kernel._on(q.device):
-        _hip.norm_rope(p, torch._C._cuda_getCurrentRawStream(q.device.index))
+    _kernel._launch_on(q.device, _hip.norm_rope, p)
     return q_out, k_out
 
 
@@ -162,33 +173,40 @@ class _QkNormRopeFn(torch.autograd.Function):
     q and k (nothing but the inputs is kept)."""
 
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-        template = _signature(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    def forward(ctx, plan, q, k, q_weight, k_weight, cos, sin, positions):
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.template = template
-        return _forward(template, q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.plan = plan
+        return _forward(plan, q, k, q_weight, k_weight, cos, sin, positions)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+        plan, device = ctx.plan, q.device
         b = _hip.MfaNormRopeBwdParams()
-        b.fwd = ctx.template
-        held = _fill(b.fwd, q, k, q_weight, k_weight, cos, sin, positions)  # noqa: F841 (kept until the launch)
-        dq_out, dk_out = _rows(dq_out.to(q.dtype)), _rows(dk_out.to(k.dtype))
+        b.fwd = plan.params
+        held = _fill(b.fwd, plan, q, k, q_weight, k_weight, cos, sin, positions)  # noqa: F841 (kept until the launch)
+        if dq_out.dtype is not q.dtype or dq_out.stride(-1) != 1:
+            dq_out = _rows(dq_out.to(q.dtype))
+        if dk_out.dtype is not k.dtype or dk_out.stride(-1) != 1:
+            dk_out = _rows(dk_out.to(k.dtype))
         b.dq_out, b.dk_out = dq_out.data_ptr(), dk_out.data_ptr()
         b.dqo_batch_stride, b.dqo_seq_stride, b.dqo_head_stride = _strides(dq_out)
         b.dko_batch_stride, b.dko_seq_stride, b.dko_head_stride = _strides(dk_out)
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
         b.dq, b.dk = dq.data_ptr(), dk.data_ptr()
-        dw = [None, None]
-        for i, w in enumerate((q_weight, k_weight)):
-            if w is not None and ctx.needs_input_grad[2 + i]:
-                dw[i] = torch.empty(w.shape, dtype=w.dtype, device=w.device)
-        b.dq_weight, b.dk_weight = (None if d is None else d.data_ptr() for d in dw)
-        with _kernel._on(q.device):
-            nbytes = _hip.norm_rope_bwd_workspace_bytes(b)
-            ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=q.device)
-            _hip.norm_rope_bwd(b, ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(q.device.index))
-        return dq, dk, dw[0], dw[1], None, None, None, None, None
+        dqw = q_weight.new_empty(q_weight.shape) if q_weight is not None and ctx.needs_input_grad[3] else None
+        dkw = k_weight.new_empty(k_weight.shape) if k_weight is not None and ctx.needs_input_grad[4] else None
+        if dqw is not None:
+            b.dq_weight = dqw.data_ptr()
+        if dkw is not None:
+            b.dk_weight = dkw.data_ptr()
+        which = (dqw is not None, dkw is not None)
+        nbytes = plan.ws.get(which)
+        if nbytes is None:
+            with _kernel._on(device):
+                nbytes = _hip.norm_rope_bwd_workspace_bytes(b)
+            plan.ws[which] = nbytes
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        _kernel._launch_on(device, _hip.norm_rope_bwd, b, None if ws is None else ws.data_ptr(), nbytes)
+        return None, dq, dk, dqw, dkw, None, None, None
