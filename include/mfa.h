@@ -522,7 +522,7 @@ typedef struct mfa_norm_rope_params {
     int32_t positions_64, interleaved;
     int32_t dtype;        /* of q, k and the outputs */
     int32_t dtype_weight; /* of the weights and their gradients */
-    int32_t dtype_table;  /* of cos and sin */
+    int32_t dtype_table;  /* of cos and sin: dtype or MFA_DTYPE_F32 */
     float eps;
 } mfa_norm_rope_params;
 int mfa_norm_rope(const mfa_norm_rope_params* params, void* stream);

@@ -25,13 +25,14 @@
 namespace {
 
 constexpr int kNThreads = 256;
-#ifndef MFA_NORM_BLOCKS
-#define MFA_NORM_BLOCKS 1024
-#endif
-#ifndef MFA_NORM_FWD
-#define MFA_NORM_FWD 16
-#endif
-constexpr int kNMaxBlocks = MFA_NORM_BLOCKS;  // workgroups of the backward per tensor (partial weight sums)
+// Workgroups per tensor: a row per lane group up to here, then walks.  Few, as a
+// workgroup's start (weights, first positions, first angles) is a chain of loads:
+// 8192 tokens of 16 + 16 heads of 128 in bf16 take 27.8 us forward with 768 (3 per
+// CU; 35.0 with 4096, 30.2 with 512) and 41.9 us backward with 640 (47.8 with 1024,
+// 44.9 with 512, 53 with 256), 4.8 TB/s where a large copy reaches 5.15; two rows
+// of a lane group in flight at once measured 27.5 and 44.3.
+constexpr int kNFwdPerCu = 3;
+constexpr int kNMaxBlocks = 640;  // (backward: each leaves a partial sum of the weight gradients)
 enum { kHalf = 0, kInterleaved = 1, kAny = 2 };
 
 struct NTensor {
@@ -49,8 +50,8 @@ struct NArgs {
     const char* cos;
     const char* sin;
     int64_t table_stride;
-    const char* pos;
-    int64_t pos_b;
+    const uint32_t* pos;  // 32-bit words
+    int64_t pos_b;        // elements
     int32_t pos64, table_rows;
     int32_t L, D, rot;
     FastDiv by_l;
@@ -112,6 +113,32 @@ __device__ __forceinline__ void store4(char* p, const float* x) {
     }
 }
 
+// what is loaded in place of a position or a table row that is not there
+__device__ const uint32_t kZeros[64] = {0};
+
+// Token and head of a row, and the table row of the token's position.
+struct Where {
+    int b, i, h;
+    int64_t row;
+    bool ok;  // the position is in the table
+};
+__device__ __forceinline__ Where where_of(const NArgs& a, const NTensor& t, int64_t r) {
+    Where w;
+    const uint32_t tok = quotient((uint32_t)r, t.by_h);
+    w.h = (int)((uint32_t)r - tok * (uint32_t)t.H);
+    w.b = (int)quotient(tok, a.by_l);
+    w.i = (int)(tok - (uint32_t)w.b * (uint32_t)a.L);
+    // (low and high word of an int64, the word twice of an int32; without positions
+    // a zero is loaded, and the token's place counts)
+    const uint32_t* p = a.pos ? a.pos : kZeros;
+    const int64_t at = a.pos ? (w.b * a.pos_b + w.i) << a.pos64 : 0;
+    const uint32_t lo = p[at], hi = p[at + a.pos64];
+    const uint32_t pos = a.pos ? lo : (uint32_t)w.i;
+    w.ok = pos < (uint32_t)a.table_rows && (!a.pos64 || hi == 0);
+    w.row = w.ok ? pos : 0;
+    return w;
+}
+
 // A lane's elements: pair i of its four is (x[i], x[4 + i]).
 template <int MODE, int LPR>
 struct Lane {
@@ -125,12 +152,12 @@ struct Lane {
         const int nr = a.rot / 8;  // lanes of the rotated part
         turn = sub < nr;
         in = MODE == kAny || sub < a.D / 8;
-        p0 = 4 * sub;
+        p0 = turn ? 4 * sub : 0;
         if (MODE == kHalf && turn) {
             d0 = 4 * sub;
             d1 = a.rot / 2 + 4 * sub;
         } else {
-            d0 = 8 * sub;
+            d0 = in ? 8 * sub : 0;
             d1 = d0 + 4;
         }
     }
@@ -150,17 +177,13 @@ struct Lane {
                 x[i] = d >= 0 ? load1<DT>(row + d * ES) : 0.f;
             }
         } else {
-            if (in) {
-                float u[8];
-                load4<DT>(row + d0 * ES, u);
-                load4<DT>(row + d1 * ES, u + 4);
-                // (interleaved: adjacent elements are the pairs)
+            // (a lane without elements loads the row's first ones and drops them)
+            float u[8];
+            load4<DT>(row + d0 * ES, u);
+            load4<DT>(row + d1 * ES, u + 4);
+            // (interleaved: adjacent elements are the pairs)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[MODE == kInterleaved ? 4 * (i & 1) + (i >> 1) : i] = u[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = 0.f;
-            }
+            for (int i = 0; i < 8; ++i) x[MODE == kInterleaved ? 4 * (i & 1) + (i >> 1) : i] = in ? u[i] : 0.f;
         }
     }
     template <int DT>
@@ -195,37 +218,33 @@ struct Lane {
         }
     }
     // cosine and sine of the lane's pairs (1 and 0 where not rotated, NaN at a
-    // position outside the table)
-    __device__ __forceinline__ void angles(const NArgs& a, int64_t pos, float (&c)[4], float (&s)[4]) const {
-        const bool ok = pos >= 0 && pos < a.table_rows;
-        const int64_t row = pos * a.table_stride;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            c[i] = 1.f;
-            s[i] = 0.f;
-        }
+    // position outside the table); TDT: the tables' type
+    template <int TDT>
+    __device__ __forceinline__ void angles(const NArgs& a, const Where& w, float (&c)[4], float (&s)[4]) const {
+        constexpr int TS = TDT == MFA_DTYPE_F32 ? 4 : 2;
+        const float off = w.ok ? 0.f : __builtin_nanf("");
         if constexpr (MODE != kAny) {
-            if (!turn) return;
-            if (!ok) {
+            // (without branches: these loads run beside the elements';
+            // zeros stand for a table that has no rows or columns)
+            const bool some = a.table_rows > 0 && a.rot > 0;
+            const char* cos = some ? a.cos : reinterpret_cast<const char*>(kZeros);
+            const char* sin = some ? a.sin : reinterpret_cast<const char*>(kZeros);
+            load4<TDT>(cos + (w.row * a.table_stride + p0) * TS, c);
+            load4<TDT>(sin + (w.row * a.table_stride + p0) * TS, s);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) c[i] = s[i] = __builtin_nanf("");
-            } else if (a.tdt == MFA_DTYPE_F32) {
-                load4<MFA_DTYPE_F32>(a.cos + (row + p0) * 4, c);
-                load4<MFA_DTYPE_F32>(a.sin + (row + p0) * 4, s);
-            } else if (a.tdt == MFA_DTYPE_BF16) {
-                load4<MFA_DTYPE_BF16>(a.cos + (row + p0) * 2, c);
-                load4<MFA_DTYPE_BF16>(a.sin + (row + p0) * 2, s);
-            } else {
-                load4<MFA_DTYPE_F16>(a.cos + (row + p0) * 2, c);
-                load4<MFA_DTYPE_F16>(a.sin + (row + p0) * 2, s);
+            for (int i = 0; i < 4; ++i) {
+                c[i] = turn ? c[i] + off : 1.f;
+                s[i] = turn ? s[i] + off : 0.f;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int p = sub + LPR * i;
+                c[i] = 1.f;
+                s[i] = 0.f;
                 if (p >= a.rot / 2) continue;
-                c[i] = ok ? load1(a.cos, row + p, a.tdt) : __builtin_nanf("");
-                s[i] = ok ? load1(a.sin, row + p, a.tdt) : __builtin_nanf("");
+                c[i] = w.ok ? load1<TDT>(a.cos + (w.row * a.table_stride + p) * TS) : off;
+                s[i] = w.ok ? load1<TDT>(a.sin + (w.row * a.table_stride + p) * TS) : off;
             }
         }
     }
@@ -241,70 +260,38 @@ __device__ __forceinline__ float sum8(const float (&x)[8]) {
     return ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 }
 
-// Token and head of a row, and the token's position.
-struct Row {
-    int b, i, h;
-    int64_t pos;
-};
-__device__ __forceinline__ Row row_of(const NArgs& a, const NTensor& t, int64_t r) {
-    Row w;
-    const uint32_t tok = quotient((uint32_t)r, t.by_h);
-    w.h = (int)((uint32_t)r - tok * (uint32_t)t.H);
-    w.b = (int)quotient(tok, a.by_l);
-    w.i = (int)(tok - (uint32_t)w.b * (uint32_t)a.L);
-    const int64_t at = w.b * a.pos_b + w.i;
-    w.pos = !a.pos ? w.i : a.pos64 ? reinterpret_cast<const int64_t*>(a.pos)[at] : reinterpret_cast<const int32_t*>(a.pos)[at];
-    return w;
-}
-
-// rows of a lane group whose loads are in flight together
-#ifndef MFA_NORM_ROWS
-#define MFA_NORM_ROWS 2
-#endif
-template <int DT, int MODE, int LPR>
+template <int DT, int TDT, int MODE, int LPR>
 __global__ void __launch_bounds__(kNThreads) mfa_norm_rope_kernel(NArgs a) {
     constexpr int ES = DT == MFA_DTYPE_F32 ? 4 : 2;
-    constexpr int kRows = MODE == kAny ? 1 : MFA_NORM_ROWS;
+    constexpr int RPB = kNThreads / LPR;
     const Lane<MODE, LPR> ln(a);
     const int which = blockIdx.x >= (unsigned)a.blocks[0];
     const NTensor& t = a.t[which];
     const int64_t blk = blockIdx.x - (which ? a.blocks[0] : 0);
     float w[8];
     ln.weights(a, t.w, w);
-    const int64_t step = (int64_t)a.blocks[which] * (kNThreads / LPR);
-    for (int64_t r0 = blk * (kNThreads / LPR) + threadIdx.x / LPR; r0 < t.rows; r0 += kRows * step) {
-        float x[kRows][8], c[kRows][4], s[kRows][4];
+    for (int64_t r = blk * RPB + threadIdx.x / LPR; r < t.rows; r += (int64_t)a.blocks[which] * RPB) {
+        const Where at = where_of(a, t, r);
+        float x[8], c[4], s[4], sq[8], y[8];
+        ln.template load<DT>(a, t.x + (at.b * t.xb + at.i * t.xs + at.h * t.xh) * ES, x);
+        ln.template angles<TDT>(a, at, c, s);
 #pragma unroll
-        for (int u = 0; u < kRows; ++u) {
-            const int64_t r = min(r0 + u * step, t.rows - 1);
-            const Row row = row_of(a, t, r);
-            ln.template load<DT>(a, t.x + (row.b * t.xb + row.i * t.xs + row.h * t.xh) * ES, x[u]);
-            ln.angles(a, row.pos, c[u], s[u]);
+        for (int i = 0; i < 8; ++i) sq[i] = x[i] * x[i];
+        const float rs = rsqrtf(fmaf(row_sum<LPR>(sum8(sq)), a.inv_d, a.eps));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float u = x[i] * rs * w[i], v = x[4 + i] * rs * w[4 + i];
+            y[i] = u * c[i] - v * s[i];
+            y[4 + i] = v * c[i] + u * s[i];
         }
-#pragma unroll
-        for (int u = 0; u < kRows; ++u) {
-            float sq[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sq[i] = x[u][i] * x[u][i];
-            const float rs = rsqrtf(fmaf(row_sum<LPR>(sum8(sq)), a.inv_d, a.eps));
-            float y[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = x[u][i] * rs * w[i], q = x[u][4 + i] * rs * w[4 + i];
-                y[i] = p * c[u][i] - q * s[u][i];
-                y[4 + i] = q * c[u][i] + p * s[u][i];
-            }
-            const int64_t r = r0 + u * step;
-            if (u == 0 || r < t.rows) ln.template store<DT>(a, t.out + r * a.D * ES, y);
-        }
+        ln.template store<DT>(a, t.out + r * a.D * ES, y);
     }
 }
 
-template <int DT, int MODE, int LPR>
+template <int DT, int TDT, int MODE, int LPR>
 __global__ void __launch_bounds__(kNThreads) mfa_norm_rope_bwd_kernel(NArgs a) {
     constexpr int ES = DT == MFA_DTYPE_F32 ? 4 : 2;
     constexpr int RPB = kNThreads / LPR;
-    constexpr int kRows = MODE == kAny ? 1 : MFA_NORM_ROWS;
     __shared__ float sh[4][128];
     const Lane<MODE, LPR> ln(a);
     const int which = blockIdx.x >= (unsigned)a.blocks[0];
@@ -314,46 +301,32 @@ __global__ void __launch_bounds__(kNThreads) mfa_norm_rope_bwd_kernel(NArgs a) {
     ln.weights(a, t.w, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[i] = 0.f;
-    const int64_t step = (int64_t)a.blocks[which] * RPB;
-    for (int64_t r0 = blk * RPB + threadIdx.x / LPR; r0 < t.rows; r0 += kRows * step) {
-        float xs[kRows][8], gs[kRows][8], cs[kRows][4], ss[kRows][4];
+    for (int64_t r = blk * RPB + threadIdx.x / LPR; r < t.rows; r += (int64_t)a.blocks[which] * RPB) {
+        const Where at = where_of(a, t, r);
+        float x[8], g[8], c[4], s[4], sq[8], hn[8];
+        ln.template load<DT>(a, t.x + (at.b * t.xb + at.i * t.xs + at.h * t.xh) * ES, x);
+        ln.template load<DT>(a, t.g + (at.b * t.gb + at.i * t.gs + at.h * t.gh) * ES, g);
+        ln.template angles<TDT>(a, at, c, s);
 #pragma unroll
-        for (int u = 0; u < kRows; ++u) {
-            const int64_t r = min(r0 + u * step, t.rows - 1);
-            const Row row = row_of(a, t, r);
-            ln.template load<DT>(a, t.x + (row.b * t.xb + row.i * t.xs + row.h * t.xh) * ES, xs[u]);
-            ln.template load<DT>(a, t.g + (row.b * t.gb + row.i * t.gs + row.h * t.gh) * ES, gs[u]);
-            ln.angles(a, row.pos, cs[u], ss[u]);
+        for (int i = 0; i < 8; ++i) sq[i] = x[i] * x[i];
+        const float rs = rsqrtf(fmaf(row_sum<LPR>(sum8(sq)), a.inv_d, a.eps));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // g turned back, then g w n
+            const float u = g[i] * c[i] + g[4 + i] * s[i], v = g[4 + i] * c[i] - g[i] * s[i];
+            g[i] = u;
+            g[4 + i] = v;
         }
 #pragma unroll
-        for (int u = 0; u < kRows; ++u) {
-            float(&x)[8] = xs[u];
-            float(&g)[8] = gs[u];
-            const int64_t r = r0 + u * step;
-            const bool in = u == 0 || r < t.rows;
-            float sq[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sq[i] = x[i] * x[i];
-            const float rs = rsqrtf(fmaf(row_sum<LPR>(sum8(sq)), a.inv_d, a.eps));
-            float hn[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {  // g turned back, then g w n
-                const float p = g[i] * cs[u][i] + g[4 + i] * ss[u][i], q = g[4 + i] * cs[u][i] - g[i] * ss[u][i];
-                g[i] = p;
-                g[4 + i] = q;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] *= rs;
-                if (in) dw[i] = fmaf(g[i], x[i], dw[i]);
-                g[i] *= w[i];
-                hn[i] = g[i] * x[i];
-            }
-            const float mean = row_sum<LPR>(sum8(hn)) * a.inv_d;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = rs * fmaf(-x[i], mean, g[i]);
-            if (in) ln.template store<DT>(a, t.out + r * a.D * ES, x);
+        for (int i = 0; i < 8; ++i) {
+            x[i] *= rs;
+            dw[i] = fmaf(g[i], x[i], dw[i]);
+            g[i] *= w[i];
+            hn[i] = g[i] * x[i];
         }
+        const float mean = row_sum<LPR>(sum8(hn)) * a.inv_d;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = rs * fmaf(-x[i], mean, g[i]);
+        ln.template store<DT>(a, t.out + r * a.D * ES, x);
     }
     if (!a.dw[which]) return;
     // the workgroup's sums: over the rows of a wavefront, then over wavefronts
@@ -404,19 +377,24 @@ __global__ void __launch_bounds__(kNThreads) mfa_norm_rope_dw_kernel(NArgs a) {
 }
 
 typedef void (*n_fn)(NArgs);
-template <int DT, int MODE>
+template <int DT, int TDT, int MODE>
 n_fn pick(bool bwd, int lpr) {
     switch (lpr) {
-        case 4: return bwd ? mfa_norm_rope_bwd_kernel<DT, MODE, 4> : mfa_norm_rope_kernel<DT, MODE, 4>;
-        case 8: return bwd ? mfa_norm_rope_bwd_kernel<DT, MODE, 8> : mfa_norm_rope_kernel<DT, MODE, 8>;
-        default: return bwd ? mfa_norm_rope_bwd_kernel<DT, MODE, 16> : mfa_norm_rope_kernel<DT, MODE, 16>;
+        case 4: return bwd ? mfa_norm_rope_bwd_kernel<DT, TDT, MODE, 4> : mfa_norm_rope_kernel<DT, TDT, MODE, 4>;
+        case 8: return bwd ? mfa_norm_rope_bwd_kernel<DT, TDT, MODE, 8> : mfa_norm_rope_kernel<DT, TDT, MODE, 8>;
+        default: return bwd ? mfa_norm_rope_bwd_kernel<DT, TDT, MODE, 16> : mfa_norm_rope_kernel<DT, TDT, MODE, 16>;
     }
 }
-template <int DT>
+template <int DT, int TDT>
 n_fn pick(bool bwd, int mode, int lpr) {
-    if (mode == kHalf) return pick<DT, kHalf>(bwd, lpr);
-    if (mode == kInterleaved) return pick<DT, kInterleaved>(bwd, lpr);
-    return bwd ? mfa_norm_rope_bwd_kernel<DT, kAny, 16> : mfa_norm_rope_kernel<DT, kAny, 16>;
+    if (mode == kHalf) return pick<DT, TDT, kHalf>(bwd, lpr);
+    if (mode == kInterleaved) return pick<DT, TDT, kInterleaved>(bwd, lpr);
+    return bwd ? mfa_norm_rope_bwd_kernel<DT, TDT, kAny, 16> : mfa_norm_rope_kernel<DT, TDT, kAny, 16>;
+}
+// tables in fp32 or in the tensors' type
+template <int DT>
+n_fn pick_tables(bool bwd, int tdt, int mode, int lpr) {
+    return tdt == MFA_DTYPE_F32 ? pick<DT, MFA_DTYPE_F32>(bwd, mode, lpr) : pick<DT, DT>(bwd, mode, lpr);
 }
 
 int nerr(int code, const char* fmt, ...) {
@@ -436,7 +414,7 @@ struct NPlan {
 
 // b: NULL forward
 int n_plan(const mfa_norm_rope_params* p, const mfa_norm_rope_bwd_params* b, NPlan* plan, const char* who, int cus) {
-    if (!known(p->dtype) || !known(p->dtype_weight) || !known(p->dtype_table))
+    if (!known(p->dtype) || !known(p->dtype_weight) || (p->dtype_table != p->dtype && p->dtype_table != MFA_DTYPE_F32))
         return nerr(MFA_ERR_INVALID, "%s: unknown dtype (%d, weight %d, table %d)", who, p->dtype, p->dtype_weight, p->dtype_table);
     if (p->batch < 0 || p->seqlen < 0 || p->heads_q < 0 || p->heads_kv < 0 || p->table_rows < 0)
         return nerr(MFA_ERR_INVALID, "%s: negative size", who);
@@ -494,7 +472,7 @@ int n_plan(const mfa_norm_rope_params* p, const mfa_norm_rope_bwd_params* b, NPl
     a.cos = static_cast<const char*>(p->cos);
     a.sin = static_cast<const char*>(p->sin);
     a.table_stride = p->table_stride;
-    a.pos = static_cast<const char*>(p->positions);
+    a.pos = static_cast<const uint32_t*>(p->positions);
     a.pos_b = p->positions_batch_stride;
     a.pos64 = p->positions_64 != 0;
     a.table_rows = p->table_rows;
@@ -509,9 +487,7 @@ int n_plan(const mfa_norm_rope_params* p, const mfa_norm_rope_bwd_params* b, NPl
     a.inv_d = 1.f / p->head_dim;
     plan->mode = !whole ? kAny : p->interleaved ? kInterleaved : kHalf;
     plan->lpr = plan->mode == kAny ? 16 : p->head_dim <= 32 ? 4 : p->head_dim <= 64 ? 8 : 16;
-    // forward: a row per lane group, up to 16 workgroups per CU, then a walk;
-    // backward: fewer workgroups, each one partial sum of the weight gradients
-    const int64_t rpb = kNThreads / plan->lpr, most = b ? kNMaxBlocks : (int64_t)cus * MFA_NORM_FWD;
+    const int64_t rpb = kNThreads / plan->lpr, most = b ? kNMaxBlocks : (int64_t)cus * kNFwdPerCu;
     for (int i = 0; i < 2; ++i) a.blocks[i] = (int32_t)std::min<int64_t>((a.t[i].rows + rpb - 1) / rpb, most);
     if (b) {
         a.dw[0] = p->q_weight ? static_cast<char*>(b->dq_weight) : nullptr;
@@ -530,9 +506,10 @@ int64_t n_ws_bytes(const NPlan& plan) {
 }
 
 void n_launch(const NPlan& plan, bool bwd, int dtype, hipStream_t st) {
-    const n_fn fn = dtype == MFA_DTYPE_F32    ? pick<MFA_DTYPE_F32>(bwd, plan.mode, plan.lpr)
-                    : dtype == MFA_DTYPE_BF16 ? pick<MFA_DTYPE_BF16>(bwd, plan.mode, plan.lpr)
-                                              : pick<MFA_DTYPE_F16>(bwd, plan.mode, plan.lpr);
+    const int tdt = plan.a.tdt;
+    const n_fn fn = dtype == MFA_DTYPE_F32    ? pick_tables<MFA_DTYPE_F32>(bwd, tdt, plan.mode, plan.lpr)
+                    : dtype == MFA_DTYPE_BF16 ? pick_tables<MFA_DTYPE_BF16>(bwd, tdt, plan.mode, plan.lpr)
+                                              : pick_tables<MFA_DTYPE_F16>(bwd, tdt, plan.mode, plan.lpr);
     hipLaunchKernelGGL(fn, dim3(plan.a.blocks[0] + plan.a.blocks[1]), dim3(kNThreads), 0, st, plan.a);
 }
 
