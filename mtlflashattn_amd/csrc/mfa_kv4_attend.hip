@@ -16,7 +16,9 @@
 //    S^T = K Q^T with v_mfma_f32_16x16x32_bf16: lane = column, registers = keys;
 //  * turns V into bf16 rows in LDS, whose transposed operand is read with
 //    ds_read_b64_tr_b16, and adds O^T += V^T P^T.
-// The codes of the next kStages blocks are on their way into registers meanwhile.
+// The codes of the next block are on their way into registers from the moment the
+// current one's are consumed (two blocks ahead took the registers of the third
+// workgroup of a CU: below).
 // fp16 queries are two bf16 terms (exact), and probabilities are two bf16 terms,
 // hi = round(p) and lo = round(p - hi): a row over thousands of near-equal
 // weights averages V, and one 16-bit rounding of every weight would be visible
@@ -72,35 +74,39 @@ struct Block4 {
     uint8_t vs[VG];
 };
 
-// buffer loads, non-temporal (AUX 2) or not (0)
-template <int AUX, int DP>
+// Non-temporal buffer loads: a unit holds all columns of its K/V head, so a byte
+// of the cache is read once a call (64 sequences of 512 to 16384 keys, Hq=32
+// Hkv=8 D=128 bf16: 104.6 us, 108.9 with ordinary loads; 31 of 256 to 4096, which the
+// last-level cache holds from call to call: 22.9 and 22.4 us).
+constexpr int kOnce4 = 2;
+template <int DP>
 __device__ __forceinline__ void load_block4(Block4<DP>& w, const __amdgpu_buffer_rsrc_t (&rs)[4], const uint32_t (&koff)[2],
                                             const uint32_t (&ksoff)[2][2], const uint32_t* voff, const uint32_t* vsoff,
                                             uint32_t kr, uint32_t ksr, uint32_t vr, uint32_t vsr) {
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
         if constexpr (DP == 128) {
-            const u32x4_t y = __builtin_amdgcn_raw_buffer_load_b128(rs[0], koff[kk] + kr, 0, AUX);
+            const u32x4_t y = __builtin_amdgcn_raw_buffer_load_b128(rs[0], koff[kk] + kr, 0, kOnce4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) w.k[kk][i] = y[i];
         } else if constexpr (DP == 96) {
-            const auto y = __builtin_amdgcn_raw_buffer_load_b96(rs[0], koff[kk] + kr, 0, AUX);
+            const auto y = __builtin_amdgcn_raw_buffer_load_b96(rs[0], koff[kk] + kr, 0, kOnce4);
 #pragma unroll
             for (int i = 0; i < 3; ++i) w.k[kk][i] = y[i];
         } else if constexpr (DP == 64) {
-            const auto y = __builtin_amdgcn_raw_buffer_load_b64(rs[0], koff[kk] + kr, 0, AUX);
+            const auto y = __builtin_amdgcn_raw_buffer_load_b64(rs[0], koff[kk] + kr, 0, kOnce4);
             w.k[kk][0] = y[0];
             w.k[kk][1] = y[1];
         } else {
-            w.k[kk][0] = __builtin_amdgcn_raw_buffer_load_b32(rs[0], koff[kk] + kr, 0, AUX);
+            w.k[kk][0] = __builtin_amdgcn_raw_buffer_load_b32(rs[0], koff[kk] + kr, 0, kOnce4);
         }
-        w.ks[kk][0] = __builtin_amdgcn_raw_buffer_load_b8(rs[1], ksoff[kk][0] + ksr, 0, AUX);
-        if constexpr (DP == 96) w.ks[kk][1] = __builtin_amdgcn_raw_buffer_load_b8(rs[1], ksoff[kk][1] + ksr, 0, AUX);
+        w.ks[kk][0] = __builtin_amdgcn_raw_buffer_load_b8(rs[1], ksoff[kk][0] + ksr, 0, kOnce4);
+        if constexpr (DP == 96) w.ks[kk][1] = __builtin_amdgcn_raw_buffer_load_b8(rs[1], ksoff[kk][1] + ksr, 0, kOnce4);
     }
 #pragma unroll
     for (int i = 0; i < Block4<DP>::VG; ++i) {
-        w.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rs[2], voff[i] + vr, 0, AUX);
-        w.vs[i] = __builtin_amdgcn_raw_buffer_load_b8(rs[3], vsoff[i] + vsr, 0, AUX);
+        w.v[i] = __builtin_amdgcn_raw_buffer_load_b128(rs[2], voff[i] + vr, 0, kOnce4);
+        w.vs[i] = __builtin_amdgcn_raw_buffer_load_b8(rs[3], vsoff[i] + vsr, 0, kOnce4);
     }
 }
 
@@ -124,19 +130,17 @@ __device__ __forceinline__ void clear_rest() {
     }
 }
 
-#ifndef MFA_KV4_NT
-#define MFA_KV4_NT 0
-#endif
-#ifndef MFA_KV4_STAGES
-#define MFA_KV4_STAGES 2
-#endif
+// Workgroups per CU, at NT column tiles: as many as the registers hold (the batch
+// above: 98.6 us with three, 107 with two, 118 with four, which spill; at D = 64
+// three and four measure the same).
+constexpr int wgs4(int nt) { return nt == 1 ? 3 : 2; }
+constexpr int kTileWgs4 = 2;  // of 128 columns (a third is dealt work but not resident: 335 us become 369)
 
 template <int DP, int NT, bool IS_BF16>
-__global__ void __launch_bounds__(kThreads4) __attribute__((amdgpu_waves_per_eu(NT == 1 && DP <= 64 ? 3 : 2)))
+__global__ void __launch_bounds__(kThreads4) __attribute__((amdgpu_waves_per_eu(wgs4(NT))))
 mfa_kv4_kernel(K4Args) {
     typedef Block4<DP> Blk;
     constexpr int NQ = IS_BF16 ? 1 : 2;  // bf16 terms of a query
-    constexpr int kStages = NT == 1 ? MFA_KV4_STAGES : 1;  // blocks whose codes are in registers or on their way
     constexpr int KS = DP / 32;          // k-steps of QK^T
     constexpr int DT = DP / 16;          // 16-row tiles of O^T
     constexpr int CPR = DP / 8;          // 16-byte chunks of a bf16 row
@@ -210,7 +214,7 @@ mfa_kv4_kernel(K4Args) {
             const bool on = n < n1;
             const uint32_t kr = on ? row * pg.rstride[0] : 0x80000000u, ksr = on ? row * pg.rstride[1] : 0x80000000u;
             const uint32_t vr = on ? row * pg.rstride[2] : 0x80000000u, vsr = on ? row * pg.rstride[3] : 0x80000000u;
-            load_block4<MFA_KV4_NT * 2, DP>(w, pg.rs, koff, ksoff, voff, vsoff, kr, ksr, vr, vsr);
+            load_block4<DP>(w, pg.rs, koff, ksoff, voff, vsoff, kr, ksr, vr, vsr);
         };
         // ---- queries: lane (column l16, group grp) holds elements
         // grp DP/4 + 8 s .. + 7 of its row as the operand of step s
@@ -239,9 +243,8 @@ mfa_kv4_kernel(K4Args) {
                 }
             }
         }
-        Blk blk[kStages];
-#pragma unroll
-        for (int z = 0; z < kStages; ++z) load(n0 + z, blk[z]);
+        Blk blk;
+        load(n0, blk);
         // (waited for here: a wait inside the loop would drain the codes' loads too)
 #pragma unroll
         for (int t = 0; t < NT; ++t) pin(slope[t]);
@@ -319,11 +322,16 @@ mfa_kv4_kernel(K4Args) {
                             st[t][kk] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, query(t, z, s), st[t][kk], 0, 0, 0);
                 }
             }
-            // V to LDS as bf16 rows
+            // V to LDS as bf16 rows; NaN groups of a block that some column does not
+            // see whole as zeros (below)
+            const bool masked = j < f_lo || j + 31 > f_hi;
+            uint64_t nans[Blk::VG];
 #pragma unroll
             for (int i = 0; i < Blk::VG; ++i) {
+                const bool nan = masked && w.vs[i] == 255;
+                nans[i] = __ballot(nan);
                 if (32 * GPR % 64 == 0 || 64 * i + lane < 32 * GPR) {
-                    const float s = kv4_scale(w.vs[i]);
+                    const float s = nan ? 0.f : kv4_scale(w.vs[i]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         *reinterpret_cast<u32x4_t*>(vt + vrow[i] * DP + (((4 * vgrp[i] + e) ^ vswz(vrow[i])) << 3)) =
@@ -332,7 +340,6 @@ mfa_kv4_kernel(K4Args) {
             }
             refill();
             u32x4_t ph[NT], pl[NT];
-            const bool masked = j < f_lo || j + 31 > f_hi;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 f32x4_t(&s)[2] = st[t];
@@ -407,19 +414,28 @@ mfa_kv4_kernel(K4Args) {
                     o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8_t, pl[t]), o[t][d], 0, 0, 0);
                 }
             }
+            // NaN groups for the columns that see their keys (a product with the zero
+            // weight of a masked key would reach the others too)
+#pragma unroll
+            for (int i = 0; i < Blk::VG; ++i) {
+                for (uint64_t x = nans[i]; x; x &= x - 1) {
+                    const int cc = 64 * i + __builtin_ctzll(x), row = cc / GPR;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const bool sees = j + row >= lo[t] && j + row <= hi[t];
+#pragma unroll
+                        for (int g = 0; g < GPR; ++g) {
+                            float y = sees && g == cc - row * GPR ? __builtin_nanf("") : 0.f;
+                            pin(y);  // (no indexing of o by the group)
+                            o[t][2 * g] += y;
+                            o[t][2 * g + 1] += y;
+                        }
+                    }
+                }
+            }
         };
 
-        // (whole rounds of stages, then the rest: every way round the loop issues the
-        // same loads, so the waits count exactly)
-        int n = n0;
-        for (; n + kStages <= n1; n += kStages) {
-#pragma unroll
-            for (int z = 0; z < kStages; ++z)
-                compute(key0 + (n + z) * kChunk4, blk[z], [&]() { load(n + z + kStages, blk[z]); });
-        }
-#pragma unroll
-        for (int z = 0; z < kStages - 1; ++z)
-            if (n + z < n1) compute(key0 + (n + z) * kChunk4, blk[z], [] {});
+        for (int n = n0; n < n1; ++n) compute(key0 + n * kChunk4, blk, [&]() { load(n + 1, blk); });
 
         // ---- the four wavefronts' sums, 16 columns at a time through their V
         // tiles: elements 4 c .. of column r at 4 (c ^ (r mod 8))
@@ -548,9 +564,6 @@ __global__ void __launch_bounds__(kThreads4) mfa_kv4_merge_kernel(K4Args, K4Args
 static_assert(kMergeCols * (MFA_MAX_HEAD_DIM / 4) <= kThreads4, "a thread per four elements");
 
 typedef void (*k4_fn)(K4Args);
-#ifndef MFA_KV4_WGS
-#define MFA_KV4_WGS 2
-#endif
 typedef void (*k4_merge_fn)(K4Args, K4Args);
 struct K4Kernels {
     k4_fn attend;
@@ -685,7 +698,7 @@ int k4_plan(const mfa_kv4_fwd_params* p, K4Plan* plan, int cus) {
                                                    : (cols + l.a.cols - 1) / l.a.cols + std::min<int64_t>(p->batch, rows);
         const int64_t units = tiles * a.Hkv;
         if (units > 0x3fffffff || units * chunks > 0x7fffffffLL) return k4err(MFA_ERR_INVALID, "mfa_kv4_fwd: problem too large");
-        l.a.G = (int32_t)std::min<int64_t>(units * chunks, (int64_t)cus * MFA_KV4_WGS);
+        l.a.G = (int32_t)std::min<int64_t>(units * chunks, (int64_t)cus * (l.a.cols == kTileCols4 ? kTileWgs4 : wgs4(l.a.cols / 16)));
         // (neighbouring tiles of a K/V head share its rows in their XCD's L2)
         l.a.xcds = l.a.cols == kTileCols4 && l.a.G % 8 == 0 ? 8 : 1;
         l.parts = chunks > 1 ? (int64_t)l.a.G * 2 * l.a.cols : 0;

@@ -45,6 +45,7 @@ mfa_kv4_tile_kernel(K4Args) {
     __shared__ __attribute__((aligned(16))) uint16_t smem[R_ELEMS > K_ELEMS + V_ELEMS ? R_ELEMS : K_ELEMS + V_ELEMS];
     uint16_t* const ktile = smem;
     uint16_t* const vtile = smem + K_ELEMS;
+    __shared__ uint64_t nan_s[GPR];  // NaN groups of a block's V, a bit each
 
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -87,6 +88,7 @@ mfa_kv4_tile_kernel(K4Args) {
         const int wcol = wk.col0 + 32 * wave, wlast = min(wcol + 32, wk.col0 + wk.ncol) - 1;
         const bool live = wlast >= wcol;
         const int wi0 = (int)div4(wcol, a.by_r), wi1 = (int)div4(max(wlast, wcol), a.by_r);
+        const int a_lo = lo4(a.wl, i_last + dq), a_hi = hi4(a.causal, a.wr, i_first + dq, Lk);  // of every column of the tile
         const int w_lo = lo4(a.wl, wi0 + dq), w_hi = hi4(a.causal, a.wr, wi1 + dq, Lk);    // of any column
         const int f_lo = lo4(a.wl, wi1 + dq), f_hi = hi4(a.causal, a.wr, wi0 + dq, Lk);    // of every column
         // (a lane behind the last column holds zero queries and stores nothing)
@@ -124,12 +126,19 @@ mfa_kv4_tile_kernel(K4Args) {
                 gs[i] = __builtin_amdgcn_raw_buffer_load_b8(gv[i] ? pg.rs[3] : pg.rs[1], gsoff[i] + (uint32_t)(row * pg.rstride[x + 1]), 0, 0);
             }
         };
-        auto swrite = [&]() {
+        // part: some column of the tile does not see the whole block
+        auto swrite = [&](bool part) {
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
                 if (GROUPS % kThreads4 == 0 || tid + kThreads4 * i < GROUPS) {
                     uint16_t* p = smem + glds[i];
-                    const float s = kv4_scale(gs[i]);
+                    float s = kv4_scale(gs[i]);
+                    if (part && gv[i]) {
+                        const bool nan = gs[i] == 255;
+                        const uint64_t nans = __ballot(nan);
+                        if (lane == 0) nan_s[(tid + kThreads4 * i - kTK * GPR) >> 6] = nans;
+                        s = nan ? 0.f : s;
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         *reinterpret_cast<u32x4_t*>(p + 8 * (e ^ gsw[i])) = IS_BF16 ? kv4_bf16x8(gc[i][e], s) : kv4_f16x8(gc[i][e], s);
@@ -268,16 +277,41 @@ mfa_kv4_tile_kernel(K4Args) {
             l += acc[0] + acc[1];
         };
 
+        // NaN groups for the columns that see their keys (a product with the zero weight
+        // of a masked key would reach the others too)
+        auto nan_groups = [&](int j) {
+#pragma unroll
+            for (int i = 0; i < GPR; ++i) {
+                for (uint64_t x = nan_s[i]; x; x &= x - 1) {
+                    const int u = __builtin_amdgcn_readfirstlane(64 * i + __builtin_ctzll(x)), row = u / GPR;
+                    K4Const& b = args4();
+                    const int lo = lo4(b.wl, center), hi = hi4(b.causal, b.wr, center, Lk);
+                    const bool sees = j + row >= lo && j + row <= hi;
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        float y = sees && db == u - row * GPR ? __builtin_nanf("") : 0.f;
+                        pin(y);  // (no indexing of o by the group)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[db][r] += y;
+                    }
+                }
+            }
+        };
+
         if (jbeg < jend) gload(jbeg);
         // (waited for here: a wait inside the loop would drain the codes' loads too)
 #pragma unroll
         for (int s = 0; s < DS; ++s) pin(qf[s]);
         pin(slope);
         for (int j = jbeg; j < jend; j += kTK) {
-            swrite();
+            const bool part = j < a_lo || j + kTK - 1 > a_hi;
+            swrite(part);
             if (j + kTK < jend) gload(j + kTK);
             __syncthreads();
-            if (live && j <= w_hi && j + kTK - 1 >= w_lo) block(j < f_lo || j + kTK - 1 > f_hi, j);
+            if (live && j <= w_hi && j + kTK - 1 >= w_lo) {
+                block(j < f_lo || j + kTK - 1 > f_hi, j);
+                if (part) nan_groups(j);
+            }
             __syncthreads();
         }
 

@@ -325,3 +325,31 @@ def test_row_offsets_past_32_bits():
     ref = mfa.flash_attn_kv4_func(q, small_k, small_v, lens, table, causal=True)
     out = mfa.flash_attn_kv4_func(q, *big, lens, table + (pages - 4), causal=True)
     assert torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("lq,Hq,window", [(1, 4, (40, 0)), (5, 4, (-1, 0)), (9, 6, (33, 0)), (70, 4, (-1, 0)), (70, 4, (50, 3)),
+                                          (150, 2, (-1, -1))])
+def test_nan_values_reach_only_the_rows_that_see_them(D, lq, Hq, window):
+    """Groups of V that are NaN: NaN in the rows whose mask holds their key, and in
+    every other row the bits that it has without them."""
+    L = 333
+    q, kc, vc, lens_t, table = make([L], 64, Hq, 2, D, torch.bfloat16, [lq])
+    q = q.view(1, lq, Hq, D)
+    call = lambda: mfa.flash_attn_kv4_func(q, kc, vc, lens_t, table, window_size=window)[0]  # noqa: E731
+    clean = call()
+    i = torch.arange(lq)[:, None] + L - lq
+    j = torch.arange(L)[None]
+    seen = torch.ones(lq, L, dtype=torch.bool)
+    if window[0] >= 0:
+        seen &= j >= i - window[0]
+    if window[1] >= 0:
+        seen &= j <= i + window[1]
+    spots = [(L - 1, 0, 0), (L - lq // 2 - 1, 1, D // 32 - 1), (L - lq, 0, D // 64), (max(L - lq - 36, 0), 1, 0), (258, 0, 0)]
+    want = torch.zeros(lq, Hq, D, dtype=torch.bool)
+    for key, h, grp in spots:
+        vc[1][table[0, key // 64].item(), key % 64, h, grp] = 255
+        want[:, h * Hq // 2:(h + 1) * Hq // 2, 32 * grp:32 * grp + 32] |= seen[:, key][:, None, None]
+    out = call()
+    assert torch.equal(out.isnan().cpu(), want)
+    assert torch.equal(out.cpu()[~want], clean.cpu()[~want])
