@@ -496,7 +496,9 @@ mfa_kv4_kernel(K4Args) {
 // then of the second); a thread holds four elements of a column, and where there
 // are few of them (one or a few columns) groups of threads take every P-th part.
 // Bound by the latency of its loads: a part's reference, sum and elements are
-// loaded at once (no pass for the largest reference first), N parts at a time.
+// loaded at once (no pass for the largest reference first), N parts at a time (4,
+// not 8, for columns that fill the block: 13.6 us instead of 16.5 after a launch of
+// 512 rows over 4096 keys beside 31 decoding sequences).
 constexpr int kMergeCols = 8;
 template <int DP, bool IS_BF16>
 __global__ void __launch_bounds__(kThreads4) mfa_kv4_merge_kernel(K4Args, K4Args) {
@@ -528,7 +530,7 @@ __global__ void __launch_bounds__(kThreads4) mfa_kv4_merge_kernel(K4Args, K4Args
         for (int k = 0; k < 4; ++k) acc[k] = fmaf(y[k], e1, acc[k] * e0);
         m = mn;
     };
-    auto walk = [&](auto ahead) {
+    auto walk = [&](auto ahead, int P) {
         constexpr int N = decltype(ahead)::value;
         for (int v0 = w0 + g; v0 <= w1; v0 += P * N) {
             float2 ml[N];
@@ -545,9 +547,11 @@ __global__ void __launch_bounds__(kThreads4) mfa_kv4_merge_kernel(K4Args, K4Args
         }
     };
     if (w1 - w0 + 1 <= 2 * P)
-        walk(std::integral_constant<int, 2>{});
+        walk(std::integral_constant<int, 2>{}, P);
+    else if (P > 1)
+        walk(std::integral_constant<int, 8>{}, P);
     else
-        walk(std::integral_constant<int, 8>{});
+        walk(std::integral_constant<int, 4>{}, 1);
     if (P > 1) {
         o_s[tid] = acc;
         ml_s[tid] = make_float2(m, l);

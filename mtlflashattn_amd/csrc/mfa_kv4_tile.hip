@@ -196,18 +196,24 @@ mfa_kv4_tile_kernel(K4Args) {
             if constexpr (BIAS) {
                 // natural-log units: x = scale*s, soft-cap c tanh(x/c) =
                 // c - 2c / (exp(2x/c) + 1), ALiBi
+                if (softcap > 0.f) {
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        float x = s[kb][r];
-                        if (softcap > 0.f)
-                            x = fmaf(-2.f * softcap, __builtin_amdgcn_rcpf(fast_exp2(x * softcap_sk) + 1.f), softcap);
-                        else
-                            x *= scale;
-                        if (alibi) x = fmaf(-slope, fabsf((float)(center - (j + 32 * kb + 4 * half) - acc_row(r))), x);
-                        s[kb][r] = x;
+                        for (int r = 0; r < 16; ++r)
+                            s[kb][r] = fmaf(-2.f * softcap, __builtin_amdgcn_rcpf(fast_exp2(s[kb][r] * softcap_sk) + 1.f), softcap);
+                } else {
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) s[kb] *= scale;
+                }
+                if (alibi) {
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) {
+                        const float dist = (float)(center - (j + 32 * kb + 4 * half));
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[kb][r] = fmaf(-slope, fabsf(dist - (float)acc_row(r)), s[kb][r]);
                     }
+                }
             }
             if (masked) {
                 // (the pinned copy keeps the key indices out of the other blocks)
