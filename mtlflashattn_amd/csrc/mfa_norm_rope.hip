@@ -27,10 +27,11 @@ namespace {
 constexpr int kNThreads = 256;
 // Workgroups per tensor: a row per lane group up to here, then walks.  Few, as a
 // workgroup's start (weights, first positions, first angles) is a chain of loads:
-// 8192 tokens of 16 + 16 heads of 128 in bf16 take 27.8 us forward with 768 (3 per
-// CU; 35.0 with 4096, 30.2 with 512) and 41.9 us backward with 640 (47.8 with 1024,
-// 44.9 with 512, 53 with 256), 4.8 TB/s where a large copy reaches 5.15; two rows
-// of a lane group in flight at once measured 27.5 and 44.3.
+// 8192 tokens of 16 + 16 heads of 128 in bf16 took 28.4 us forward with 768 (3 per
+// CU; 35.0 with 4096, 30.2 with 512) and 42.6 us backward with 640 (47.8 with 1024,
+// 44.9 with 512, 53 with 256); two rows of a lane group in flight at once measured
+// 27.5 and 44.3.  With non-temporal stores 27.7 and 39.4 us (4.9 and 5.1 TB/s read
+// and written, a large library copy reaches 5.15).
 constexpr int kNFwdPerCu = 3;
 constexpr int kNMaxBlocks = 640;  // (backward: each leaves a partial sum of the weight gradients)
 enum { kHalf = 0, kInterleaved = 1, kAny = 2 };
@@ -109,7 +110,7 @@ __device__ __forceinline__ void store4(char* p, const float* x) {
             if constexpr (DT == MFA_DTYPE_BF16) v[i] = __builtin_bit_cast(uint32_t, k4_bf16x2_t{(__bf16)x[2 * i], (__bf16)x[2 * i + 1]});
             else v[i] = __builtin_bit_cast(uint32_t, k4_f16x2_t{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]});
         }
-        *reinterpret_cast<u32x2_t*>(p) = v;
+        store_stream(reinterpret_cast<u32x2_t*>(p), v);
     }
 }
 
@@ -487,6 +488,9 @@ int n_plan(const mfa_norm_rope_params* p, const mfa_norm_rope_bwd_params* b, NPl
     a.inv_d = 1.f / p->head_dim;
     plan->mode = !whole ? kAny : p->interleaved ? kInterleaved : kHalf;
     plan->lpr = plan->mode == kAny ? 16 : p->head_dim <= 32 ? 4 : p->head_dim <= 64 ? 8 : 16;
+    const int ws = p->dtype_weight == MFA_DTYPE_F32 ? 4 : 2;
+    if (off(p->q_weight, ws) || off(p->k_weight, ws) || (b && (off(b->dq_weight, ws) || off(b->dk_weight, ws))))
+        return nerr(MFA_ERR_INVALID, "%s: a weight is not aligned to its elements", who);
     const int64_t rpb = kNThreads / plan->lpr, most = b ? kNMaxBlocks : (int64_t)cus * kNFwdPerCu;
     for (int i = 0; i < 2; ++i) a.blocks[i] = (int32_t)std::min<int64_t>((a.t[i].rows + rpb - 1) / rpb, most);
     if (b) {

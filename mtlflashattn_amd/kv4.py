@@ -209,6 +209,9 @@ def _append_plan(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table)
     _check_ints(cache_seqlens, batch, k.device, "cache_seqlens")
     _check_ints(cu_seqlens, batch + 1, k.device, "cu_seqlens")
     _check_table(block_table, batch, k.device)
+    for c in (*k_cache, *v_cache):
+        if any(s == 0 for s, n in zip(c.stride()[:3], c.shape[:3]) if n > 1):
+            raise ValueError("mtlflashattn_amd: an expanded cache (rows that share memory) cannot be written")
     p = _hip.MfaKv4AppendParams()
     _cache_struct(p.cache, k_cache, v_cache, block_table)
     p.k_token_stride, p.k_head_stride = _token_strides(k)
@@ -229,7 +232,8 @@ def flash_attn_kv4_func(q, k_cache, v_cache, cache_seqlens, block_table, softmax
     written).  k_cache, v_cache: (codes, scales) pairs; cache_seqlens: int32 [B], the
     rows of each sequence in the cache, the queries' own included; block_table: int32
     [B, max_pages].  Masks, soft-cap, ALiBi, grouped-query heads as in
-    flash_attn_func; rows with no valid key give 0.  Returns [B, Lq, Hq, D] in q.dtype,
+    flash_attn_func; rows with no valid key give 0, and keys that a row's mask leaves
+    out do not reach it, NaN groups included.  Returns [B, Lq, Hq, D] in q.dtype,
     with return_softmax_lse=True also the log-sum-exp [B, Hq, Lq] fp32.
 
     Lengths and page ids are read on the device (no synchronisation: a call can be
@@ -265,6 +269,10 @@ def flash_attn_varlen_kv4_func(q, k_cache, v_cache, cu_seqlens_q, cache_seqlens,
 def _attend(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap, alibi_slopes,
             max_seqlen_k, return_lse):
     _kernel._check_options(window_size, softcap, alibi_slopes)
+    # (numbers, so that the signature holds a value whatever type it came in)
+    softmax_scale = None if softmax_scale is None else float(softmax_scale)
+    softcap, window_size = float(softcap), (int(window_size[0]), int(window_size[1]))
+    max_seqlen_k = None if max_seqlen_k is None else int(max_seqlen_k)
     try:
         (kc, ks), (vc, vs) = k_cache, v_cache
         varlen = q.dim() == 3
@@ -275,7 +283,7 @@ def _attend(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale
                block_table.shape, block_table.stride(), block_table.dtype, block_table.device,
                varlen and (cu_q.shape, cu_q.stride(), cu_q.dtype, cu_q.device),
                alibi_slopes is not None and (alibi_slopes.shape, alibi_slopes.device),
-               softmax_scale, causal, tuple(window_size), softcap, max_seqlen_k)
+               softmax_scale, bool(causal), window_size, softcap, max_seqlen_k)
     except (AttributeError, TypeError, ValueError):
         raise _not_tensors(k_cache, v_cache) from None
     if q.requires_grad and torch.is_grad_enabled():
@@ -361,7 +369,7 @@ def _attend_plan(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_
         p.o_batch_stride, p.o_seq_stride, p.o_head_stride = q.shape[1] * Hq * D, Hq * D, D
         p.lse_batch_stride, p.lse_head_stride = Hq * q.shape[1], q.shape[1]
     cap = block_table.shape[1] * k_cache[0].shape[1]
-    p.max_seqlen_k = cap if max_seqlen_k is None else min(int(max_seqlen_k), cap)
+    p.max_seqlen_k = cap if max_seqlen_k is None else min(max_seqlen_k, cap)
     if p.max_seqlen_k == 0:  # (0 means no bound to the library)
         p.cache.max_pages = 0
     p.scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)

@@ -31,9 +31,12 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, i
     tables gives NaN in the rotated elements (never a read out of bounds).
     Arithmetic is fp32, rounded once.  Differentiable in q, k and the weights
     (weight gradients are summed in fp32 in a fixed order: the same bits every
-    time); cos and sin are constants.
+    time); cos and sin are constants.  Forward and backward can be captured into a
+    graph; as for every operator, no eager autograd graph of the same leaves may be
+    alive while a backward is captured.
     """
-    plan = _plan(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    # (numbers, so that the signature holds a value whatever type it came in)
+    plan = _plan(q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (
             q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad)):
         return _QkNormRopeFn.apply(plan, q, k, q_weight, k_weight, cos, sin, positions)

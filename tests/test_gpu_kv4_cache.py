@@ -353,3 +353,118 @@ def test_page_checks_on_request(monkeypatch):
                  lambda: mfa.kv4_append(k, k, *pools, ids(0, 3), ids(126), good)):
         with pytest.raises(ValueError):
             call()
+
+
+def _serving_state(seed, D, dtype):
+    """Tensors of one server's step: a prompt chunk and decoding sequences."""
+    g = torch.Generator().manual_seed(seed)
+    Hq, Hkv, page, lens, new = 8, 2, 64, [0, 130, 700, 63], [100, 1, 1, 1]
+    pages = sum(-(-(a + b) // page) for a, b in zip(lens, new)) + 2
+    kc, vc = mfa.kv4_cache(pages, page, Hkv, D), mfa.kv4_cache(pages, page, Hkv, D)
+    for c in (kc, vc):
+        c[0].copy_(torch.randint(0, 256, c[0].shape, generator=g, dtype=torch.uint8))
+        c[1].copy_(torch.randint(122, 126, c[1].shape, generator=g, dtype=torch.uint8))
+    ids, table = torch.randperm(pages, generator=g).tolist(), torch.full((4, 12), -1, dtype=torch.int32)
+    for b, n in enumerate(zip(lens, new)):
+        for i in range(-(-sum(n) // page)):
+            table[b, i] = ids.pop()
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    rows = lambda H: torch.randn(cu[-1], H, D, generator=g).to(DEV, dtype)  # noqa: E731
+    angle = torch.randn(900, D // 2, generator=g).to(DEV)
+    pos = torch.cat([torch.arange(a, a + b) for a, b in zip(lens, new)]).to(DEV, torch.int32)
+    return dict(q=rows(Hq), k=rows(Hkv), v=rows(Hkv), qw=torch.randn(D, generator=g).to(DEV, dtype), cos=angle.cos(), sin=angle.sin(),
+                pos=pos, kc=kc, vc=vc, cu=ints(cu), old=ints(lens), total=ints([a + b for a, b in zip(lens, new)]), table=table.to(DEV))
+
+
+def _serving_step(s):
+    q, k = mfa.qk_norm_rope(s["q"], s["k"], s["qw"], None, s["cos"], s["sin"], s["pos"])
+    mfa.kv4_append(k, s["v"], s["kc"], s["vc"], s["cu"], s["old"], s["table"])
+    out, lse = mfa.flash_attn_varlen_kv4_func(q, s["kc"], s["vc"], s["cu"], s["total"], s["table"], causal=True,
+                                              return_softmax_lse=True)
+    return q, k, *(x.clone() for c in (s["kc"], s["vc"]) for x in c), out, lse
+
+
+CASES = [(1, 128, torch.bfloat16), (2, 64, torch.float16), (3, 96, torch.bfloat16), (4, 32, torch.float16)]
+
+
+def test_steps_on_two_streams_at_once():
+    refs = [_serving_step(_serving_state(*c)) for c in CASES]
+    states = [_serving_state(*c) for c in CASES]
+    streams = [torch.cuda.Stream() for _ in CASES]
+    torch.cuda.synchronize()
+    outs = [[] for _ in CASES]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                outs[i].append(_serving_step(states[i]))
+    torch.cuda.synchronize()
+    for ref, runs in zip(refs, outs):
+        for got in runs:
+            assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+def test_steps_in_two_threads_at_once():
+    import threading
+
+    refs = [_serving_step(_serving_state(*c)) for c in CASES]
+    states = [_serving_state(*c) for c in CASES]
+    torch.cuda.synchronize()
+    outs, errors = [[] for _ in CASES], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    outs[i].append(_serving_step(states[i]))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # (shown by the main thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(CASES))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for ref, runs in zip(refs, outs):
+        assert len(runs) == 5
+        for got in runs:
+            assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+def test_two_captured_steps_replayed_in_turn():
+    """Two graphs, each with its own workspace, with eager steps between the replays."""
+    states = [_serving_state(*c) for c in CASES[:2]]
+    graphs, outs = [], []
+    for s in states:
+        _serving_step(s)
+    torch.cuda.synchronize()
+    for s in states:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_serving_step(s))
+        graphs.append(graph)
+    for turn in range(4):
+        for s in states:
+            for name in ("q", "k", "v"):
+                s[name].normal_()
+        graphs[turn % 2].replay()
+        graphs[1 - turn % 2].replay()
+        torch.cuda.synchronize()
+        got = [[t.clone() for t in o] for o in outs]
+        for s, g in zip(states, got):
+            ref = _serving_step(s)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(g, ref)), turn
+
+
+def test_the_same_pair_of_pages_twice_and_a_page_onto_itself():
+    pool = torch.randint(0, 256, (9, 5000), dtype=torch.uint8, device=DEV)
+    want = pool.clone()
+    want[4] = want[2]
+    ids = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    mfa.copy_cache_pages([pool, pool], ids(2, 2, 7, -1), ids(4, 4, 7, 4))
+    assert torch.equal(pool, want)

@@ -333,3 +333,49 @@ def test_c_norm_rope(lib):
     b.fwd.batch = 0
     assert lib.mfa_norm_rope(ctypes.byref(b.fwd), None) == 0
     refused(lib, lib.mfa_norm_rope(None, None), -1, "NULL")
+
+
+@pytest.mark.parametrize("field", ["q_weight", "k_weight"])
+def test_c_norm_rope_weight_alignment(lib, field):
+    p = _hip.MfaNormRopeParams()
+    p.q = p.k = p.q_out = p.k_out = p.cos = p.sin = 4096
+    p.q_seq_stride = p.k_seq_stride = p.q_head_stride = p.k_head_stride = 64
+    p.batch, p.seqlen, p.heads_q, p.heads_kv, p.head_dim, p.rotary_dim, p.table_rows = 1, 1, 1, 1, 64, 64, 9
+    p.dtype = p.dtype_weight = p.dtype_table = 1
+    setattr(p, field, 4097)
+    refused(lib, lib.mfa_norm_rope(ctypes.byref(p), None), -1, "weight")
+
+
+def test_c_copy_pages_of_more_workgroups_than_a_launch_has(lib):
+    p = _hip.MfaCopyPagesParams()
+    p.pool[0] = (4097, 1 << 20, 1 << 20)  # (single bytes: at most 16 KB per workgroup)
+    p.src = p.dst = 4096
+    p.pools, p.pairs, p.num_pages = 1, 1 << 20, 8
+    refused(lib, lib.mfa_copy_pages(ctypes.byref(p), None), -1, "too large")
+
+
+def test_expanded_cache_cannot_be_written(launches):
+    k = t(3, 2, 64)
+    cu, lens, table = i32(0, 3), i32(0), i32(0, 1)[None]
+    c = mfa.kv4_cache(2, 64, 2, 64, device="cpu")
+    for which in (0, 1):
+        e = tuple(x[:1].expand(2, -1, -1, -1) if i == which else x for i, x in enumerate(c))
+        for caches in ((e, c), (c, e)):
+            with pytest.raises(ValueError, match="expanded"):
+                mfa.kv4_append(k, k, *caches, cu, lens, table)
+    mfa.kv4_append(k, k, c, c, cu, lens, table)
+    assert len(launches) == 1
+
+
+def test_numbers_given_as_tensors_are_read_at_every_call(launches):
+    """A tensor stands for its value, also after it was changed in place."""
+    c = mfa.kv4_cache(2, 64, 2, 64, device="cpu")
+    scale, eps = torch.tensor(0.5), torch.tensor(1e-3)
+    q = t(1, 1, 2, 64)
+    for i, (s, e) in enumerate(((0.5, 1e-3), (0.25, 1e-2))):
+        scale.fill_(s)
+        eps.fill_(e)
+        mfa.flash_attn_kv4_func(q, c, c, i32(5), i32(0, 1)[None], softmax_scale=scale)
+        mfa.qk_norm_rope(q, q, None, None, torch.zeros(9, 32), torch.zeros(9, 32), eps=eps)
+        assert launches[2 * i][1][0].scale == s
+        assert launches[2 * i + 1][1][0].eps == pytest.approx(e)
