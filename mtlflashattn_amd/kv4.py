@@ -181,7 +181,7 @@ def kv4_append(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, r
     _cache_pointers(p.cache, kc, ks, vc, vs, block_table)
     values = None
     if return_values:
-        values = k.new_empty(k.shape), v.new_empty(v.shape)
+        values = tuple(torch.empty_like(t, memory_format=torch.contiguous_format) for t in (k, v))
         p.k_values, p.v_values = values[0].data_ptr(), values[1].data_ptr()
     _kernel._launch_on(k.device, _hip.kv4_append, p)
     return values
@@ -306,7 +306,7 @@ def _attend(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale
             cu_q = _i32(cu_q)
     if _kernel._check_pages_enabled():
         _check_pages(block_table, cache_seqlens.clamp(max=template.max_seqlen_k), kc.shape[1], kc.shape[0])
-    out, lse = q.new_empty(q.shape), None
+    out, lse = torch.empty_like(q, memory_format=torch.contiguous_format), None
     if return_lse:
         shape = (q.shape[1], q.shape[0]) if varlen else (q.shape[0], q.shape[2], q.shape[1])
         lse = torch.empty(shape, dtype=torch.float32, device=device)

@@ -45,13 +45,18 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, i
 
 class _Plan:
     """Of a call's signature: its parameters (everything but the data pointers),
-    whether the tensors are used in place, and the backward's workspace (bytes by
-    which weights have a gradient)."""
+    whether the tensors are used in place, the backward's parameters for contiguous
+    gradients, and its workspace (bytes by which weights have a gradient)."""
 
-    __slots__ = ("params", "direct", "ws")
+    __slots__ = ("params", "direct", "bwd", "ws")
 
     def __init__(self, params, direct):
         self.params, self.direct, self.ws = params, direct, {}
+        self.bwd = b = _hip.MfaNormRopeBwdParams()
+        b.fwd = params
+        L, D = params.seqlen, params.head_dim
+        b.dqo_batch_stride, b.dqo_seq_stride, b.dqo_head_stride = L * params.heads_q * D, params.heads_q * D, D
+        b.dko_batch_stride, b.dko_seq_stride, b.dko_head_stride = L * params.heads_kv * D, params.heads_kv * D, D
 
 
 _plans = {}
@@ -162,10 +167,14 @@ def _fill(p, plan, q, k, q_weight, k_weight, cos, sin, positions):
     return q, k, q_weight, k_weight, cos, sin, positions
 
 
+def _empty(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _forward(plan, q, k, q_weight, k_weight, cos, sin, positions):
     p = _hip.MfaNormRopeParams.from_buffer_copy(plan.params)
     held = _fill(p, plan, q, k, q_weight, k_weight, cos, sin, positions)  # noqa: F841 (kept until the launch)
-    q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
+    q_out, k_out = _empty(q), _empty(k)
     p.q_out, p.k_out = q_out.data_ptr(), k_out.data_ptr()
     _kernel._launch_on(q.device, _hip.norm_rope, p)
     return q_out, k_out
@@ -186,20 +195,19 @@ class _QkNormRopeFn(torch.autograd.Function):
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         plan, device = ctx.plan, q.device
-        b = _hip.MfaNormRopeBwdParams()
-        b.fwd = plan.params
+        b = _hip.MfaNormRopeBwdParams.from_buffer_copy(plan.bwd)
         held = _fill(b.fwd, plan, q, k, q_weight, k_weight, cos, sin, positions)  # noqa: F841 (kept until the launch)
-        if dq_out.dtype is not q.dtype or dq_out.stride(-1) != 1:
-            dq_out = _rows(dq_out.to(q.dtype))
-        if dk_out.dtype is not k.dtype or dk_out.stride(-1) != 1:
-            dk_out = _rows(dk_out.to(k.dtype))
+        dq_out, dk_out = _rows(dq_out.to(q.dtype)), _rows(dk_out.to(k.dtype))
+        if not dq_out.is_contiguous():
+            b.dqo_batch_stride, b.dqo_seq_stride, b.dqo_head_stride = _strides(dq_out)
+        if not dk_out.is_contiguous():
+            b.dko_batch_stride, b.dko_seq_stride, b.dko_head_stride = _strides(dk_out)
         b.dq_out, b.dk_out = dq_out.data_ptr(), dk_out.data_ptr()
-        b.dqo_batch_stride, b.dqo_seq_stride, b.dqo_head_stride = _strides(dq_out)
-        b.dko_batch_stride, b.dko_seq_stride, b.dko_head_stride = _strides(dk_out)
-        dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
+        dq, dk = _empty(q), _empty(k)
         b.dq, b.dk = dq.data_ptr(), dk.data_ptr()
-        dqw = q_weight.new_empty(q_weight.shape) if q_weight is not None and ctx.needs_input_grad[3] else None
-        dkw = k_weight.new_empty(k_weight.shape) if k_weight is not None and ctx.needs_input_grad[4] else None
+        needs = ctx.needs_input_grad
+        dqw = _empty(q_weight) if q_weight is not None and needs[3] else None
+        dkw = _empty(k_weight) if k_weight is not None and needs[4] else None
         if dqw is not None:
             b.dq_weight = dqw.data_ptr()
         if dkw is not None:
