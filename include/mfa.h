@@ -436,7 +436,10 @@ int mfa_kv4_append_params_size(void);
  * head_dim], sequence b owning tokens [cu_seqlens_q[b], cu_seqlens_q[b + 1])
  * (tokens of no sequence get 0, lse -inf).  The query rows are the last
  * positions of their sequence.  q and o: fp16 or bf16, 16-byte aligned, strides
- * multiples of 8 elements.  head_dim: 32, 64, 96 or 128.
+ * multiples of 8 elements.  head_dim: 32, 64, 96 or 128.  A NaN of V reaches only
+ * the rows whose mask holds its key.  With fp16 queries and more than 32 rows per
+ * K/V head in a sequence (positions times heads), elements of K and V beyond
+ * +/-65504 saturate.
  * Enqueues up to three kernels; never synchronizes, never allocates.  The results
  * do not depend on the workspace's address or content; they may differ in the
  * last bit with the batch a sequence stands in (its keys are dealt over
