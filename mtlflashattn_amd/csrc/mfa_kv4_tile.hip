@@ -2,14 +2,17 @@
 // chunk of a prompt): tiles of 128 columns, a column being one (query position,
 // query head) pair of a K/V head.
 //
-// Bound by the matrix cores and the softmax's vector work.  Each of the four
-// wavefronts owns 32 columns; 64 keys at a time, the workgroup turns the codes of
-// K and V into 16-bit rows in LDS once for all of them (a thread takes one
-// 32-element scale group of each: 16 conversions, exact in bf16 and saturating in
-// fp16), while the codes of the next 64 keys are on their way into registers (one
-// tile of each in LDS: two measured the same, 343 and 338 us for 1024 rows over
-// 16384 keys, Hq=32 Hkv=8 D=128 bf16, as the other workgroup of the CU computes
-// meanwhile).
+// Each of the four wavefronts owns 32 columns; 64 keys at a time, the workgroup
+// turns the codes of K and V into 16-bit rows in LDS once for all of them (a thread
+// takes one 32-element scale group of each: 16 conversions, exact in bf16 and
+// saturating in fp16).  There are two tiles: the next 64 keys are converted between
+// the products of the current ones, and the codes of the 64 after those are on
+// their way into registers.  1024 rows over 16384 keys, Hq=32 Hkv=8 D=128 bf16,
+// take 316 to 324 us (822 to 843 TFLOP/s; one tile, converted between two barriers: 329 to
+// 334), and with soft-cap over 8192 keys 206 (220).  Bound by no one unit: the
+// matrix pipe is busy 39 % of the time and LDS 48 %; taken out one at a time (of
+// 332 us), the products of the scores are worth 64 us, those of the values 37, the
+// softmax 43, the conversion 50 and most reads of K 17.
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16: a lane owns a column, its
 // probabilities go from the accumulators into the second product as they are, and
 // V is read transposed (ds_read_b64_tr_b16).  Exponent references are integers
@@ -42,10 +45,10 @@ mfa_kv4_tile_kernel(K4Args) {
     constexpr int GROUPS = 2 * kTK * GPR;       // scale groups of a block, K's then V's
     constexpr int NG = (GROUPS + kThreads4 - 1) / kThreads4;
     constexpr int R_ELEMS = 4 * 32 * KST;       // the wavefronts' result rows, in the tiles' place
-    __shared__ __attribute__((aligned(16))) uint16_t smem[R_ELEMS > K_ELEMS + V_ELEMS ? R_ELEMS : K_ELEMS + V_ELEMS];
-    uint16_t* const ktile = smem;
-    uint16_t* const vtile = smem + K_ELEMS;
-    __shared__ uint64_t nan_s[GPR];  // NaN groups of a block's V, a bit each
+    constexpr int T_ELEMS = K_ELEMS + V_ELEMS;
+    static_assert(R_ELEMS <= 2 * T_ELEMS, "the result rows fit the tiles' place");
+    __shared__ __attribute__((aligned(16))) uint16_t smem[2 * T_ELEMS];
+    __shared__ uint64_t nan_s[2][GPR + 1];  // NaN groups of a block's V, a bit each (and a place for what nobody reads)
 
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -80,7 +83,7 @@ mfa_kv4_tile_kernel(K4Args) {
         const float c = BIAS ? kLog2e : a.scale_log2;
         const float scale = a.scale, softcap = a.softcap, softcap_sk = a.softcap_sk;
         const bool alibi = BIAS && a.alibi != nullptr;
-        // key ranges: of the tile, and of this wavefront's columns
+        // key ranges: of the tile, and those that all columns of the tile or of this wavefront see
         const int i_first = (int)div4(wk.col0, a.by_r), i_last = (int)div4(wk.col0 + wk.ncol - 1, a.by_r);
         const int t_lo = lo4(a.wl, i_first + dq), t_hi = hi4(a.causal, a.wr, i_last + dq, Lk);
         const int key0 = (t_lo / kChunk4 + wk.c0) * kChunk4;
@@ -89,7 +92,6 @@ mfa_kv4_tile_kernel(K4Args) {
         const bool live = wlast >= wcol;
         const int wi0 = (int)div4(wcol, a.by_r), wi1 = (int)div4(max(wlast, wcol), a.by_r);
         const int a_lo = lo4(a.wl, i_last + dq), a_hi = hi4(a.causal, a.wr, i_first + dq, Lk);  // of every column of the tile
-        const int w_lo = lo4(a.wl, wi0 + dq), w_hi = hi4(a.causal, a.wr, wi1 + dq, Lk);    // of any column
         const int f_lo = lo4(a.wl, wi1 + dq), f_hi = hi4(a.causal, a.wr, wi0 + dq, Lk);    // of every column
         // (a lane behind the last column holds zero queries and stores nothing)
         int center;
@@ -122,23 +124,22 @@ mfa_kv4_tile_kernel(K4Args) {
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
                 const int x = gv[i] ? 2 : 0;
-                gc[i] = __builtin_amdgcn_raw_buffer_load_b128(gv[i] ? pg.rs[2] : pg.rs[0], goff[i] + (uint32_t)(row * pg.rstride[x]), 0, 0);
-                gs[i] = __builtin_amdgcn_raw_buffer_load_b8(gv[i] ? pg.rs[3] : pg.rs[1], gsoff[i] + (uint32_t)(row * pg.rstride[x + 1]), 0, 0);
+                gc[i] = __builtin_amdgcn_raw_buffer_load_b128(gv[i] ? pg.rs[2] : pg.rs[0], goff[i] + (uint32_t)row * (uint32_t)pg.rstride[x], 0, 0);
+                gs[i] = __builtin_amdgcn_raw_buffer_load_b8(gv[i] ? pg.rs[3] : pg.rs[1], gsoff[i] + (uint32_t)row * (uint32_t)pg.rstride[x + 1], 0, 0);
             }
         };
-        // part: some column of the tile does not see the whole block
-        auto swrite = [&](bool part) {
+        // the codes into tile `to`, the even or odd (half_) of this thread's groups; part:
+        // some column of the tile does not see the whole block (no branches: these run
+        // between the products of the other tile)
+        auto swrite = [&](bool part, int to, int half_) {
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
+                if (i % 2 != half_) continue;
                 if (GROUPS % kThreads4 == 0 || tid + kThreads4 * i < GROUPS) {
-                    uint16_t* p = smem + glds[i];
-                    float s = kv4_scale(gs[i]);
-                    if (part && gv[i]) {
-                        const bool nan = gs[i] == 255;
-                        const uint64_t nans = __ballot(nan);
-                        if (lane == 0) nan_s[(tid + kThreads4 * i - kTK * GPR) >> 6] = nans;
-                        s = nan ? 0.f : s;
-                    }
+                    uint16_t* p = smem + to * T_ELEMS + glds[i];
+                    const bool nan = part & gv[i] & (gs[i] == 255);
+                    nan_s[to][gv[i] && lane == 0 ? (tid + kThreads4 * i - kTK * GPR) >> 6 : GPR] = __ballot(nan);
+                    const float s = nan ? 0.f : kv4_scale(gs[i]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         *reinterpret_cast<u32x4_t*>(p + 8 * (e ^ gsw[i])) = IS_BF16 ? kv4_bf16x8(gc[i][e], s) : kv4_f16x8(gc[i][e], s);
@@ -160,7 +161,7 @@ mfa_kv4_tile_kernel(K4Args) {
                 return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, acc, 0, 0, 0);
         };
         const int tr_row = 4 * half + ((lane & 15) >> 2), tr_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-        auto load_vf = [&](int db, int kb, int st) -> op_t {
+        auto load_vf = [&](const uint16_t* vtile, int db, int kb, int st) -> op_t {
             // (rows 16 apart have the same swizzle)
             auto at = [&](int r) { return r * VST + (((4 * db + tr_chunk) ^ vswz4<DP>(r)) << 3) + 4 * (lane & 1); };
             const uint16_t* p0 = vtile + (32 * kb + 16 * st) * VST + at(tr_row);
@@ -180,18 +181,41 @@ mfa_kv4_tile_kernel(K4Args) {
             }
         };
 
-        auto block = [&](bool masked, int j) {
+        auto block = [&](bool masked, int j, int at, auto&& stage, auto&& fetch) {
+            const uint16_t *ktile = smem + at * T_ELEMS, *vtile = ktile + K_ELEMS;
+            // (the barriers to scheduling keep the LDS reads of 32 keys in flight ahead of
+            // the products that take them; left alone, each is read and waited for: 2 %)
             f32x16_t s[2];
-            __builtin_amdgcn_s_setprio(1);
+            op_t kf[DS], vf[DB][2];
+            auto load_k = [&](int kb) {
+#pragma unroll
+                for (int t = 0; t < DS; ++t)
+                    kf[t] = *reinterpret_cast<const op_t*>(ktile + (32 * kb + l32) * KST + 16 * t + 8 * half);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            load_k(0);
+            stage(0);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
 #pragma unroll
-                for (int t = 0; t < DS; ++t)
-                    s[kb] = mfma(*reinterpret_cast<const op_t*>(ktile + (32 * kb + l32) * KST + 16 * t + 8 * half), qf[t], s[kb]);
+                for (int t = 0; t < DS; ++t) s[kb] = mfma(kf[t], qf[t], s[kb]);
+                if (kb == 0) {
+                    load_k(1);
+                    stage(1);
+                }
             }
-            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch();
+            auto load_v = [&](int kb) {
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) vf[db][st] = load_vf(vtile, db, kb, st);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            load_v(0);
             // register r of s[kb] is key j + 32 kb + 4 half + acc_row(r)
             if constexpr (BIAS) {
                 // natural-log units: x = scale*s, soft-cap c tanh(x/c) =
@@ -277,18 +301,19 @@ mfa_kv4_tile_kernel(K4Args) {
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
                     for (int st = 0; st < 2; ++st)
-                        o[db] = mfma(load_vf(db, kb, st), __builtin_bit_cast(op_t, pw[st]), o[db]);
+                        o[db] = mfma(vf[db][st], __builtin_bit_cast(op_t, pw[st]), o[db]);
                 __builtin_amdgcn_s_setprio(0);
+                if (kb == 0) load_v(1);
             }
             l += acc[0] + acc[1];
         };
 
         // NaN groups for the columns that see their keys (a product with the zero weight
         // of a masked key would reach the others too)
-        auto nan_groups = [&](int j) {
+        auto nan_groups = [&](int j, int at) {
 #pragma unroll
             for (int i = 0; i < GPR; ++i) {
-                for (uint64_t x = nan_s[i]; x; x &= x - 1) {
+                for (uint64_t x = nan_s[at][i]; x; x &= x - 1) {
                     const int u = __builtin_amdgcn_readfirstlane(64 * i + __builtin_ctzll(x)), row = u / GPR;
                     K4Const& b = args4();
                     const int lo = lo4(b.wl, center), hi = hi4(b.causal, b.wr, center, Lk);
@@ -309,15 +334,21 @@ mfa_kv4_tile_kernel(K4Args) {
 #pragma unroll
         for (int s = 0; s < DS; ++s) pin(qf[s]);
         pin(slope);
-        for (int j = jbeg; j < jend; j += kTK) {
-            const bool part = j < a_lo || j + kTK - 1 > a_hi;
-            swrite(part);
-            if (j + kTK < jend) gload(j + kTK);
-            __syncthreads();
-            if (live && j <= w_hi && j + kTK - 1 >= w_lo) {
-                block(j < f_lo || j + kTK - 1 > f_hi, j);
-                if (part) nan_groups(j);
-            }
+        auto part = [&](int j) { return (j < a_lo) | (j + kTK - 1 > a_hi); };
+        if (jbeg < jend) {
+            swrite(part(jbeg), 0, 0);
+            swrite(part(jbeg), 0, 1);
+            gload(jbeg + kTK);
+        }
+        __syncthreads();
+        for (int j = jbeg, at = 0; j < jend; j += kTK, at ^= 1) {
+            // (behind the last block the tile that is written is not read)
+            auto stage = [&](int half_) { swrite(part(j + kTK), at ^ 1, half_); };
+            auto fetch = [&]() { gload(j + 2 * kTK); };  // (behind the last key: zeros or rows that are not used)
+            // (also where a wavefront's columns see nothing of it: a second path past the
+            // products would copy the accumulators)
+            block(j < f_lo || j + kTK - 1 > f_hi, j, at, stage, fetch);
+            if (part(j)) nan_groups(j, at);
             __syncthreads();
         }
 
