@@ -353,3 +353,35 @@ def test_nan_values_reach_only_the_rows_that_see_them(D, lq, Hq, window):
     out = call()
     assert torch.equal(out.isnan().cpu(), want)
     assert torch.equal(out.cpu()[~want], clean.cpu()[~want])
+
+
+@pytest.mark.parametrize("page", [64, 128, 192, 256, 320])
+@pytest.mark.parametrize("lq", [[1, 3, 1], [40, 1, 70]])
+def test_page_sizes(page, lq):
+    """Pages that end inside a chunk, hold several, or begin between two."""
+    run_and_check([777, 1000, 320], lq, page, 8, 2, 64, torch.bfloat16, causal=True)
+    run_and_check([777, 1000, 320], lq, page, 8, 2, 128, torch.float16, window_size=(200, 30))
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(16, 1), (17, 1), (32, 1), (40, 1), (128, 1), (130, 1)])
+def test_heads_that_fill_the_tiles(Hq, Hkv):
+    """Single rows whose heads alone are 16, 32, 128 columns and one or two more."""
+    run_and_check([257, 64, 1], [1, 1, 1], 64, Hq, Hkv, 64, torch.bfloat16, causal=True)
+
+
+def test_many_sequences_of_many_rows():
+    g = torch.Generator().manual_seed(5)
+    lq = torch.randint(0, 45, (100,), generator=g).tolist()
+    lens = [n + int(x) for n, x in zip(lq, torch.randint(0, 200, (100,), generator=g))]
+    run_and_check(lens, lq, 64, 4, 1, 32, torch.bfloat16, causal=True)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.5])
+@pytest.mark.parametrize("lq", [2, 50])
+def test_scales(scale, lq):
+    """A scale of 0 (uniform weights), a negative one, and one that makes weights of a single key."""
+    q, kc, vc, lens, table = make([300], 64, 4, 2, 64, torch.bfloat16, [lq])
+    kc[1].copy_(torch.full_like(kc[1], 122))
+    ref, _ = oracle(q, kc, vc, lens.cpu(), table, [lq], True, scale=scale)
+    out = mfa.flash_attn_kv4_func(q.view(1, lq, 4, 64), kc, vc, lens, table, softmax_scale=scale, causal=True)
+    check(out[0], ref, float(rows64(*vc).abs().max()), torch.bfloat16, on_tiles([lq], 2, False))
