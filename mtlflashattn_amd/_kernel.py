@@ -598,6 +598,13 @@ def _needs_grad(*tensors):
     return False
 
 
+def _check_no_tangent(*tensors):
+    """Forward-mode derivatives, which a launch would drop without a word."""
+    fw = torch.autograd.forward_ad
+    if fw._current_level >= 0 and any(t is not None and fw.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("mtlflashattn_amd: no forward-mode derivatives (use reverse mode)")
+
+
 def _run_bwd(q, k, v, out, dout, lse, *, scale, causal, softcap, window_left, window_right, alibi, alibi_bstride,
              cu_q=None, cu_k=None, seqlen_q=None, seqlen_k=None, grad_f32=False, dlse=None, into=None):
     """(dq, dk, dv) of the forward on [B, S, H, D] views (varlen: [1, T, H, D]).

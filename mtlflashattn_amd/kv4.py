@@ -162,6 +162,7 @@ def kv4_append(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, r
                block_table.shape, block_table.stride(), block_table.dtype, block_table.device)
     except (AttributeError, TypeError, ValueError):
         raise _not_tensors(k_cache, v_cache) from None
+    _kernel._check_no_tangent(k, v)
     if _kernel._needs_grad(k, v):
         raise NotImplementedError("mtlflashattn_amd: kv4_append is not differentiable; run it under torch.no_grad() or on "
                                   "detached rows")
@@ -286,6 +287,7 @@ def _attend(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale
                softmax_scale, bool(causal), window_size, softcap, max_seqlen_k)
     except (AttributeError, TypeError, ValueError):
         raise _not_tensors(k_cache, v_cache) from None
+    _kernel._check_no_tangent(q)
     if q.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("mtlflashattn_amd: attention over a 4-bit cache is forward-only; run it under "
                                   "torch.no_grad() or without inputs that require grad")

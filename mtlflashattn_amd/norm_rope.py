@@ -37,6 +37,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, i
     """
     # (numbers, so that the signature holds a value whatever type it came in)
     plan = _plan(q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved))
+    _kernel._check_no_tangent(q, k, q_weight, k_weight, cos, sin)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (
             q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad)):
         return _QkNormRopeFn.apply(plan, q, k, q_weight, k_weight, cos, sin, positions)

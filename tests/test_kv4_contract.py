@@ -379,3 +379,21 @@ def test_numbers_given_as_tensors_are_read_at_every_call(launches):
         mfa.qk_norm_rope(q, q, None, None, torch.zeros(9, 32), torch.zeros(9, 32), eps=eps)
         assert launches[2 * i][1][0].scale == s
         assert launches[2 * i + 1][1][0].eps == pytest.approx(e)
+
+
+def test_forward_mode_derivatives_are_refused(launches):
+    import torch.autograd.forward_ad as fw
+
+    c = mfa.kv4_cache(2, 64, 2, 64, device="cpu")
+    q, table = t(1, 3, 2, 64), i32(0, 1)[None]
+    tables = torch.zeros(9, 32), torch.zeros(9, 32)
+    with fw.dual_level():
+        d = fw.make_dual(q, torch.ones_like(q))
+        for call in (lambda: mfa.qk_norm_rope(d, q, None, None, *tables), lambda: mfa.qk_norm_rope(q, d, None, None, *tables),
+                     lambda: mfa.flash_attn_kv4_func(d, c, c, i32(5), table),
+                     lambda: mfa.kv4_append(d[0], q[0], c, c, i32(0, 3), i32(0), table)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert not launches
+        mfa.qk_norm_rope(q, q, None, None, *tables)
+    assert len(launches) == 1
