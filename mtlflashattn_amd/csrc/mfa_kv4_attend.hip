@@ -669,7 +669,7 @@ int k4_plan(const mfa_kv4_fwd_params* p, K4Plan* plan, int cus) {
     a.Lq = p->seqlen_q;
     a.rows_q = (int32_t)rows;
     // (a sequence holds at most what its table can name)
-    const int64_t cap = p->cache.num_pages ? (int64_t)p->cache.max_pages * p->cache.page_block_size : 0;
+    const int64_t cap = (int64_t)p->cache.max_pages * p->cache.page_block_size;
     a.max_k = (int32_t)std::min<int64_t>(p->max_seqlen_k ? p->max_seqlen_k : cap, std::min<int64_t>(cap, 0x7fffff00));
     a.page = p->cache.page_block_size;
     a.npages = p->cache.num_pages;

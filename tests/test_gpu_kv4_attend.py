@@ -385,3 +385,25 @@ def test_scales(scale, lq):
     ref, _ = oracle(q, kc, vc, lens.cpu(), table, [lq], True, scale=scale)
     out = mfa.flash_attn_kv4_func(q.view(1, lq, 4, 64), kc, vc, lens, table, softmax_scale=scale, causal=True)
     check(out[0], ref, float(rows64(*vc).abs().max()), torch.bfloat16, on_tiles([lq], 2, False))
+
+
+@pytest.mark.parametrize("lq", [1, 40])
+@pytest.mark.parametrize("pages,cols", [(0, 0), (0, 2), (3, 0)])
+def test_empty_pools_and_tables(lq, pages, cols):
+    """No page, or none named: no key where the table is empty, zero keys and values
+    where its ids name nothing; what is appended is dropped."""
+    q = torch.randn(2, lq, 4, 64, device=DEV, dtype=torch.bfloat16)
+    kc, vc = (mfa.kv4_cache(pages, 64, 2, 64) for _ in range(2))
+    lens = torch.tensor([70, 5], dtype=torch.int32, device=DEV)
+    table = torch.zeros(2, cols, dtype=torch.int32, device=DEV)
+    out, lse = mfa.flash_attn_kv4_func(q, kc, vc, lens, table, return_softmax_lse=True)
+    want = torch.full((2, 4, lq), -math.inf)
+    if cols:
+        want[:] = torch.tensor([70.0, 5.0]).log()[:, None, None]
+    assert not out.any() and torch.allclose(lse.cpu(), want, rtol=1e-5, atol=1e-5)
+    k = torch.randn(7, 2, 64, device=DEV, dtype=torch.bfloat16)
+    mfa.kv4_append(k, k, kc, vc, torch.tensor([0, 3, 7], dtype=torch.int32, device=DEV), torch.zeros_like(lens), table)
+    assert not any(x.any() for c in (kc, vc) for x in c)
+    cu = torch.tensor([0, 0, 0], dtype=torch.int32, device=DEV)
+    assert mfa.flash_attn_varlen_kv4_func(q[:0, 0], kc, vc, cu, lens, table).shape == (0, 4, 64)
+    assert not mfa.flash_attn_varlen_kv4_func(q[:, 0], kc, vc, cu, lens, table).any()
