@@ -291,3 +291,84 @@ def test_captured_forward_and_backward():
         ref = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, ref)), i
+
+
+@pytest.mark.parametrize("D,rot", [(64, 64), (64, 16), (36, 18)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_tables_without_rows(D, rot, interleaved):
+    """Every position is outside: the rotated elements are NaN, the others normalised."""
+    q, k, qw, kw, cos, sin, pos = inputs((5,), 2, 1, D, rot, torch.float32)
+    ref = mfa.qk_norm_rope(q, k, qw, kw, cos, sin, pos, interleaved=interleaved)
+    got = mfa.qk_norm_rope(q, k, qw, kw, cos[:0], sin[:0], pos, interleaved=interleaved)
+    for a, b in zip(got, ref):
+        assert a[..., :rot].isnan().all() and torch.equal(a[..., rot:], b[..., rot:])
+
+
+def test_heads_of_one_side_only_and_gradients_of_weights_only():
+    q, k, qw, kw, cos, sin, pos = inputs((3, 50), 4, 2, 64, 64, torch.bfloat16)
+    ref = mfa.qk_norm_rope(q, k, qw, kw, cos, sin, pos)
+    no_k = mfa.qk_norm_rope(q, k[:, :, :0], qw, kw, cos, sin, pos)
+    no_q = mfa.qk_norm_rope(q[:, :, :0], k, qw, kw, cos, sin, pos)
+    assert torch.equal(no_k[0], ref[0]) and torch.equal(no_q[1], ref[1])
+    assert no_k[1].shape == (3, 50, 0, 64) and no_q[0].shape == (3, 50, 0, 64)
+    leaves = [t.clone().requires_grad_() for t in (q, k, qw, kw)]
+    ups = [torch.randn_like(q), torch.randn_like(k)]
+    full = torch.autograd.grad(mfa.qk_norm_rope(*leaves, cos, sin, pos), leaves, ups)
+    some = torch.autograd.grad(mfa.qk_norm_rope(q, k, *leaves[2:], cos, sin, pos), leaves[2:], ups)
+    assert all(torch.equal(a, b) for a, b in zip(some, full[2:]))
+    some = torch.autograd.grad(mfa.qk_norm_rope(leaves[0], k, qw, kw, cos, sin, pos), leaves[:1], ups)
+    assert torch.equal(some[0], full[0])
+    one = mfa.qk_norm_rope(q, k[:, :, :0], leaves[2], leaves[3], cos, sin, pos)
+    gw = torch.autograd.grad(one, leaves[2:], (ups[0], ups[1][:, :, :0]))
+    assert torch.equal(gw[0], full[2]) and not gw[1].any()
+
+
+def test_inputs_expanded_over_the_batch():
+    """One sequence for three batches (batch stride 0): gradients are summed over them."""
+    q, k, qw, kw, cos, sin, pos = inputs((1, 40), 4, 2, 64, 64, torch.float32)
+    q0, k0 = q.clone().requires_grad_(), k.clone().requires_grad_()
+    q3, k3 = q0.expand(3, -1, -1, -1), k0.expand(3, -1, -1, -1)
+    p3 = torch.stack([pos[0], pos[0].flip(0), pos[0] // 2])
+    outs = mfa.qk_norm_rope(q3, k3, qw, kw, cos, sin, p3)
+    ups = [torch.randn_like(o) for o in outs]
+    got = torch.autograd.grad(outs, (q0, k0), ups)
+    qc, kc = (t.detach().repeat(3, 1, 1, 1).requires_grad_() for t in (q, k))
+    ref = torch.autograd.grad(mfa.qk_norm_rope(qc, kc, qw, kw, cos, sin, p3), (qc, kc), ups)
+    for a, b in zip(got, ref):
+        assert torch.equal(a, b.sum(0, keepdim=True))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_gradients_through_norm_rotation_and_attention(interleaved):
+    """A training step's way from a packed projection: views, norm and rotation,
+    causal grouped-query attention; gradients against float64 autograd on the CPU.
+
+    fp32: the attention's gradients are within 2e-6 of their largest value, the
+    norm's backward scales them and the reference by the same factors and adds 64 U,
+    and its difference h - n mean(h n) at most doubles what is relative to h: below
+    1e-5 of the largest value by a factor that leaves room for one row's.
+    """
+    B, L, Hq, Hkv, D = 2, 70, 4, 2, 64
+    g = torch.Generator().manual_seed(3)
+    packed = torch.randn(B, L, (Hq + 2 * Hkv) * D, generator=g).to(DEV).requires_grad_()
+    _, _, qw, kw, cos, sin, _ = inputs((1,), 1, 1, D, D, torch.float32, top=L)
+    qw, kw = qw.requires_grad_(), kw.requires_grad_()
+    up = torch.randn(B, L, Hq, D, generator=g)
+
+    def split(x):
+        return [t.unflatten(-1, (-1, D)) for t in x.split([Hq * D, Hkv * D, Hkv * D], -1)]
+
+    q, k, v = split(packed)
+    q, k = mfa.qk_norm_rope(q, k, qw, kw, cos, sin, interleaved=interleaved)
+    got = torch.autograd.grad(mfa.flash_attn_func(q, k, v, causal=True), (packed, qw, kw), up.to(DEV))
+
+    leaves = [t.detach().cpu().double().requires_grad_() for t in (packed, qw, kw)]
+    c, s, pos = cos.cpu().double(), sin.cpu().double(), torch.arange(L).expand(B, L)
+    q, k, v = split(leaves[0])
+    q, k = (formula(x, w, c, s, pos, 1e-6, interleaved) for x, w in ((q, leaves[1]), (k, leaves[2])))
+    k, v = (x.repeat_interleave(Hq // Hkv, 2) for x in (k, v))
+    w = torch.matmul(q.transpose(1, 2), k.permute(0, 2, 3, 1)) / D ** 0.5
+    w = torch.softmax(w.masked_fill(~torch.ones(L, L, dtype=torch.bool).tril(), float("-inf")), -1)
+    ref = torch.autograd.grad(torch.matmul(w, v.transpose(1, 2)).transpose(1, 2), leaves, up.double())
+    for a, b in zip(got, ref):
+        assert float((a.cpu().double() - b).abs().max()) <= 1e-5 * float(b.abs().max())
