@@ -491,7 +491,7 @@ mfa_kv4_kernel(K4Args) {
 }
 
 // The parts of a unit that several workgroups walked, added in the order of its
-// keys: block (w, z) takes kMergeCols columns of the unit whose walk workgroup w is
+// keys: block (w, z) takes merge_cols columns of the unit whose walk workgroup w is
 // the first to go on with.  Up to two launches' units in one (blocks of the first,
 // then of the second); a thread holds four elements of a column, and where there
 // are few of them (one or a few columns) groups of threads take every P-th part.
@@ -499,11 +499,16 @@ mfa_kv4_kernel(K4Args) {
 // loaded at once (no pass for the largest reference first), N parts at a time (4,
 // not 8, for columns that fill the block: 13.6 us instead of 16.5 after a launch of
 // 512 rows over 4096 keys beside 31 decoding sequences).
-constexpr int kMergeCols = 8;
-template <int DP, bool IS_BF16>
-__global__ void __launch_bounds__(kThreads4) mfa_kv4_merge_kernel(K4Args, K4Args) {
-    __shared__ f32x4_t o_s[kThreads4];
-    __shared__ float2 ml_s[kThreads4];
+// Blocks of T threads: 512 where all units have few columns, more threads per column
+// (5 rows of 6 sequences at head dim 64: 3.9 us, 5.9 with 256, 6.4 with 1024); 256
+// where some have many (13.6 us for the step above, 18.8 with 512).
+constexpr int kMergeFew = 512, kMergeMany = 256;
+constexpr int merge_cols(int threads) { return threads / (MFA_MAX_HEAD_DIM / 4); }
+template <int DP, bool IS_BF16, int T>
+__global__ void __launch_bounds__(T) mfa_kv4_merge_kernel(K4Args, K4Args) {
+    constexpr int kMergeCols = merge_cols(T);
+    __shared__ f32x4_t o_s[T];
+    __shared__ float2 ml_s[T];
     const int tid = threadIdx.x;
     const int first = args4(0).ws_merge ? args4(0).G * (args4(0).cols / kMergeCols) : 0;
     const int which = __builtin_amdgcn_readfirstlane((int)blockIdx.x >= first);
@@ -515,7 +520,7 @@ __global__ void __launch_bounds__(kThreads4) mfa_kv4_merge_kernel(K4Args, K4Args
     if (w1 < 0 || ncol <= 0) return;
     // the part of workgroup v: its first unit, unless it began before this one
     auto at = [&](int v) { return ((int64_t)v * 2 + (v == w0 ? g4.slot0 : 0)) * cols + cbeg; };
-    const int P = items <= 32 ? 8 : items <= 64 ? 4 : items <= 128 ? 2 : 1, S = kThreads4 / P;
+    const int P = items <= T / 8 ? 8 : items <= T / 4 ? 4 : items <= T / 2 ? 2 : 1, S = T / P;
     const int g = tid / S, it = tid - g * S;  // (a round holds every item)
     const bool in = it < items;
     const int r = in ? it / (DP / 4) : 0, d = in ? 4 * (it - r * (DP / 4)) : 0;
@@ -565,7 +570,7 @@ __global__ void __launch_bounds__(kThreads4) mfa_kv4_merge_kernel(K4Args, K4Args
         if (d == 0) store_lse4(a, g4.b, g4.q0, i, h, m, l);
     }
 }
-static_assert(kMergeCols * (MFA_MAX_HEAD_DIM / 4) <= kThreads4, "a thread per four elements");
+static_assert(16 % merge_cols(kMergeFew) == 0 && kTileCols4 % merge_cols(kMergeMany) == 0, "whole blocks per unit");
 
 typedef void (*k4_fn)(K4Args);
 typedef void (*k4_merge_fn)(K4Args, K4Args);
@@ -573,21 +578,21 @@ struct K4Kernels {
     k4_fn attend;
     k4_merge_fn merge;
 };
-// cols: columns of a unit, 16, 32 or kTileCols4
+// cols: columns of a unit, 16, 32 or kTileCols4; threads: of the merge's blocks
 template <int DP, bool IS_BF16>
-K4Kernels kernels4(int cols, bool bias) {
-    const k4_merge_fn merge = mfa_kv4_merge_kernel<DP, IS_BF16>;
+K4Kernels kernels4(int cols, bool bias, int threads) {
+    const k4_merge_fn merge = threads == kMergeFew ? mfa_kv4_merge_kernel<DP, IS_BF16, kMergeFew> : mfa_kv4_merge_kernel<DP, IS_BF16, kMergeMany>;
     if (cols == 16) return {mfa_kv4_kernel<DP, 1, IS_BF16>, merge};
     if (cols == 32) return {mfa_kv4_kernel<DP, 2, IS_BF16>, merge};
     return {(k4_fn)mfa_kv4_tile_kernel_of(DP, IS_BF16, bias), merge};
 }
 template <bool IS_BF16>
-K4Kernels kernels4(int dp, int cols, bool bias) {
+K4Kernels kernels4(int dp, int cols, bool bias, int threads) {
     switch (dp) {
-        case 32: return kernels4<32, IS_BF16>(cols, bias);
-        case 64: return kernels4<64, IS_BF16>(cols, bias);
-        case 96: return kernels4<96, IS_BF16>(cols, bias);
-        default: return kernels4<128, IS_BF16>(cols, bias);
+        case 32: return kernels4<32, IS_BF16>(cols, bias, threads);
+        case 64: return kernels4<64, IS_BF16>(cols, bias, threads);
+        case 96: return kernels4<96, IS_BF16>(cols, bias, threads);
+        default: return kernels4<128, IS_BF16>(cols, bias, threads);
     }
 }
 
@@ -743,20 +748,22 @@ int mfa_kv4_fwd(const mfa_kv4_fwd_params* p, void* workspace, int64_t workspace_
     char* ws = static_cast<char*>(workspace);
     K4Kernels k{};
     int merge = 0;
+    const int threads = plan.l[plan.n - 1].a.cols == kTileCols4 ? kMergeMany : kMergeFew;
     for (int i = 0; i < plan.n; ++i) {
         K4Launch& l = plan.l[i];
         const bool bias = l.a.bias != 0;
-        k = p->dtype == MFA_DTYPE_BF16 ? kernels4<true>(p->head_dim, l.a.cols, bias) : kernels4<false>(p->head_dim, l.a.cols, bias);
+        k = p->dtype == MFA_DTYPE_BF16 ? kernels4<true>(p->head_dim, l.a.cols, bias, threads)
+                                          : kernels4<false>(p->head_dim, l.a.cols, bias, threads);
         if (l.parts) {
             l.a.ws_o = reinterpret_cast<float*>(ws);
             l.a.ws_ml = l.a.ws_o + l.parts * p->head_dim;
             l.a.ws_merge = reinterpret_cast<Merge4*>(l.a.ws_ml + l.parts * 2);
             ws += part_bytes(l, p->head_dim);
-            merge += l.a.G * (l.a.cols / kMergeCols);
+            merge += l.a.G * (l.a.cols / merge_cols(threads));
         }
         hipLaunchKernelGGL(k.attend, dim3(l.a.G), dim3(kThreads4), 0, st, l.a);
     }
-    if (merge) hipLaunchKernelGGL(k.merge, dim3(merge), dim3(kThreads4), 0, st, plan.l[0].a, plan.l[plan.n - 1].a);
+    if (merge) hipLaunchKernelGGL(k.merge, dim3(merge), dim3(threads), 0, st, plan.l[0].a, plan.l[plan.n - 1].a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return k4err(MFA_ERR_LAUNCH, "mfa_kv4_fwd: launch failed: %s", hipGetErrorString(e));
     return MFA_OK;
