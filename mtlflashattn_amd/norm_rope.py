@@ -40,7 +40,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, i
     _kernel._check_no_tangent(q, k, q_weight, k_weight, cos, sin)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (
             q_weight is not None and q_weight.requires_grad) or (k_weight is not None and k_weight.requires_grad)):
-        return _QkNormRopeFn.apply(plan, q, k, q_weight, k_weight, cos, sin, positions)
+        return _QkNormRopeFn.apply(plan, float(eps), bool(interleaved), q, k, q_weight, k_weight, cos, sin, positions)
     return _forward(plan, q, k, q_weight, k_weight, cos, sin, positions)
 
 
@@ -183,19 +183,24 @@ def _forward(plan, q, k, q_weight, k_weight, cos, sin, positions):
 
 class _QkNormRopeFn(torch.autograd.Function):
     """qk_norm_rope with the HIP backward, which forms the statistics again from
-    q and k (nothing but the inputs is kept)."""
+    q and k (nothing but the inputs is kept).  The backward's plan is that of the
+    tensors it gets: saved-tensor hooks (save_on_cpu, activation offload) may give
+    back copies with other strides than the forward's views."""
 
     @staticmethod
-    def forward(ctx, plan, q, k, q_weight, k_weight, cos, sin, positions):
+    def forward(ctx, plan, eps, interleaved, q, k, q_weight, k_weight, cos, sin, positions):
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.plan = plan
+        ctx.options = eps, interleaved
         return _forward(plan, q, k, q_weight, k_weight, cos, sin, positions)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        plan, device = ctx.plan, q.device
+        if q.shape != dq_out.shape or k.shape != dk_out.shape or q.device != dq_out.device:
+            raise ValueError(f"mtlflashattn_amd: saved q {tuple(q.shape)} and k {tuple(k.shape)} on {q.device} came back for "
+                             f"gradients {tuple(dq_out.shape)} and {tuple(dk_out.shape)} on {dq_out.device}")
+        plan, device = _plan(q, k, q_weight, k_weight, cos, sin, positions, *ctx.options), q.device
         b = _hip.MfaNormRopeBwdParams.from_buffer_copy(plan.bwd)
         held = _fill(b.fwd, plan, q, k, q_weight, k_weight, cos, sin, positions)  # noqa: F841 (kept until the launch)
         dq_out, dk_out = _rows(dq_out.to(q.dtype)), _rows(dk_out.to(k.dtype))
@@ -207,8 +212,8 @@ class _QkNormRopeFn(torch.autograd.Function):
         dq, dk = _empty(q), _empty(k)
         b.dq, b.dk = dq.data_ptr(), dk.data_ptr()
         needs = ctx.needs_input_grad
-        dqw = _empty(q_weight) if q_weight is not None and needs[3] else None
-        dkw = _empty(k_weight) if k_weight is not None and needs[4] else None
+        dqw = _empty(q_weight) if q_weight is not None and needs[5] else None
+        dkw = _empty(k_weight) if k_weight is not None and needs[6] else None
         if dqw is not None:
             b.dq_weight = dqw.data_ptr()
         if dkw is not None:
@@ -221,4 +226,4 @@ class _QkNormRopeFn(torch.autograd.Function):
             plan.ws[which] = nbytes
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         _kernel._launch_on(device, _hip.norm_rope_bwd, b, None if ws is None else ws.data_ptr(), nbytes)
-        return None, dq, dk, dqw, dkw, None, None, None
+        return None, None, None, dq, dk, dqw, dkw, None, None, None

@@ -1,0 +1,39 @@
+"""Calls of the operators around the attention call that their first tests leave out."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import mtlflashattn_amd as mfa
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def i32(*x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("how", ["cpu", "dense"])
+def test_gradients_through_saved_tensor_hooks(how, dtype):
+    """Hooks that give back dense copies of views: the bits of the call without hooks
+    (the same values, sizes and alignment, so the same sums in the same order)."""
+    g = torch.Generator().manual_seed(1)
+    Hq, Hkv, D, L = 8, 2, 64, 300
+    qkv = torch.randn(L, Hq + 2 * Hkv, D, generator=g).to(DEV, dtype).requires_grad_()
+    w = [(1 + 0.2 * torch.randn(D, generator=g)).to(DEV, dtype).requires_grad_() for _ in range(2)]
+    table = torch.randn(4096, 3 * D, generator=g).to(DEV)
+    cos, sin = table[:, :D // 2], table[:, D // 2:D]
+    pos = torch.randint(0, 4096, (L, 2), generator=g).to(DEV)[:, 0]
+    ups = [torch.randn(L, h, D, generator=g).to(DEV, dtype) for h in (Hq, Hkv)]
+
+    def grads():
+        outs = mfa.qk_norm_rope(qkv[:, :Hq], qkv[:, Hq:Hq + Hkv], *w, cos, sin, pos)
+        return torch.autograd.grad(outs, (qkv, *w), ups)
+
+    want = grads()
+    with (torch.autograd.graph.save_on_cpu() if how == "cpu" else
+          torch.autograd.graph.saved_tensors_hooks(lambda x: x.contiguous().clone(), lambda x: x)):
+        got = grads()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

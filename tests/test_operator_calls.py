@@ -1,0 +1,81 @@
+"""Calls of the operators around the attention call that their first tests leave out,
+on the CPU: the device predicate patched and the launches recorded instead of made."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import mtlflashattn_amd as mfa
+from mtlflashattn_amd import _hip, _kernel
+
+
+def t(*shape, dtype=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def i32(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """(name, parameters) of every launch; CPU tensors count as ROCm tensors."""
+    calls = []
+    monkeypatch.setattr(_kernel, "_is_rocm_tensor", lambda x: True)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 0, raising=False)
+    for name in ("norm_rope", "norm_rope_bwd", "kv4_append", "kv4_fwd", "copy_pages"):
+        monkeypatch.setattr(_hip, name, lambda *a, name=name: calls.append((name, a[0])))
+    for name in ("kv4_fwd_workspace_bytes", "norm_rope_bwd_workspace_bytes"):
+        monkeypatch.setattr(_hip, name, lambda p: 0)
+    return calls
+
+
+class TestSavedTensorHooks:
+    """The backward of qk_norm_rope reads what the hooks give back, by its own strides."""
+
+    def call(self, unpack):
+        """Gradients of views of packed tensors, whose saved copies `unpack` gives back."""
+        qkv = t(5, 12, 64).requires_grad_()
+        w = t(2, 64)
+        table = t(9, 96, dtype=torch.float32)
+        pos = torch.zeros(5, 2, dtype=torch.int64)
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, unpack):
+            q, k = mfa.qk_norm_rope(qkv[:, :4], qkv[:, 4:8], w[0], w[1], table[:, :32], table[:, 32:64], pos[:, 0])
+        torch.autograd.grad((q, k), qkv, (torch.ones_like(q), torch.ones_like(k)))
+
+    def test_dense_copies(self, launches):
+        given = []
+
+        def dense(x):
+            given.append(x.contiguous().clone())
+            return given[-1]
+
+        self.call(dense)
+        (_, fwd), (_, bwd) = launches
+        assert (fwd.q_seq_stride, fwd.k_seq_stride, fwd.table_stride) == (12 * 64, 12 * 64, 96)
+        b = bwd.fwd
+        assert (b.q_seq_stride, b.q_head_stride, b.k_seq_stride, b.k_head_stride) == (4 * 64, 64, 4 * 64, 64)
+        assert b.table_stride == 32
+        assert [b.q, b.k, b.q_weight, b.k_weight, b.cos, b.sin, b.positions] == [x.data_ptr() for x in given]
+
+    def test_rows_that_are_not_contiguous(self, launches):
+        """A copy with other strides, which the kernel cannot address, is made dense first."""
+        self.call(lambda x: x.transpose(0, -1).clone(memory_format=torch.contiguous_format).transpose(0, -1)
+                  if x.dim() == 3 else x)
+        b = launches[1][1].fwd
+        assert (b.q_seq_stride, b.q_head_stride, b.k_seq_stride, b.k_head_stride) == (4 * 64, 64, 4 * 64, 64)
+        assert b.table_stride == 96
+
+    @pytest.mark.parametrize("unpack", [lambda x: x[:3], lambda x: x[..., :2, :] if x.dim() == 3 else x,
+                                        lambda x: x.double() if x.dim() == 3 else x])
+    def test_other_sizes_or_types_are_refused(self, launches, unpack):
+        with pytest.raises((ValueError, NotImplementedError), match="mtlflashattn_amd"):
+            self.call(unpack)
+        assert len(launches) == 1
+
+    def test_without_hooks(self, launches):
+        qkv = t(5, 12, 64).requires_grad_()
+        q, k = mfa.qk_norm_rope(qkv[:, :4], qkv[:, 4:8], None, None, t(9, 32), t(9, 32))
+        torch.autograd.grad((q, k), qkv, (torch.ones_like(q), torch.ones_like(k)))
+        b = launches[1][1].fwd
+        assert (b.q_seq_stride, b.k_seq_stride) == (12 * 64, 12 * 64)
