@@ -114,8 +114,9 @@ __device__ __forceinline__ void store4(char* p, const float* x) {
     }
 }
 
-// what is loaded in place of a position or a table row that is not there
-__device__ const uint32_t kZeros[64] = {0};
+// what is loaded in place of a position or a table row that is not there (at most
+// four floats from its start)
+__device__ alignas(16) const uint32_t kZeros[64] = {0};
 
 // Token and head of a row, and the table row of the token's position.
 struct Where {
@@ -472,7 +473,8 @@ int n_plan(const mfa_norm_rope_params* p, const mfa_norm_rope_bwd_params* b, NPl
         return nerr(MFA_ERR_INVALID, "%s: positions are not aligned or have a negative stride", who);
     a.cos = static_cast<const char*>(p->cos);
     a.sin = static_cast<const char*>(p->sin);
-    a.table_stride = p->table_stride;
+    // (a table without columns has one row: kZeros stands for it, whatever the position)
+    a.table_stride = p->rotary_dim > 0 ? p->table_stride : 0;
     a.pos = static_cast<const uint32_t*>(p->positions);
     a.pos_b = p->positions_batch_stride;
     a.pos64 = p->positions_64 != 0;

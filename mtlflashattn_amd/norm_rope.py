@@ -136,7 +136,7 @@ def _prepare(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
     p.k_batch_stride, p.k_seq_stride, p.k_head_stride = _strides(k)
     if cos.stride(0) != sin.stride(0):
         cos, sin = cos.contiguous(), sin.contiguous()
-    p.table_stride = cos.stride(0) if cos.shape[0] > 1 else 0
+    p.table_stride = cos.stride(0) if cos.shape[0] > 1 and cos.shape[1] > 0 else 0
     p.batch, p.seqlen = (q.shape[0], q.shape[1]) if q.dim() == 4 else (1, q.shape[0])
     p.heads_q, p.heads_kv, p.head_dim = q.shape[-2], k.shape[-2], q.shape[-1]
     p.rotary_dim, p.table_rows = 2 * cos.shape[1], cos.shape[0]

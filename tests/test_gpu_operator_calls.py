@@ -37,3 +37,32 @@ def test_gradients_through_saved_tensor_hooks(how, dtype):
           torch.autograd.graph.saved_tensors_hooks(lambda x: x.contiguous().clone(), lambda x: x)):
         got = grads()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D", [64, 36])
+@pytest.mark.parametrize("wide", [0, 64])
+def test_norm_without_rotation(wide, D, interleaved):
+    """Tables of no columns and many rows (empty, or a slice of wide ones): the norm
+    alone, forward and backward, at every position.  Bounds as in
+    test_gpu_norm_rope: an output 32, a gradient 64 steps of 2^-24 of the row's largest."""
+    g = torch.Generator().manual_seed(2)
+    rows = 65536
+    table = torch.randn(rows, wide, generator=g).to(DEV)[:, :0]
+    pos = torch.cat((torch.arange(rows - 40, rows), torch.randint(0, rows, (60,), generator=g))).to(DEV)
+    x = torch.randn(100, 3, D, generator=g).to(DEV).requires_grad_()
+    up = torch.randn(100, 3, D, generator=g).to(DEV)
+    out, _ = mfa.qk_norm_rope(x, x.detach(), None, None, table, table, pos, interleaved=interleaved)
+    dx, = torch.autograd.grad(out, x, up)
+    y = x.detach().double().cpu().requires_grad_()
+    ref = y / torch.sqrt(y.square().mean(-1, keepdim=True) + 1e-6)
+    dref, = torch.autograd.grad(ref, y, up.double().cpu())
+    for got, want, steps in ((out.detach(), ref.detach(), 32), (dx, dref, 64)):
+        err = (got.double().cpu() - want).abs()
+        scale = want.abs().amax(-1, keepdim=True)
+        if steps == 64:  # rs max|h|
+            rs = 1 / torch.sqrt(y.detach().square().mean(-1, keepdim=True) + 1e-6)
+            scale = scale + rs * up.double().cpu().abs().amax(-1, keepdim=True)
+        assert bool((err <= steps * 2.0 ** -24 * scale).all())
+    fwd, _ = mfa.qk_norm_rope(x.detach(), x.detach(), None, None, table, table, interleaved=interleaved)
+    assert torch.equal(fwd, out.detach())

@@ -79,3 +79,10 @@ class TestSavedTensorHooks:
         torch.autograd.grad((q, k), qkv, (torch.ones_like(q), torch.ones_like(k)))
         b = launches[1][1].fwd
         assert (b.q_seq_stride, b.k_seq_stride) == (12 * 64, 12 * 64)
+
+
+@pytest.mark.parametrize("table", [t(9000, 0), t(9000, 64)[:, :0]])
+def test_tables_without_columns_have_one_row(launches, table):
+    mfa.qk_norm_rope(t(5, 4, 64), t(5, 2, 64), None, None, table, table)
+    p = launches[0][1]
+    assert (p.rotary_dim, p.table_rows, p.table_stride) == (0, 9000, 0)
