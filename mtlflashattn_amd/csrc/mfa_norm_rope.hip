@@ -116,7 +116,7 @@ __device__ __forceinline__ void store4(char* p, const float* x) {
 
 // what is loaded in place of a position or a table row that is not there (at most
 // four floats from its start)
-__device__ alignas(16) const uint32_t kZeros[64] = {0};
+alignas(16) __device__ const uint32_t kZeros[64] = {0};
 
 // Token and head of a row, and the table row of the token's position.
 struct Where {
