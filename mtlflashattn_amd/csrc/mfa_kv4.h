@@ -13,9 +13,9 @@
 #include "mfa.h"
 #include "mfa_common.h"
 
-// Checks of a cache's pointers, strides and sizes: MFA_OK, or an error code with
-// the message set (mfa_kv4.hip).
-__attribute__((visibility("hidden"))) int mfa_kv4_check_cache(const mfa_kv4_cache* cache, int head_dim,
+// Checks of the pointers, strides and sizes of the cache of `batch` sequences:
+// MFA_OK, or an error code with the message set (mfa_kv4.hip).
+__attribute__((visibility("hidden"))) int mfa_kv4_check_cache(const mfa_kv4_cache* cache, int batch, int head_dim,
                                                               const char* who);
 
 namespace {

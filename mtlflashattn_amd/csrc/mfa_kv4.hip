@@ -141,14 +141,15 @@ int aerr(int code, const char* fmt, ...) {
 
 }  // namespace
 
-int mfa_kv4_check_cache(const mfa_kv4_cache* c, int head_dim, const char* who) {
+int mfa_kv4_check_cache(const mfa_kv4_cache* c, int batch, int head_dim, const char* who) {
     if (c->page_block_size <= 0 || c->page_block_size % 64)
         return aerr(MFA_ERR_INVALID, "%s: page_block_size %d must be a positive multiple of 64", who, c->page_block_size);
     if (c->num_pages < 0 || c->max_pages < 0 || c->block_table_batch_stride < 0)
         return aerr(MFA_ERR_INVALID, "%s: negative num_pages, max_pages or block_table stride", who);
     if ((int64_t)c->max_pages * c->page_block_size > 0x7fffffffLL)
         return aerr(MFA_ERR_INVALID, "%s: a block table names at most 2^31 - 1 rows", who);
-    if (c->max_pages > 0 && (!c->block_table || (reinterpret_cast<uintptr_t>(c->block_table) & 3)))
+    // (no sequences: a table of no rows, which may have no memory)
+    if (batch > 0 && c->max_pages > 0 && (!c->block_table || (reinterpret_cast<uintptr_t>(c->block_table) & 3)))
         return aerr(MFA_ERR_INVALID, "%s: block_table is required", who);
     const mfa_kv4_pool* pools[2] = {&c->k, &c->v};
     for (const mfa_kv4_pool* p : pools) {
@@ -180,7 +181,7 @@ int mfa_kv4_append(const mfa_kv4_append_params* p, void* stream) {
     if (p->head_dim <= 0 || p->head_dim % kKv4Group || p->head_dim > MFA_MAX_HEAD_DIM)
         return aerr(MFA_ERR_UNSUPPORTED, "mfa_kv4_append: head_dim %d is not a multiple of %d up to %d", p->head_dim, kKv4Group,
                     MFA_MAX_HEAD_DIM);
-    const int rc = mfa_kv4_check_cache(&p->cache, p->head_dim, "mfa_kv4_append");
+    const int rc = mfa_kv4_check_cache(&p->cache, p->batch, p->head_dim, "mfa_kv4_append");
     if (rc != MFA_OK) return rc;
     if (p->batch == 0 || p->total == 0 || p->heads_kv == 0) return MFA_OK;
     auto bad = [](const void* x, uintptr_t al) { return !x || (reinterpret_cast<uintptr_t>(x) & (al - 1)); };

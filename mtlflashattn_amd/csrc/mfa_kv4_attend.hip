@@ -639,7 +639,7 @@ int k4_plan(const mfa_kv4_fwd_params* p, K4Plan* plan, int cus) {
     if (!(p->softcap >= 0.f)) return k4err(MFA_ERR_INVALID, "mfa_kv4_fwd: softcap must be >= 0");
     if (p->window_left < -1 || p->window_right < -1)
         return k4err(MFA_ERR_INVALID, "mfa_kv4_fwd: window bounds must be >= -1");
-    const int rc = mfa_kv4_check_cache(&p->cache, D, "mfa_kv4_fwd");
+    const int rc = mfa_kv4_check_cache(&p->cache, p->batch, D, "mfa_kv4_fwd");
     if (rc != MFA_OK) return rc;
     const bool varlen = p->cu_seqlens_q != nullptr;
     const int64_t rows = varlen ? p->total_q : (int64_t)p->batch * p->seqlen_q;

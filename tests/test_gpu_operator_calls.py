@@ -66,3 +66,19 @@ def test_norm_without_rotation(wide, D, interleaved):
         assert bool((err <= steps * 2.0 ** -24 * scale).all())
     fwd, _ = mfa.qk_norm_rope(x.detach(), x.detach(), None, None, table, table, interleaved=interleaved)
     assert torch.equal(fwd, out.detach())
+
+
+def test_calls_of_no_sequences():
+    """A step without sequences: nothing to write, rows of no sequence are 0 and -inf."""
+    kc, vc = (mfa.kv4_cache(3, 64, 2, 64) for _ in range(2))
+    cu, none = i32(0), torch.zeros(0, dtype=torch.int32, device=DEV)
+    for table in (torch.zeros(0, 4, dtype=torch.int32, device=DEV), torch.zeros(0, 0, dtype=torch.int32, device=DEV)):
+        q = torch.randn(0, 2, 4, 64, device=DEV, dtype=torch.bfloat16)
+        out, lse = mfa.flash_attn_kv4_func(q, kc, vc, none, table, return_softmax_lse=True)
+        assert out.shape == q.shape and lse.shape == (0, 4, 2)
+        q = torch.randn(5, 4, 64, device=DEV, dtype=torch.bfloat16)
+        out, lse = mfa.flash_attn_varlen_kv4_func(q, kc, vc, cu, none, table, return_softmax_lse=True)
+        assert not out.any() and bool((lse == float("-inf")).all()) and lse.shape == (4, 5)
+        assert mfa.kv4_append(q[:0, :2], q[:0, :2], kc, vc, cu, none, table) is None
+        assert mfa.kv4_append(q[:, :2], q[:, :2], kc, vc, cu, none, table) is None
+        assert not any(t.any() for t in (*kc, *vc))

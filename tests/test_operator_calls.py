@@ -2,11 +2,14 @@
 on the CPU: the device predicate patched and the launches recorded instead of made."""
 from __future__ import annotations
 
+import ctypes
+import os
+
 import pytest
 import torch
 
 import mtlflashattn_amd as mfa
-from mtlflashattn_amd import _hip, _kernel
+from mtlflashattn_amd import _build, _hip, _kernel
 
 
 def t(*shape, dtype=torch.bfloat16):
@@ -86,3 +89,34 @@ def test_tables_without_columns_have_one_row(launches, table):
     mfa.qk_norm_rope(t(5, 4, 64), t(5, 2, 64), None, None, table, table)
     p = launches[0][1]
     assert (p.rotary_dim, p.table_rows, p.table_stride) == (0, 9000, 0)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not os.path.exists(_build.LIB_PATH):
+        _build.build()
+    return _hip.load()
+
+
+def test_no_sequences_need_no_table(lib):
+    """A table of no rows has no memory: torch gives a null pointer for it."""
+    f = _hip.MfaKv4FwdParams()
+    c = f.cache
+    for pool in (c.k, c.v):
+        pool.codes = pool.scales = 4096
+        pool.code_page_stride, pool.code_row_stride, pool.code_head_stride = 64 * 32, 32, 64 * 32
+        pool.scale_page_stride, pool.scale_row_stride, pool.scale_head_stride = 64 * 2, 2, 64 * 2
+    c.max_pages, c.page_block_size, c.num_pages = 4, 64, 8
+    f.q = f.o = 4096
+    f.q_seq_stride = f.o_seq_stride = f.q_head_stride = f.o_head_stride = 64
+    f.seqlen_q, f.heads_q, f.heads_kv, f.head_dim, f.scale, f.dtype = 1, 1, 1, 64, 0.125, _hip.MFA_DTYPE_BF16
+    f.window_left = f.window_right = -1
+    a = _hip.MfaKv4AppendParams()
+    a.cache, a.k, a.v, a.cu_seqlens = c, 4096, 4096, 4096
+    a.heads_kv, a.head_dim, a.dtype = 1, 64, _hip.MFA_DTYPE_BF16
+    assert lib.mfa_kv4_fwd(ctypes.byref(f), None, 0, None) == 0
+    assert lib.mfa_kv4_append(ctypes.byref(a), None) == 0
+    f.batch = f.total_q = a.batch = a.total = 1
+    f.cache_seqlens = a.cache_seqlens = 4096
+    assert lib.mfa_kv4_fwd(ctypes.byref(f), None, 0, None) == -1 and b"block_table" in lib.mfa_last_error()
+    assert lib.mfa_kv4_append(ctypes.byref(a), None) == -1 and b"block_table" in lib.mfa_last_error()
