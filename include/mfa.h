@@ -408,7 +408,8 @@ typedef struct mfa_kv4_cache {
  * more than half a step; elements are rounded to the nearest value, ties to the
  * even code, and a group that holds an infinity or NaN becomes NaN.
  * k_values / v_values (optional, both or none): what the cache now holds for
- * every token, contiguous [total, heads_kv, head_dim] of `dtype`.
+ * every token (what it would, for one that is dropped), contiguous [total,
+ * heads_kv, head_dim] of `dtype`.
  * head_dim: a multiple of 32 up to MFA_MAX_HEAD_DIM.  One kernel; never
  * synchronizes, never allocates.
  */

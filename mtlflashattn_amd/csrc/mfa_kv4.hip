@@ -183,7 +183,8 @@ int mfa_kv4_append(const mfa_kv4_append_params* p, void* stream) {
                     MFA_MAX_HEAD_DIM);
     const int rc = mfa_kv4_check_cache(&p->cache, p->batch, p->head_dim, "mfa_kv4_append");
     if (rc != MFA_OK) return rc;
-    if (p->batch == 0 || p->total == 0 || p->heads_kv == 0) return MFA_OK;
+    // (tokens of no sequence have values too)
+    if (p->total == 0 || p->heads_kv == 0 || (p->batch == 0 && !p->k_values && !p->v_values)) return MFA_OK;
     auto bad = [](const void* x, uintptr_t al) { return !x || (reinterpret_cast<uintptr_t>(x) & (al - 1)); };
     if (bad(p->k, 16) || bad(p->v, 16)) return aerr(MFA_ERR_INVALID, "mfa_kv4_append: k and v must be 16-byte aligned");
     const int al = p->dtype == MFA_DTYPE_F32 ? 4 : 8;
@@ -191,7 +192,7 @@ int mfa_kv4_append(const mfa_kv4_append_params* p, void* stream) {
         return aerr(MFA_ERR_INVALID, "mfa_kv4_append: k and v strides must be multiples of %d elements", al);
     if ((p->k_values == nullptr) != (p->v_values == nullptr) || (p->k_values && (bad(p->k_values, 16) || bad(p->v_values, 16))))
         return aerr(MFA_ERR_INVALID, "mfa_kv4_append: k_values and v_values must both be NULL or 16-byte aligned");
-    if (bad(p->cu_seqlens, 4) || bad(p->cache_seqlens, 4))
+    if (bad(p->cu_seqlens, 4) || (p->batch > 0 && bad(p->cache_seqlens, 4)))
         return aerr(MFA_ERR_INVALID, "mfa_kv4_append: cu_seqlens and cache_seqlens are required");
     const int64_t per_token = (int64_t)p->heads_kv * (p->head_dim / 8);
     if (per_token > 0x7fffffffLL || per_token * p->total > 0x7fffffffLL)

@@ -148,7 +148,7 @@ def kv4_append(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, r
     code.  A group with an infinity or a NaN is held as NaN.
 
     return_values=True returns (k', v') [total, Hkv, D] in k.dtype: the rows as the
-    cache now holds them, for attention over a prompt that later steps will read
+    cache now holds them (or would, where a row is dropped), for attention over a prompt that later steps will read
     back from the cache (flash_attn_varlen_func(q, k', v', ...)).  Not
     differentiable: inputs that require grad raise.
     """

@@ -82,3 +82,18 @@ def test_calls_of_no_sequences():
         assert mfa.kv4_append(q[:0, :2], q[:0, :2], kc, vc, cu, none, table) is None
         assert mfa.kv4_append(q[:, :2], q[:, :2], kc, vc, cu, none, table) is None
         assert not any(t.any() for t in (*kc, *vc))
+
+
+def test_values_of_tokens_of_no_sequence():
+    """What the cache would hold for them, also where there is no sequence at all."""
+    k, v = (torch.randn(300, 2, 64, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    pools = [mfa.kv4_cache(8, 64, 2, 64) for _ in range(2)]
+    table, none = i32(*range(8))[None], torch.zeros(0, dtype=torch.int32, device=DEV)
+    want = mfa.kv4_append(k, v, *pools, i32(0, 300), i32(0), table, return_values=True)
+    held = [t.clone() for c in pools for t in c]
+    marks = [torch.full_like(k, 7.0) for _ in range(4)]  # (memory that the results may come to lie in)
+    del marks
+    some = mfa.kv4_append(k, v, *pools, i32(0, 0), i32(0), table, return_values=True)
+    got = mfa.kv4_append(k, v, *pools, i32(0), none, table[:0], return_values=True)
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, some, got))
+    assert all(torch.equal(a, b) for a, b in zip(held, (t for c in pools for t in c)))
