@@ -643,10 +643,10 @@ int k4_plan(const mfa_kv4_fwd_params* p, K4Plan* plan, int cus) {
     if (rc != MFA_OK) return rc;
     const bool varlen = p->cu_seqlens_q != nullptr;
     const int64_t rows = varlen ? p->total_q : (int64_t)p->batch * p->seqlen_q;
-    if (p->batch == 0 || rows == 0) return MFA_OK;
+    if (rows == 0) return MFA_OK;
     auto bad = [](const void* x, uintptr_t al) { return !x || (reinterpret_cast<uintptr_t>(x) & (al - 1)); };
     if (bad(p->q, 16) || bad(p->o, 16)) return k4err(MFA_ERR_INVALID, "mfa_kv4_fwd: q and o must be 16-byte aligned");
-    if (bad(p->cache_seqlens, 4)) return k4err(MFA_ERR_INVALID, "mfa_kv4_fwd: cache_seqlens is required");
+    if (p->batch > 0 && bad(p->cache_seqlens, 4)) return k4err(MFA_ERR_INVALID, "mfa_kv4_fwd: cache_seqlens is required");
     const int64_t st[] = {p->q_batch_stride, p->q_seq_stride, p->q_head_stride, p->o_batch_stride, p->o_seq_stride, p->o_head_stride};
     for (int64_t s : st)
         if (s % 8) return k4err(MFA_ERR_INVALID, "mfa_kv4_fwd: q and o strides must be multiples of 8 elements");
@@ -695,7 +695,8 @@ int k4_plan(const mfa_kv4_fwd_params* p, K4Plan* plan, int cus) {
     // Columns per workgroup: a sequence's, at most 128.  The sequences of a
     // varlen call are known on the device only: one launch takes those of at most
     // 16 columns, another the longer ones.
-    const int64_t cols = (varlen ? rows : p->seqlen_q) * (int64_t)a.R;
+    // (no sequences: the launch only clears the rows)
+    const int64_t cols = p->batch == 0 ? 1 : (varlen ? rows : p->seqlen_q) * (int64_t)a.R;
     plan->n = varlen && cols > 16 ? 2 : 1;
     const int64_t chunks = std::max<int64_t>(1, ((int64_t)a.max_k + kChunk4 - 1) / kChunk4);
     for (int i = 0; i < plan->n; ++i) {

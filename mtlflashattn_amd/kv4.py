@@ -315,10 +315,6 @@ def _attend(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale
         p.softmax_lse = lse.data_ptr()
     if varlen:
         p.cu_seqlens_q = cu_q.data_ptr()
-        if p.batch == 0:  # (nothing is launched)
-            out.zero_()
-            if return_lse:
-                lse.fill_(float("-inf"))
     if alibi_slopes is not None:
         slopes, p.alibi_batch_stride = _kernel._alibi_arg(alibi_slopes, p.batch, p.heads_q, device)
         p.alibi_slopes = slopes.data_ptr()

@@ -97,3 +97,30 @@ def test_values_of_tokens_of_no_sequence():
     got = mfa.kv4_append(k, v, *pools, i32(0), none, table[:0], return_values=True)
     assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, some, got))
     assert all(torch.equal(a, b) for a, b in zip(held, (t for c in pools for t in c)))
+
+
+def test_c_rows_of_no_sequences_are_cleared():
+    """mfa_kv4_fwd with rows but no sequences, through the C parameters."""
+    from mtlflashattn_amd import _hip
+
+    out = torch.full((40, 8, 64), 7.0, device=DEV, dtype=torch.bfloat16)
+    lse = torch.full((8, 40), 7.0, device=DEV)
+    cu, codes, scales = i32(0), torch.zeros(2, 2, 64, 32, dtype=torch.uint8, device=DEV), torch.zeros(2, 2, 64, 2, dtype=torch.uint8, device=DEV)
+    p = _hip.MfaKv4FwdParams()
+    for pool in (p.cache.k, p.cache.v):
+        pool.codes, pool.scales = codes.data_ptr(), scales.data_ptr()
+        pool.code_page_stride, pool.code_row_stride, pool.code_head_stride = codes.stride(0), codes.stride(2), codes.stride(1)
+        pool.scale_page_stride, pool.scale_row_stride, pool.scale_head_stride = scales.stride(0), scales.stride(2), scales.stride(1)
+    p.cache.max_pages, p.cache.page_block_size, p.cache.num_pages = 4, 64, 2
+    p.q = p.o = out.data_ptr()
+    p.q_seq_stride = p.o_seq_stride = 8 * 64
+    p.q_head_stride = p.o_head_stride = 64
+    p.softmax_lse, p.lse_head_stride, p.cu_seqlens_q = lse.data_ptr(), 40, cu.data_ptr()
+    p.total_q, p.heads_q, p.heads_kv, p.head_dim, p.scale = 40, 8, 2, 64, 0.125
+    p.window_left = p.window_right = -1
+    p.dtype = _hip.MFA_DTYPE_BF16
+    n = _hip.kv4_fwd_workspace_bytes(p)
+    ws = torch.empty(max(n, 1), dtype=torch.uint8, device=DEV)
+    _hip.kv4_fwd(p, ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert not out.any() and bool((lse == float("-inf")).all())
