@@ -113,6 +113,10 @@ def _cache_pointers(c, kc, ks, vc, vs, block_table):
     c.block_table = block_table.data_ptr()
 
 
+# (tensors written in place: a graph that saved one raises the usual error in its backward)
+_written = torch.autograd.graph.increment_version
+
+
 def _i32(t):
     return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
@@ -185,6 +189,7 @@ def kv4_append(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, r
         values = tuple(torch.empty_like(t, memory_format=torch.contiguous_format) for t in (k, v))
         p.k_values, p.v_values = values[0].data_ptr(), values[1].data_ptr()
     _kernel._launch_on(k.device, _hip.kv4_append, p)
+    _written((kc, ks, vc, vs))
     return values
 
 
@@ -398,7 +403,7 @@ def copy_cache_pages(pools, src, dst):
     copied before one of them writes to it) and compaction (pages move into free ones)
     need.  The destinations have to differ from each other and from every source; pairs
     are copied in no order.  MTLFLASHATTN_CHECK_PAGES=1 checks that on the host and raises
-    ValueError.
+    ValueError.  The pools count as modified in place.
     """
     pools = list(pools)
     if not pools:
@@ -430,6 +435,7 @@ def copy_cache_pages(pools, src, dst):
         first += p.pools
         p.src, p.dst = src.data_ptr(), dst.data_ptr()
         _kernel._launch_on(device, _hip.copy_pages, p)
+    _written(pools)
 
 
 def _copy_plan(pools, src, dst):

@@ -120,3 +120,43 @@ def test_no_sequences_need_no_table(lib):
     f.cache_seqlens = a.cache_seqlens = 4096
     assert lib.mfa_kv4_fwd(ctypes.byref(f), None, 0, None) == -1 and b"block_table" in lib.mfa_last_error()
     assert lib.mfa_kv4_append(ctypes.byref(a), None) == -1 and b"block_table" in lib.mfa_last_error()
+
+
+class TestVersionCounters:
+    """A graph that saved a pool notices that the pool was written."""
+
+    def saved(self, pool):
+        x = torch.ones(pool.shape, requires_grad=True)
+        return (x * pool).sum()  # saves the pool
+
+    def test_copied_pages(self, launches):
+        pools = [torch.zeros(4, 8), torch.zeros(4, 3, 8)[:, 1]]
+        losses = [self.saved(p) for p in pools]
+        mfa.copy_cache_pages(pools, i32(0), i32(1))
+        for loss in losses:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                loss.backward()
+
+    def test_appended_rows(self, launches):
+        kc, vc = (mfa.kv4_cache(2, 64, 2, 64, device="cpu") for _ in range(2))
+        losses = [self.saved(p) for p in (*kc, *vc)]
+        mfa.kv4_append(t(3, 2, 64), t(3, 2, 64), kc, vc, i32(0, 3), i32(0), i32(0, 1)[None])
+        for loss in losses:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                loss.backward()
+
+    def test_inference_tensors(self, launches):
+        with torch.inference_mode():
+            pool = torch.zeros(4, 8)
+            kc, vc = (mfa.kv4_cache(2, 64, 2, 64, device="cpu") for _ in range(2))
+        for mode in (True, False):
+            with torch.inference_mode(mode):
+                mfa.copy_cache_pages([pool], i32(0), i32(1))
+                mfa.kv4_append(t(3, 2, 64), t(3, 2, 64), kc, vc, i32(0, 3), i32(0), i32(0, 1)[None])
+        assert len(launches) == 4
+
+    def test_read_only_calls(self, launches):
+        c = mfa.kv4_cache(2, 64, 2, 64, device="cpu")
+        before = [x._version for x in c]
+        mfa.flash_attn_kv4_func(t(1, 1, 2, 64), c, c, i32(3), i32(0, 1)[None])
+        assert [x._version for x in c] == before
