@@ -149,6 +149,15 @@ def _check_pages_enabled() -> bool:
     return os.environ.get("MTLFLASHATTN_CHECK_PAGES", "").lower() in ("1", "on", "true", "yes")
 
 
+_INT32_MAX = 0x7fffffff
+
+
+def _check_sizes(*sizes):
+    """Sizes for the library's 32-bit fields (ctypes would cut larger ones off without a word)."""
+    if max(sizes) > _INT32_MAX:
+        raise ValueError(f"mtlflashattn_amd: a size of {max(sizes)} (at most 2^31 - 1 are supported)")
+
+
 def _check_options(window_size, softcap, alibi_slopes):
     """The window, soft-cap and ALiBi arguments (metal_flash_attn/__init__.py:31-46)."""
     if (

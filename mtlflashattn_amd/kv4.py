@@ -100,7 +100,8 @@ def _cache_struct(c, k_cache, v_cache, block_table):
             s if n > 1 else 0 for s, n in zip(codes.stride()[:3], codes.shape[:3]))
         pool.scale_page_stride, pool.scale_row_stride, pool.scale_head_stride = (
             s if n > 1 else 0 for s, n in zip(scales.stride()[:3], scales.shape[:3]))
-    c.num_pages, c.page_block_size = k_cache[0].shape[:2]
+    c.num_pages, c.page_block_size = pages, page = k_cache[0].shape[:2]
+    _kernel._check_sizes(pages, block_table.shape[1] * page)  # (rows that a sequence's table names)
     c.max_pages = block_table.shape[1]
     c.block_table_batch_stride = block_table.stride(0) if block_table.shape[0] > 1 else 0
 
@@ -218,6 +219,7 @@ def _append_plan(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table)
     for c in (*k_cache, *v_cache):
         if any(s == 0 for s, n in zip(c.stride()[:3], c.shape[:3]) if n > 1):
             raise ValueError("mtlflashattn_amd: an expanded cache (rows that share memory) cannot be written")
+    _kernel._check_sizes(total, Hkv, batch)
     p = _hip.MfaKv4AppendParams()
     _cache_struct(p.cache, k_cache, v_cache, block_table)
     p.k_token_stride, p.k_head_stride = _token_strides(k)
@@ -277,7 +279,9 @@ def _attend(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale
     _kernel._check_options(window_size, softcap, alibi_slopes)
     # (numbers, so that the signature holds a value whatever type it came in)
     softmax_scale = None if softmax_scale is None else float(softmax_scale)
-    softcap, window_size = float(softcap), (int(window_size[0]), int(window_size[1]))
+    # (a window as wide as a 32-bit number is as good as none)
+    most = _kernel._INT32_MAX
+    softcap, window_size = float(softcap), (min(int(window_size[0]), most), min(int(window_size[1]), most))
     max_seqlen_k = None if max_seqlen_k is None else int(max_seqlen_k)
     try:
         (kc, ks), (vc, vs) = k_cache, v_cache
@@ -357,6 +361,7 @@ def _attend_plan(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_
     if max_seqlen_k is not None and max_seqlen_k < 0:
         raise ValueError("mtlflashattn_amd: max_seqlen_k must be >= 0")
     _kernel._alibi_arg(alibi_slopes, batch, Hq, q.device)
+    _kernel._check_sizes(*q.shape, batch)
     p = _hip.MfaKv4FwdParams()
     _cache_struct(p.cache, k_cache, v_cache, block_table)
     p.batch, p.heads_q, p.heads_kv, p.head_dim = batch, Hq, Hkv, D
@@ -446,6 +451,7 @@ def _copy_plan(pools, src, dst):
     device, num_pages = pools[0].device, pools[0].shape[0]
     _check_ints(src, src.shape[0], device, "src")
     _check_ints(dst, src.shape[0], device, "dst")
+    _kernel._check_sizes(num_pages, src.shape[0])
     templates = []
     for first in range(0, len(pools), _hip.MFA_COPY_MAX_POOLS):
         p = _hip.MfaCopyPagesParams()

@@ -114,6 +114,7 @@ def _check(q, k, q_weight, k_weight, cos, sin, positions, eps):
                              f"{tuple(q.shape[-3:-2])}")
     if not eps >= 0:
         raise ValueError("mtlflashattn_amd: eps must be >= 0")
+    _kernel._check_sizes(*q.shape, *k.shape, cos.shape[0])
     _kernel._check_device(q, *weights, cos, sin, *([positions] if positions is not None else []))
 
 

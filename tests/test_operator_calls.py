@@ -160,3 +160,55 @@ class TestVersionCounters:
         before = [x._version for x in c]
         mfa.flash_attn_kv4_func(t(1, 1, 2, 64), c, c, i32(3), i32(0, 1)[None])
         assert [x._version for x in c] == before
+
+
+class TestSizesBeyond32Bits:
+    """Sizes that the library's 32-bit fields cannot hold are refused, not cut off."""
+
+    @pytest.mark.parametrize("n", [1 << 31, (1 << 32) + 3])
+    def test_append(self, launches, n):
+        c = mfa.kv4_cache(2, 64, 2, 64, device="cpu")
+        k = t(1, 2, 64).expand(n, 2, 64)
+        with pytest.raises(ValueError, match="2\\^31"):
+            mfa.kv4_append(k, k, c, c, i32(0, 3), i32(0), i32(0, 1)[None])
+        assert not launches
+
+    @pytest.mark.parametrize("n", [1 << 31, (1 << 32) + 3])
+    def test_pages(self, launches, n):
+        c = tuple(x[:1].expand(n, -1, -1, -1) for x in mfa.kv4_cache(2, 64, 2, 64, device="cpu"))
+        with pytest.raises(ValueError, match="2\\^31"):
+            mfa.flash_attn_kv4_func(t(1, 1, 2, 64), c, c, i32(3), i32(0, 1)[None])
+        with pytest.raises(ValueError, match="2\\^31"):
+            mfa.copy_cache_pages([torch.empty(n, 0)], i32(0), i32(1))
+        with pytest.raises(ValueError, match="2\\^31"):
+            mfa.copy_cache_pages([t(4, 8)], i32(0).expand(n), i32(1).expand(n))
+        assert not launches
+
+    @pytest.mark.parametrize("cols", [1 << 25, (1 << 26), (1 << 26) + 1])
+    def test_tables(self, launches, cols):
+        """Tables that name 2^31 rows and more (the memory is not touched)."""
+        c = mfa.kv4_cache(2, 64, 2, 64, device="cpu")
+        table = torch.empty(1, cols, dtype=torch.int32)
+        with pytest.raises(ValueError, match="2\\^31"):
+            mfa.flash_attn_kv4_func(t(1, 1, 2, 64), c, c, i32(3), table)
+        with pytest.raises(ValueError, match="2\\^31"):
+            mfa.kv4_append(t(3, 2, 64), t(3, 2, 64), c, c, i32(0, 3), i32(0), table)
+        assert not launches
+
+    @pytest.mark.parametrize("n", [1 << 31, (1 << 32) + 3])
+    def test_norm_and_rotation(self, launches, n):
+        table, few = t(1, 4).expand(n, 4), t(1, 4)
+        x = t(5, 2, 64)
+        with pytest.raises(ValueError, match="2\\^31"):
+            mfa.qk_norm_rope(x, x, None, None, table, table)
+        q = t(1, 1, 64).expand(n, 1, 64)
+        with pytest.raises(ValueError, match="2\\^31"):
+            mfa.qk_norm_rope(q, q, None, None, few, few)
+        assert not launches
+
+    @pytest.mark.parametrize("window", [(1 << 31, 1 << 32), (1 << 40, 1 << 63)])
+    def test_windows_are_unbounded(self, launches, window):
+        c = mfa.kv4_cache(2, 64, 2, 64, device="cpu")
+        mfa.flash_attn_kv4_func(t(1, 1, 2, 64), c, c, i32(3), i32(0, 1)[None], window_size=window)
+        p = launches[0][1]
+        assert min(p.window_left, p.window_right) >= (1 << 31) - 1
