@@ -438,7 +438,8 @@ int mfa_kv4_append_params_size(void);
  * (tokens of no sequence get 0, lse -inf).  The query rows are the last
  * positions of their sequence.  q and o: fp16 or bf16, 16-byte aligned, strides
  * multiples of 8 elements.  head_dim: 32, 64, 96 or 128.  A NaN of V reaches only
- * the rows whose mask holds its key.  With fp16 queries and more than 32 rows per
+ * the rows whose mask holds its key; elements of V of 2^128 and more (scale bytes
+ * 253 and 254) count as 1.5 * 2^127, so that they reach no other row either.  With fp16 queries and more than 32 rows per
  * K/V head in a sequence (positions times heads), elements of K and V beyond
  * +/-65504 saturate.
  * Enqueues up to three kernels; never synchronizes, never allocates.  The results

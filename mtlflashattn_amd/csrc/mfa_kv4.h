@@ -65,6 +65,18 @@ __device__ __forceinline__ u32x4_t kv4_f16x8(uint32_t w, float s) {
     return r;
 }
 
+// Eight codes of V of a group whose elements may pass the range of fp32 and bf16
+// (scale bytes 253 and 254), saturated to 1.5 * 2^127: magnitudes above 3 * 2^126
+// (code 5) or 1.5 * 2^127 (code 3) become those.  An infinite element would reach
+// the rows that mask its key, as 0 * inf.
+__device__ __forceinline__ bool kv4_beyond(uint32_t byte) { return byte == 253 || byte == 254; }
+__device__ __forceinline__ uint32_t kv4_saturate8(uint32_t w, uint32_t byte) {
+    const uint32_t top = byte == 253 ? 5 : 3;
+    // (bit 3 of a half byte that holds magnitude + 7 - top: magnitude > top)
+    const uint32_t over = ((w & 0x77777777u) + (7 - top) * 0x11111111u) >> 3 & 0x11111111u;
+    return (w & ~(over * 7)) | over * top;
+}
+
 // j / d for 0 <= j < 2^31 as umulhi(j, m) >> s (round-up method: l = ceil(log2
 // d), m = ceil(2^(31+l) / d) < 2^32, s = l - 1; d = 1 is m = 0, s = 0 and is
 // taken by the caller's quotient()).

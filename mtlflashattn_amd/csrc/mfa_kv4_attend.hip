@@ -332,10 +332,15 @@ mfa_kv4_kernel(K4Args) {
                 nans[i] = __ballot(nan);
                 if (32 * GPR % 64 == 0 || 64 * i + lane < 32 * GPR) {
                     const float s = nan ? 0.f : kv4_scale(w.vs[i]);
+                    u32x4_t codes = w.v[i];
+                    if (__builtin_expect(kv4_beyond(w.vs[i]), 0)) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) codes[e] = kv4_saturate8(codes[e], w.vs[i]);
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         *reinterpret_cast<u32x4_t*>(vt + vrow[i] * DP + (((4 * vgrp[i] + e) ^ vswz(vrow[i])) << 3)) =
-                            kv4_bf16x8(w.v[i][e], s);
+                            kv4_bf16x8(codes[e], s);
                 }
             }
             refill();

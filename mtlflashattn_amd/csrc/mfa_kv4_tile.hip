@@ -140,6 +140,12 @@ mfa_kv4_tile_kernel(K4Args) {
                     const bool nan = part & gv[i] & (gs[i] == 255);
                     nan_s[to][gv[i] && lane == 0 ? (tid + kThreads4 * i - kTK * GPR) >> 6 : GPR] = __ballot(nan);
                     const float s = nan ? 0.f : kv4_scale(gs[i]);
+                    if constexpr (IS_BF16) {  // (fp16 saturates below; the test costs 1 % of the chunk above)
+                        if (__builtin_expect(gv[i] && kv4_beyond(gs[i]), 0)) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) gc[i][e] = kv4_saturate8(gc[i][e], gs[i]);
+                        }
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         *reinterpret_cast<u32x4_t*>(p + 8 * (e ^ gsw[i])) = IS_BF16 ? kv4_bf16x8(gc[i][e], s) : kv4_f16x8(gc[i][e], s);

@@ -124,3 +124,65 @@ def test_c_rows_of_no_sequences_are_cleared():
     _hip.kv4_fwd(p, ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()
     assert not out.any() and bool((lse == float("-inf")).all())
+
+
+LEVELS = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.0, -0.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float64)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("lq,Hq,window", [(1, 4, (40, 0)), (5, 4, (-1, 0)), (9, 6, (33, 0)), (70, 4, (-1, 0)),
+                                          (70, 4, (50, 3)), (150, 2, (-1, -1))])
+def test_values_beyond_the_range_reach_only_the_rows_that_see_them(lq, Hq, window, D, dtype):
+    """Groups of V with elements of 2^128 and more (scales 2^126 and 2^127, what
+    kv4_append makes of the type's largest values): every row that masks their key
+    has the bits that it has without them; bf16 rows that see one get it as +/-1.5 *
+    2^127.  One such group per head and 32 elements, so a row's sum stays below 2^128;
+    bound there: the rounding of the result, and of its probability to one bf16 term
+    (2^-8 each of the largest value), next to 3e-4 for the rest."""
+    L, page, pages = 333, 64, 9
+    g = torch.Generator().manual_seed(D)
+    kc, vc = (tuple(torch.randint(lo, hi, (pages, 2, page, n), generator=g, dtype=torch.uint8).to(DEV).transpose(1, 2)
+                    for n, lo, hi in ((D // 2, 0, 256), (D // 32, 123, 127))) for _ in range(2))
+    table = torch.randperm(pages, generator=g)[None].to(DEV, torch.int32)
+    q, lens = torch.randn(1, lq, Hq, D, generator=g).to(DEV, dtype), i32(L)
+
+    def call():
+        return mfa.flash_attn_kv4_func(q, kc, vc, lens, table, window_size=window)[0].cpu()
+
+    i, j = torch.arange(lq)[:, None] + L - lq, torch.arange(L)[None]
+    seen = torch.ones(lq, L, dtype=torch.bool)
+    if window[0] >= 0:
+        seen &= j >= i - window[0]
+    if window[1] >= 0:
+        seen &= j <= i + window[1]
+    groups = D // 32
+    spots = {(0, 0): (L - 1, 253), (1, groups - 1): (L - lq // 2 - 1, 254)}
+    spots.setdefault((0, groups - 1), (max(L - lq - 36, 0), 254))
+    spots.setdefault((1, 0), (258, 253))
+    want = torch.zeros(lq, Hq, D, dtype=torch.bool)
+    for (h, grp), (key, byte) in spots.items():
+        p = table[0, key // page].item()
+        vc[0][p, key % page, h, 16 * grp:16 * grp + 8] = torch.tensor([0x67, 0xEF, 0x54, 0xDC, 0x32, 0xBA, 0x10, 0x98],
+                                                                      dtype=torch.uint8, device=DEV)
+    clean = call()  # (the codes with ordinary scales)
+    for (h, grp), (key, byte) in spots.items():
+        vc[1][table[0, key // page].item(), key % page, h, grp] = byte
+        want[:, h * Hq // 2:(h + 1) * Hq // 2, 32 * grp:32 * grp + 32] |= seen[:, key][:, None, None]
+    out = call()
+    assert torch.equal(out[~want], clean[~want])
+    if dtype == torch.float16:
+        return
+    rows = []
+    for codes, scales in (kc, vc):
+        codes, scales = (x.cpu()[table[0].cpu().long()].flatten(0, 1)[:L] for x in (codes, scales))
+        x = torch.stack((LEVELS[codes.long() & 15], LEVELS[codes.long() >> 4]), -1).flatten(-2)
+        x = x * torch.pow(2.0, scales.double() - 127).repeat_interleave(32, -1)
+        rows.append(x.clamp(-1.5 * 2.0 ** 127, 1.5 * 2.0 ** 127))
+    ref = torch.zeros(lq, Hq, D, dtype=torch.float64)
+    for h in range(Hq):
+        s = (q[0, :, h].cpu().double() @ rows[0][:, h * 2 // Hq].T / D ** 0.5).masked_fill(~seen, -float("inf"))
+        p = torch.softmax(s, -1)
+        ref[:, h] = p @ rows[1][:, h * 2 // Hq]
+    err = (out.double() - ref).abs()[want]
+    assert bool((err <= (2.0 ** -8 * 2 + 3e-4) * 1.5 * 2.0 ** 127).all()) and bool(out[want].isfinite().all())
