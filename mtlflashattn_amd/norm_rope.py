@@ -204,7 +204,9 @@ class _QkNormRopeFn(torch.autograd.Function):
         plan, device = _plan(q, k, q_weight, k_weight, cos, sin, positions, *ctx.options), q.device
         b = _hip.MfaNormRopeBwdParams.from_buffer_copy(plan.bwd)
         held = _fill(b.fwd, plan, q, k, q_weight, k_weight, cos, sin, positions)  # noqa: F841 (kept until the launch)
-        dq_out, dk_out = _rows(dq_out.to(q.dtype)), _rows(dk_out.to(k.dtype))
+        if dq_out.dtype is not q.dtype or dk_out.dtype is not k.dtype:
+            dq_out, dk_out = dq_out.to(q.dtype), dk_out.to(k.dtype)
+        dq_out, dk_out = _rows(dq_out), _rows(dk_out)
         if not dq_out.is_contiguous():
             b.dqo_batch_stride, b.dqo_seq_stride, b.dqo_head_stride = _strides(dq_out)
         if not dk_out.is_contiguous():
