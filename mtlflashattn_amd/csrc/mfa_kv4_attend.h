@@ -64,7 +64,7 @@ __device__ __forceinline__ int lo4(int wl, int c) { return wl >= 0 ? max(c - wl,
 __device__ __forceinline__ int hi4(int causal, int wr, int c, int Lk) {
     int hi = Lk - 1;
     if (causal) hi = min(hi, c);
-    if (wr >= 0) hi = min(hi, c + wr);
+    if (wr >= 0 && wr < hi - c) hi = c + wr;  // (c + wr may pass 31 bits)
     return hi;
 }
 

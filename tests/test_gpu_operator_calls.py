@@ -186,3 +186,21 @@ def test_values_beyond_the_range_reach_only_the_rows_that_see_them(lq, Hq, windo
         ref[:, h] = p @ rows[1][:, h * 2 // Hq]
     err = (out.double() - ref).abs()[want]
     assert bool((err <= (2.0 ** -8 * 2 + 3e-4) * 1.5 * 2.0 ** 127).all()) and bool(out[want].isfinite().all())
+
+
+@pytest.mark.parametrize("lq,Hq,window", [(1, 4, (100, 300)), (5, 4, (0, 300)), (70, 4, (100, 300))])
+def test_right_window_at_the_longest_sequence(lq, Hq, window):
+    """The last positions of 2^31 - 256 keys (a table that repeats five pages), whose
+    right window's end has no 32-bit number: the bits of the same keys in a short
+    sequence with a window that ends behind them."""
+    page, pages, D, cols = 256, 5, 64, (1 << 23) - 1
+    g = torch.Generator().manual_seed(lq)
+    kc, vc = (tuple(torch.randint(lo, hi, (pages, 2, page, n), generator=g, dtype=torch.uint8).to(DEV).transpose(1, 2)
+                    for n, lo, hi in ((D // 2, 0, 256), (D // 32, 123, 127))) for _ in range(2))
+    q = torch.randn(1, lq, Hq, D, generator=g).to(DEV, torch.bfloat16)
+    table = (torch.arange(cols, dtype=torch.int32, device=DEV) % pages)[None]
+    first = (cols - 4) // 2 * 2  # (the last pages from a multiple of a chunk of both)
+    short = table[:, first:].contiguous()
+    want = mfa.flash_attn_kv4_func(q, kc, vc, i32(short.shape[1] * page), short, window_size=(window[0], 300))
+    got = mfa.flash_attn_kv4_func(q, kc, vc, i32(cols * page), table, window_size=window)
+    assert bool(want.any(-1).all()) and torch.equal(got, want)
