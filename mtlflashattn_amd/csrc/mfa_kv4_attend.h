@@ -68,6 +68,17 @@ __device__ __forceinline__ int hi4(int causal, int wr, int c, int Lk) {
     return hi;
 }
 
+// The chunks with keys among chunks c0 to c0 + nch - 1 of a unit with keys t_lo to
+// t_hi, counted from the sequence's first key (none: beg = end, behind t_hi; the
+// dealt ones behind it may begin past 31 bits).
+struct Chunks4 {
+    int beg, end;
+};
+__device__ __forceinline__ Chunks4 chunks4(int t_lo, int t_hi, int c0, int nch) {
+    const int past = t_hi < 0 ? 0 : t_hi / kChunk4 + 1, beg = t_lo / kChunk4 + c0;
+    return Chunks4{min(beg, past), min(beg + nch, past)};
+}
+
 // The work of a sequence: its rows, keys, column tiles and chunks per unit.
 struct Seq4 {
     int q0, Lq, Lk, tiles, chunks;

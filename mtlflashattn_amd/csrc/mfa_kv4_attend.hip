@@ -200,7 +200,7 @@ mfa_kv4_kernel(K4Args) {
         // the keys of any column, and of every column, of the tile
         const int t_lo = lo4(a.wl, i_first + dq), t_hi = hi4(a.causal, a.wr, i_last + dq, Lk);
         const int f_lo = lo4(a.wl, i_last + dq), f_hi = hi4(a.causal, a.wr, i_first + dq, Lk);
-        const int key0 = (t_lo / kChunk4 + wk.c0) * kChunk4 + 32 * wave;
+        const int key0 = chunks4(t_lo, t_hi, wk.c0, wk.nch).beg * kChunk4 + 32 * wave;
         // this wavefront's blocks with keys: n0 .. n1 - 1
         const int n0 = t_lo - key0 > 31 ? 1 : 0;  // (only the first chunk may begin outside)
         const int n1 = t_hi < key0 ? 0 : min(wk.nch, (t_hi - key0) / kChunk4 + 1);

@@ -86,8 +86,8 @@ mfa_kv4_tile_kernel(K4Args) {
         // key ranges: of the tile, and those that all columns of the tile or of this wavefront see
         const int i_first = (int)div4(wk.col0, a.by_r), i_last = (int)div4(wk.col0 + wk.ncol - 1, a.by_r);
         const int t_lo = lo4(a.wl, i_first + dq), t_hi = hi4(a.causal, a.wr, i_last + dq, Lk);
-        const int key0 = (t_lo / kChunk4 + wk.c0) * kChunk4;
-        const int jbeg = max(key0, t_lo / kTK * kTK), jend = min(key0 + wk.nch * kChunk4, t_hi + 1);
+        const Chunks4 ch = chunks4(t_lo, t_hi, wk.c0, wk.nch);
+        const int jbeg = max(ch.beg * kChunk4, t_lo / kTK * kTK), jend = min(ch.end * kChunk4, t_hi + 1);
         const int wcol = wk.col0 + 32 * wave, wlast = min(wcol + 32, wk.col0 + wk.ncol) - 1;
         const bool live = wlast >= wcol;
         const int wi0 = (int)div4(wcol, a.by_r), wi1 = (int)div4(max(wlast, wcol), a.by_r);

@@ -188,10 +188,12 @@ def test_values_beyond_the_range_reach_only_the_rows_that_see_them(lq, Hq, windo
     assert bool((err <= (2.0 ** -8 * 2 + 3e-4) * 1.5 * 2.0 ** 127).all()) and bool(out[want].isfinite().all())
 
 
-@pytest.mark.parametrize("lq,Hq,window", [(1, 4, (100, 300)), (5, 4, (0, 300)), (70, 4, (100, 300))])
+@pytest.mark.parametrize("lq,Hq,window", [(1, 4, (100, 300)), (5, 4, (0, 300)), (70, 4, (100, 300)),
+                                          (70, 4, (100, 1 << 29)), (3, 4, (100, 1 << 29)), (70, 4, (100, -1)), (3, 4, (100, -1))])
 def test_right_window_at_the_longest_sequence(lq, Hq, window):
     """The last positions of 2^31 - 256 keys (a table that repeats five pages), whose
-    right window's end has no 32-bit number: the bits of the same keys in a short
+    right window's end has no 32-bit number, nor the chunks of the window that lie
+    behind the last key: the bits of the same keys in a short
     sequence with a window that ends behind them."""
     page, pages, D, cols = 256, 5, 64, (1 << 23) - 1
     g = torch.Generator().manual_seed(lq)
