@@ -60,7 +60,7 @@ __device__ __forceinline__ uint32_t div4(uint32_t j, const __attribute__((addres
     return f.d <= 1 ? j : __umulhi(j, f.m) >> f.s;
 }
 
-__device__ __forceinline__ int lo4(int wl, int c) { return wl >= 0 ? max(c - wl, 0) : 0; }
+__device__ __forceinline__ int lo4(int wl, int c) { return wl >= 0 && c > wl ? c - wl : 0; }
 __device__ __forceinline__ int hi4(int causal, int wr, int c, int Lk) {
     int hi = Lk - 1;
     if (causal) hi = min(hi, c);

@@ -690,10 +690,9 @@ int k4_plan(const mfa_kv4_fwd_params* p, K4Plan* plan, int cus) {
     a.softcap = p->softcap;
     a.softcap_sk = p->softcap > 0.f ? p->scale * (2.f * kLog2e / p->softcap) : 0.f;
     a.bias = p->softcap > 0.f || p->alibi_slopes || !(p->scale > 0.f);
-    // clamp windows so center +/- window cannot overflow int32
-    const int64_t wmax = std::min<int64_t>(rows + (int64_t)a.max_k + 1, 0x3fffffff);
-    a.wl = p->window_left < 0 ? -1 : (int32_t)std::min<int64_t>(p->window_left, wmax);
-    a.wr = p->window_right < 0 ? -1 : (int32_t)std::min<int64_t>(p->window_right, wmax);
+    // (a window that holds every key of every row is none)
+    a.wl = p->window_left >= a.max_k ? -1 : p->window_left;
+    a.wr = p->window_right >= rows + a.max_k ? -1 : p->window_right;
     a.causal = p->causal ? 1 : 0;
     if (rows > 0x3fffffff || rows * a.Hq > 0x3fffffff) return k4err(MFA_ERR_INVALID, "mfa_kv4_fwd: problem too large");
 

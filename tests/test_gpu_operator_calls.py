@@ -206,3 +206,46 @@ def test_right_window_at_the_longest_sequence(lq, Hq, window):
     want = mfa.flash_attn_kv4_func(q, kc, vc, i32(short.shape[1] * page), short, window_size=(window[0], 300))
     got = mfa.flash_attn_kv4_func(q, kc, vc, i32(cols * page), table, window_size=window)
     assert bool(want.any(-1).all()) and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("lq", [1, 40])
+def test_left_windows_above_2_30_keys(lq):
+    """2^31 - 256 keys that repeat every 1280: a window of w keys has w / 1280 of their
+    sum, so the log-sum-exp differs from the whole row's by the logarithm of the shares
+    (a walk adds at most 2^31 / (512 * 64) = 2^16 blocks in fp32: 2^16 * 2^-24 = 2^-8 of
+    either sum)."""
+    page, pages, D, cols = 256, 5, 32, (1 << 23) - 1
+    g = torch.Generator().manual_seed(lq)
+    kc, vc = (tuple(torch.randint(lo, hi, (pages, 1, page, n), generator=g, dtype=torch.uint8).to(DEV).transpose(1, 2)
+                    for n, lo, hi in ((D // 2, 0, 256), (D // 32, 123, 127))) for _ in range(2))
+    q = torch.randn(1, lq, 2, D, generator=g).to(DEV, torch.bfloat16)
+    table = (torch.arange(cols, dtype=torch.int32, device=DEV) % pages)[None]
+    n = cols * page
+
+    def lse(left):
+        return mfa.flash_attn_kv4_func(q, kc, vc, i32(n), table, causal=True, window_size=(left, 0),
+                                       return_softmax_lse=True)[1]
+
+    whole = lse(-1)
+    assert torch.equal(lse(n), whole) and torch.equal(lse((1 << 31) - 1), whole) and torch.equal(lse(1 << 40), whole)
+    for w in (5 << 28, 3 << 28):
+        want = whole.double() + torch.log(torch.tensor(w / n, dtype=torch.float64))
+        assert float((lse(w).double() - want).abs().max()) <= 2.0 ** -8 * 2
+
+
+def test_gradients_of_a_checkpointed_block():
+    """Recomputed inputs (torch.utils.checkpoint works through saved-tensor hooks)."""
+    from torch.utils.checkpoint import checkpoint
+
+    qkv = torch.randn(200, 12, 64, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    w = torch.ones(64, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    table = torch.randn(200, 32, device=DEV)
+
+    def block(x):
+        q, k = mfa.qk_norm_rope(x[:, :8], x[:, 8:10], w, w, table, table)
+        return mfa.flash_attn_func(q[None], k[None], x[None, :, 10:], causal=True)
+
+    up = torch.randn(1, 200, 8, 64, device=DEV, dtype=torch.bfloat16)
+    want = torch.autograd.grad(block(qkv), (qkv, w), up)
+    got = torch.autograd.grad(checkpoint(block, qkv, use_reentrant=False), (qkv, w), up)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
