@@ -439,9 +439,13 @@ int mfa_kv4_append_params_size(void);
  * positions of their sequence.  q and o: fp16 or bf16, 16-byte aligned, strides
  * multiples of 8 elements.  head_dim: 32, 64, 96 or 128.  A NaN of V reaches only
  * the rows whose mask holds its key; elements of V of 2^128 and more (scale bytes
- * 253 and 254) count as 1.5 * 2^127, so that they reach no other row either.  With fp16 queries and more than 32 rows per
- * K/V head in a sequence (positions times heads), elements of K and V beyond
- * +/-65504 saturate.
+ * 253 and 254) count as 1.5 * 2^127, so that they reach no other row either.
+ * The columns of a sequence are its query positions times the query heads per K/V
+ * head.  Sequences of more than 32 columns, and in a varlen call of more than 32
+ * columns in total those of more than 16, run on tiles of 128 columns: there a
+ * probability is rounded to one 16-bit term (elsewhere to two bf16 terms), and with
+ * fp16 queries K and V are rounded to fp16, so that elements beyond +/-65504 saturate
+ * and those of groups with scales below 2^-23 lose bits (elsewhere both are exact).
  * Enqueues up to three kernels; never synchronizes, never allocates.  The results
  * do not depend on the workspace's address or content; they may differ in the
  * last bit with the batch a sequence stands in (its keys are dealt over
@@ -539,7 +543,7 @@ int mfa_norm_rope_params_size(void);
  *   dq = (h - n mean(h n)) / sqrt(mean(x^2) + eps),  dq_weight = sum over rows g n
  * and the same for k.  dq / dk are contiguous.  Weight gradients (dtype_weight)
  * where the weight is set and the pointer is not NULL: summed in fp32, in an
- * order that the sizes alone decide.  `workspace`: 256-byte aligned, at least
+ * order that sizes, strides and alignment decide.  `workspace`: 256-byte aligned, at least
  * mfa_norm_rope_bwd_workspace_bytes bytes.  One or two kernels; never
  * synchronizes, never allocates.
  */

@@ -50,8 +50,11 @@ __device__ __forceinline__ u32x4_t kv4_bf16x8(uint32_t w, float s) {
     return r;
 }
 
-// ... as eight fp16, saturating: 65504 may be held as 4 * 2^14, one step above
-// fp16's range (IEEE minimum and maximum: NaN stays NaN).
+// ... as eight fp16, the operand type of fp16 queries in the 128-column kernel (bf16
+// operands, exact, would need the queries as two terms and twice the products):
+// saturating, as 65504 may be held as 4 * 2^14, one step above fp16's range (IEEE
+// minimum and maximum: NaN stays NaN), and rounded where 2^-24 is above half a unit of
+// the scale, below 2^-23.
 __device__ __forceinline__ u32x4_t kv4_f16x8(uint32_t w, float s) {
     const k4_f16x2_t top = {(_Float16)65504.f, (_Float16)65504.f};
     auto sat = [&](k4_f16x2_t x) {

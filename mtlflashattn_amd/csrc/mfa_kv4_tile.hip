@@ -8,11 +8,13 @@
 // saturating in fp16).  There are two tiles: the next 64 keys are converted between
 // the products of the current ones, and the codes of the 64 after those are on
 // their way into registers.  1024 rows over 16384 keys, Hq=32 Hkv=8 D=128 bf16,
-// take 316 to 324 us (822 to 843 TFLOP/s; one tile, converted between two barriers: 329 to
-// 334), and with soft-cap over 8192 keys 206 (220).  Bound by no one unit: the
-// matrix pipe is busy 39 % of the time and LDS 48 %; taken out one at a time (of
-// 332 us), the products of the scores are worth 64 us, those of the values 37, the
-// softmax 43, the conversion 50 and most reads of K 17.
+// take 298 to 304 us with the merge in a timed loop (876 to 893 TFLOP/s), the kernel
+// alone 324 to 340 in short traces over machines (side by side on one: 316 to 324, and
+// 329 to 334 with one tile, converted between two barriers); over 8192 keys 167 us,
+// with soft-cap 212, with ALiBi 188.  Bound by no one unit: the matrix pipe is busy 40 % of the time, LDS bank conflicts take 10 % of it.
+// In the form with one tile (332 us), with one part taken out at a time, the products
+// of the scores were worth 64 us, those of the values 37, the softmax 43, the
+// conversion 50 and most reads of K 17.
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16: a lane owns a column, its
 // probabilities go from the accumulators into the second product as they are, and
 // V is read transposed (ds_read_b64_tr_b16).  Exponent references are integers
@@ -280,7 +282,11 @@ mfa_kv4_tile_kernel(K4Args) {
                 m = mn;
             }
             const float mu = m == -INFINITY ? 0.f : m;
-            // probabilities rounded to 16 bits; l adds them as rounded.  The second 32
+            // probabilities rounded to 16 bits; l adds them as rounded.  (A second term
+            // doubles the values' products: the chunk above takes 395 us, not 303, a mixed
+            // step 97, not 87.  One term has an error of 1.4 times that of rounding the
+            // result: 4.3e-5 rms against 3.1e-5 for results of 1.8e-2 over 8192 keys in
+            // bf16, 5.4e-6 against 3.8e-6 in fp16; two have the latter.)  The second 32
             // keys' are formed while the first's products run.
             float acc[2] = {0.f, 0.f};
 #pragma unroll

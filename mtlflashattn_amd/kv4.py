@@ -247,7 +247,11 @@ def flash_attn_kv4_func(q, k_cache, v_cache, cache_seqlens, block_table, softmax
     Lengths and page ids are read on the device (no synchronisation: a call can be
     captured into a graph and replayed as the sequences grow).  A sequence has at
     most max_seqlen_k keys (None: as many as the table names); a tight bound keeps
-    the workspace and the grid small.  A page id outside the pool reads as zeros and
+    the workspace and the grid small.  Sequences of more than 32 columns (query
+    positions times heads per K/V head) run on tiles of 128 columns, whose
+    probabilities are rounded once to q.dtype (bf16: an error of 1.4 times the output's
+    rounding alone) and which, for fp16 queries, round K and V to fp16 (beyond 65504
+    they saturate); fewer columns keep two terms and exact K and V.  A page id outside the pool reads as zeros and
     its keys are not masked; MTLFLASHATTN_CHECK_PAGES=1 checks the ids on the host.
     Forward only: a query that requires grad raises.
     """
@@ -265,7 +269,10 @@ def flash_attn_varlen_kv4_func(q, k_cache, v_cache, cu_seqlens_q, cache_seqlens,
 
     q: [total, Hq, D] packed without padding, sequence b owning rows
     [cu_seqlens_q[b], cu_seqlens_q[b + 1]) (int32 [B + 1], read on the device; it must
-    be non-decreasing).  Rows of no sequence come back as 0.  Returns [total, Hq, D]
+    be non-decreasing).  Rows of no sequence come back as 0 (one workgroup clears them:
+    8128 rows of 32 x 128 take 1 ms, so a captured step is padded little).  In a call
+    of more than 32 columns in total sequences of more than 16 run on the tiles of 128.
+    Returns [total, Hq, D]
     and, if asked, the log-sum-exp [Hq, total].
     """
     if torch.is_tensor(q) and q.dim() != 3:

@@ -30,8 +30,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps=1e-6, i
     2, ... in each sequence.  They are read on the device: a position outside the
     tables gives NaN in the rotated elements (never a read out of bounds).
     Arithmetic is fp32, rounded once.  Differentiable in q, k and the weights
-    (weight gradients are summed in fp32 in a fixed order: the same bits every
-    time); cos and sin are constants.  Forward and backward can be captured into a
+    (weight gradients are summed in fp32 in an order that sizes, strides and alignment
+    decide: the same bits for the same layout); cos and sin are constants.  Forward and backward can be captured into a
     graph; as for every operator, no eager autograd graph of the same leaves may be
     alive while a backward is captured.
     """
