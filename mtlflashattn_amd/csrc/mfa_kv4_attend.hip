@@ -702,7 +702,7 @@ int k4_plan(const mfa_kv4_fwd_params* p, K4Plan* plan, int cus) {
     // (no sequences: the launch only clears the rows)
     const int64_t cols = p->batch == 0 ? 1 : (varlen ? rows : p->seqlen_q) * (int64_t)a.R;
     plan->n = varlen && cols > 16 ? 2 : 1;
-    const int64_t chunks = std::max<int64_t>(1, ((int64_t)a.max_k + kChunk4 - 1) / kChunk4);
+    const int64_t chunks = p->batch == 0 ? 1 : std::max<int64_t>(1, ((int64_t)a.max_k + kChunk4 - 1) / kChunk4);
     for (int i = 0; i < plan->n; ++i) {
         K4Launch& l = plan->l[i];
         l.a = a;
