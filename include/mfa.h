@@ -473,6 +473,98 @@ int mfa_kv4_fwd(const mfa_kv4_fwd_params* params, void* workspace, int64_t works
 int mfa_kv4_fwd_params_size(void);
 
 /*
+ * Paged 8-bit K/V cache.  No counterpart in the reference.
+ *
+ * The structures, tables and rules of the 4-bit cache with another format: a row of
+ * one head has head_dim code bytes, contiguous, each an e4m3 float (sign, four
+ * exponent bits with bias 7, three mantissa bits; largest 448, 0x7f and 0xff NaN);
+ * the 64 rows of a block (rows 64 i to 64 i + 63 of a page) and a head share the power
+ * of two 2^(s - 127) of one scale byte s (0 stands for 0).  scale_row_stride is the
+ * bytes between the scales of neighbouring blocks: scales are [num_pages,
+ * page_block_size / 64, heads_kv].
+ */
+#define MFA_KV8_BLOCK 64
+typedef mfa_kv4_pool mfa_kv8_pool;
+typedef mfa_kv4_cache mfa_kv8_cache;
+
+/*
+ * New rows into the cache: the parameters of mfa_kv4_append.  The byte of a block is
+ * the smallest from 1 on with 448 * 2^(s - 127) at least the largest finite magnitude
+ * of the rows that are written into it; where the block holds rows of the sequence
+ * already (cache_seqlens is no multiple of 64), at least the byte that it had, and if
+ * the byte rises the codes of those rows are rounded again.  Elements are rounded to
+ * the nearest code, ties to the even one; infinities and NaN become NaN.  What stands
+ * in a block behind the last row may change its value with the byte.  No two sequences
+ * may write into one block.  A negative length counts as 0.  Values of tokens of no
+ * sequence are 0; values of rows that are dropped are those of a block that holds
+ * the call's rows alone; fp16 values saturate at +/-65504.  head_dim: 32, 64, 96 or
+ * 128.  One kernel; never synchronizes, never allocates.
+ */
+typedef mfa_kv4_append_params mfa_kv8_append_params;
+int mfa_kv8_append(const mfa_kv8_append_params* params, void* stream);
+int mfa_kv8_append_params_size(void);
+
+/*
+ * Attention over the cache: the parameters and rules of mfa_kv4_fwd.  A NaN element of
+ * V reaches only the rows whose mask holds its key.  K is exact; V is exact with bf16
+ * queries and for at most 32 columns; on the tiles of 128 columns fp16 queries take V
+ * rounded to fp16 (elements beyond +/-65504 saturate, those of scales below 2^-15 may
+ * lose bits).  scale bytes above 247, which mfa_kv8_append never writes, may stand for
+ * values that are not finite.
+ */
+typedef mfa_kv4_fwd_params mfa_kv8_fwd_params;
+int64_t mfa_kv8_fwd_workspace_bytes(const mfa_kv8_fwd_params* params);
+int mfa_kv8_fwd(const mfa_kv8_fwd_params* params, void* workspace, int64_t workspace_bytes, void* stream);
+int mfa_kv8_fwd_params_size(void);
+
+/*
+ * The attention weight that each cached key received: with the forward's parameters
+ * (cache.v, o and their strides unused; softmax_lse an input, what mfa_kv8_fwd wrote)
+ *   weight[j, hkv] = (j < Lk - Lq ? weight[j, hkv] : 0)
+ *                  + sum over query rows i and query heads h of hkv of exp(score_ihj - lse_ih)
+ * for the keys j < Lk of every sequence with queries, Lq of them: keys before the
+ * queries' own rows add to what they had, the queries' own start from 0.  What a row's
+ * mask leaves out, and rows whose lse is -inf, add nothing.  weights: fp32
+ * [num_pages, page_block_size, heads_kv] by element strides (row and head strides >= 0),
+ * addressed with the cache's block table; a page id outside the pool drops what is
+ * written.  Sums in fp32, in an order that sizes alone decide; every key has one
+ * owner.  One or two kernels; never synchronizes, never allocates.
+ */
+typedef struct mfa_kv8_weights_params {
+    mfa_kv8_fwd_params fwd;
+    float* weights;
+    int64_t weight_page_stride, weight_row_stride, weight_head_stride;
+} mfa_kv8_weights_params;
+int mfa_kv8_weights(const mfa_kv8_weights_params* params, void* stream);
+int mfa_kv8_weights_params_size(void);
+
+/*
+ * Eviction: of every head of a sequence with n > budget rows, the last min(recent,
+ * budget) rows and the heaviest of the others (by weights, ties to the lower row, NaN
+ * above everything), budget in all, move together in their order: they become rows 0 ..
+ * budget - 1, weights with them.  A block of 64 rows of a head whose rows all stay where
+ * they are is left as it is; any other gets a new scale byte by the rule of
+ * mfa_kv8_append for a block without rows, from the values that its rows have, and
+ * their codes are rounded by it (NaN stays NaN).  Rows from budget on keep their codes
+ * and weights.  n = min(cache_seqlens, max_seqlen_k, what the table can name), max_seqlen_k
+ * 0 leaving that bound out; new_seqlens [batch] (may be cache_seqlens itself) receives
+ * min(n, budget).  A row on a page id outside the pool reads as zeros with weight 0 and
+ * drops what is written.  budget and recent >= 0.  `workspace`: 256-byte aligned, at least
+ * mfa_kv8_evict_workspace_bytes bytes.  Three kernels; never synchronizes, never allocates.
+ */
+typedef struct mfa_kv8_evict_params {
+    mfa_kv8_cache cache;
+    float* weights;
+    int64_t weight_page_stride, weight_row_stride, weight_head_stride;
+    const int32_t* cache_seqlens;
+    int32_t* new_seqlens;
+    int32_t batch, heads_kv, head_dim, max_seqlen_k, budget, recent;
+} mfa_kv8_evict_params;
+int64_t mfa_kv8_evict_workspace_bytes(const mfa_kv8_evict_params* params);
+int mfa_kv8_evict(const mfa_kv8_evict_params* params, void* workspace, int64_t workspace_bytes, void* stream);
+int mfa_kv8_evict_params_size(void);
+
+/*
  * Pages copied inside pools: page src[i] to page dst[i] of every pool, i < pairs
  * (a forked sequence's last page, compaction).  No counterpart in the reference.
  * A pool is `page_bytes` contiguous bytes per page, `page_stride` bytes apart.

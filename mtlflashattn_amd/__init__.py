@@ -21,7 +21,9 @@ over disjoint key sets (context-parallel shards, cache + new tokens).
 Around the attention call: `qk_norm_rope` (RMS norm and rotation of the query
 and key heads in one pass, differentiable), and a paged K/V cache held in 4 bits
 (`kv4_cache`, `kv4_append`, `flash_attn_kv4_func`, `flash_attn_varlen_kv4_func`,
-`copy_cache_pages`).
+`copy_cache_pages`) or in 8 (`kv8_cache`, `kv8_append`, `flash_attn_kv8_func`,
+`flash_attn_varlen_kv8_func`), which can be kept to a budget of rows by the attention
+weight that its keys receive (`kv8_key_weights`, `kv8_evict`).
 
 Every call runs the gfx950 HIP kernels of libmtlfa_hip.so on the tensors'
 ROCm device; there is no CPU path.
@@ -36,6 +38,8 @@ from . import _kernel
 from ._kernel import MAX_HEAD_DIM, flash_attn_forward, forward_bshd, forward_varlen
 from ._version import __version__
 from .kv4 import copy_cache_pages, flash_attn_kv4_func, flash_attn_varlen_kv4_func, kv4_append, kv4_cache
+from .kv8 import (flash_attn_kv8_func, flash_attn_varlen_kv8_func, kv8_append, kv8_cache, kv8_evict,
+                  kv8_key_weights)
 from .norm_rope import qk_norm_rope
 
 __all__ = [
@@ -54,6 +58,12 @@ __all__ = [
     "kv4_append",
     "flash_attn_kv4_func",
     "flash_attn_varlen_kv4_func",
+    "kv8_cache",
+    "kv8_append",
+    "flash_attn_kv8_func",
+    "flash_attn_varlen_kv8_func",
+    "kv8_key_weights",
+    "kv8_evict",
     "copy_cache_pages",
     "__version__",
 ]

@@ -30,6 +30,11 @@ SRCS = [
     (os.path.join(PKG_DIR, "csrc", "mfa_kv4_attend.hip"), ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]),
     (os.path.join(PKG_DIR, "csrc", "mfa_kv4_tile.hip"), ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]),
     (os.path.join(PKG_DIR, "csrc", "mfa_pages.hip"), []),
+    (os.path.join(PKG_DIR, "csrc", "mfa_kv8.hip"), []),
+    (os.path.join(PKG_DIR, "csrc", "mfa_kv8_attend.hip"), ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]),
+    (os.path.join(PKG_DIR, "csrc", "mfa_kv8_tile.hip"), ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]),
+    (os.path.join(PKG_DIR, "csrc", "mfa_kv8_weights.hip"), ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]),
+    (os.path.join(PKG_DIR, "csrc", "mfa_kv8_evict.hip"), []),
 ]
 INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_DIR = os.path.join(PKG_DIR, "_lib")

@@ -151,6 +151,30 @@ class MfaKv4FwdParams(ctypes.Structure):
     ]
 
 
+MFA_KV8_BLOCK = 64
+
+
+class MfaKv8WeightsParams(ctypes.Structure):
+    """Mirror of `mfa_kv8_weights_params` (include/mfa.h)."""
+
+    _fields_ = [
+        ("fwd", MfaKv4FwdParams), ("weights", _c_ptr),
+        ("weight_page_stride", _c_i64), ("weight_row_stride", _c_i64), ("weight_head_stride", _c_i64),
+    ]
+
+
+class MfaKv8EvictParams(ctypes.Structure):
+    """Mirror of `mfa_kv8_evict_params` (include/mfa.h)."""
+
+    _fields_ = [
+        ("cache", MfaKv4Cache), ("weights", _c_ptr),
+        ("weight_page_stride", _c_i64), ("weight_row_stride", _c_i64), ("weight_head_stride", _c_i64),
+        ("cache_seqlens", _c_ptr), ("new_seqlens", _c_ptr),
+        ("batch", _c_i32), ("heads_kv", _c_i32), ("head_dim", _c_i32), ("max_seqlen_k", _c_i32), ("budget", _c_i32),
+        ("recent", _c_i32),
+    ]
+
+
 MFA_COPY_MAX_POOLS = 64
 
 
@@ -216,6 +240,10 @@ _SIMPLE_CALLS = (
     ("mfa_kv4_append", MfaKv4AppendParams, False),
     ("mfa_kv4_fwd", MfaKv4FwdParams, True),
     ("mfa_copy_pages", MfaCopyPagesParams, False),
+    ("mfa_kv8_append", MfaKv4AppendParams, False),
+    ("mfa_kv8_fwd", MfaKv4FwdParams, True),
+    ("mfa_kv8_weights", MfaKv8WeightsParams, False),
+    ("mfa_kv8_evict", MfaKv8EvictParams, True),
 )
 
 _lock = threading.Lock()
@@ -425,6 +453,30 @@ def kv4_fwd(params: MfaKv4FwdParams, workspace: int, workspace_bytes_: int, stre
 
 def copy_pages(params: MfaCopyPagesParams, stream: int) -> None:
     _checked("mfa_copy_pages", load().mfa_copy_pages(ctypes.byref(params), stream))
+
+
+def kv8_append(params: MfaKv4AppendParams, stream: int) -> None:
+    _checked("mfa_kv8_append", load().mfa_kv8_append(ctypes.byref(params), stream))
+
+
+def kv8_fwd_workspace_bytes(params: MfaKv4FwdParams) -> int:
+    return _checked("mfa_kv8_fwd_workspace_bytes", load().mfa_kv8_fwd_workspace_bytes(ctypes.byref(params)))
+
+
+def kv8_fwd(params: MfaKv4FwdParams, workspace: int, workspace_bytes_: int, stream: int) -> None:
+    _checked("mfa_kv8_fwd", load().mfa_kv8_fwd(ctypes.byref(params), workspace, workspace_bytes_, stream))
+
+
+def kv8_weights(params: MfaKv8WeightsParams, stream: int) -> None:
+    _checked("mfa_kv8_weights", load().mfa_kv8_weights(ctypes.byref(params), stream))
+
+
+def kv8_evict_workspace_bytes(params: MfaKv8EvictParams) -> int:
+    return _checked("mfa_kv8_evict_workspace_bytes", load().mfa_kv8_evict_workspace_bytes(ctypes.byref(params)))
+
+
+def kv8_evict(params: MfaKv8EvictParams, workspace: int, workspace_bytes_: int, stream: int) -> None:
+    _checked("mfa_kv8_evict", load().mfa_kv8_evict(ctypes.byref(params), workspace, workspace_bytes_, stream))
 
 
 def launch_info(params: MfaFwdParams) -> MfaLaunchInfo:

@@ -1,6 +1,6 @@
-// mfa_kv4_attend.h -- what the kernels of attention over the paged 4-bit cache
-// (mfa_kv4_attend.hip, mfa_kv4_tile.hip) share: arguments, the dealing of work
-// over workgroups, pages and result rows.
+// mfa_kv4_attend.h -- what the kernels of attention over paged quantised caches
+// (mfa_kv_rows.h, mfa_kv_tile.h; 4 and 8 bits) share: arguments, the dealing of work
+// over workgroups, pages, result rows, and the host's plan.
 #pragma once
 
 #include "mfa_kv4.h"
@@ -223,10 +223,11 @@ struct Walk4 {
 
 // A wavefront's way through the pages of a unit: the buffer resources of the
 // current page of K's codes and scales and V's, which end with the sequence
-// (rows behind it, and any row of a page id outside the pool, read as zeros).
+// (rows behind it, and any row of a page id outside the pool, read as zeros).  F:
+// the bytes of resource x that a row has, and the rows that share them.
 // The id of the page that is expected next is loaded ahead, by the scalar unit: a
 // vector load of it would have to wait for all the codes on their way.
-template <int DP>
+template <class F>
 struct Pages4 {
     typedef const __attribute__((address_space(4))) int32_t* ids_t;
     __amdgpu_buffer_rsrc_t rs[4];
@@ -270,9 +271,10 @@ struct Pages4 {
             const int rows = min(Lk - row0, (int)by_page.d);
             const bool ok = (uint32_t)id < (uint32_t)npages && rows > 0;
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
+            for (int x = 0; x < 4; ++x) {
                 rs[x] = __builtin_amdgcn_make_buffer_rsrc((void*)(base[x] + (ok ? id : 0) * ps[x]), (short)0,
-                                                          ok ? (rows - 1) * rstride[x] + (x & 1 ? DP / 32 : DP / 2) : 0, kBufferDword3);
+                                                          ok ? (rows - 1) / F::rows_per(x) * rstride[x] + F::bytes(x) : 0, kBufferDword3);
+            }
         }
         return j - row0;
     }
@@ -304,6 +306,23 @@ __device__ __forceinline__ void store_lse4(K4Const& a, int b, int q0, int i, int
 
 }  // namespace
 
-// 128-column tiles (mfa_kv4_tile.hip): void(*)(K4Args)
-__attribute__((visibility("hidden"))) void* mfa_kv4_tile_kernel_of(int dp, bool bf16, bool bias);
 constexpr int kTileCols4 = 128;
+
+// A cache format as the host's plan and launches see it.
+struct MfaKvFormat {
+    const char* who;                                // the entry point, for messages
+    int rows_wgs[2];                                // workgroups per CU of the kernels of 16 and 32 columns
+    int tile_wgs;                                   // ... of 128
+    void* (*rows_kernel)(int dp, int cols, bool bf16);   // void(*)(K4Args), for 16 or 32 columns
+    void* (*tile_kernel)(int dp, bool bf16, bool bias);  // ... for 128
+};
+// mfa_kv4_attend.hip; the parameters mean what include/mfa.h says of mfa_kv4_fwd.
+// mfa_kv_args: checks them and fills K4Args with what does not depend on how the work
+// is dealt; rows_q stays 0 where there is nothing to do.
+__attribute__((visibility("hidden"))) int mfa_kv_args(const mfa_kv4_fwd_params* p, const char* who, void* args);
+__attribute__((visibility("hidden"))) int64_t mfa_kv_fwd_workspace_bytes(const mfa_kv4_fwd_params* p, const MfaKvFormat& f);
+__attribute__((visibility("hidden"))) int mfa_kv_fwd(const mfa_kv4_fwd_params* p, const MfaKvFormat& f, void* workspace,
+                                                     int64_t workspace_bytes, void* stream);
+// mfa_kv4_tile.hip, mfa_kv8_tile.hip
+__attribute__((visibility("hidden"))) void* mfa_kv4_tile_kernel_of(int dp, bool bf16, bool bias);
+__attribute__((visibility("hidden"))) void* mfa_kv8_tile_kernel_of(int dp, bool bf16, bool bias);

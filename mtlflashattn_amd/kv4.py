@@ -1,5 +1,5 @@
 """A paged K/V cache held in 4 bits: writing it, attention over it, and copies of
-its pages.  The reference has no cache (block_table raises,
+its pages; and what the 8-bit cache (kv8.py) shares with it.  The reference has no cache (block_table raises,
 metal_flash_attn/__init__.py:130-131); here 16-bit pages are read by
 flash_attn_varlen_func and 4-bit pages, 17/64 of their size, by the functions of
 this module.
@@ -31,11 +31,24 @@ def _remember(key, plan):
     return plan
 
 
-def _not_tensors(k_cache, v_cache):
+class _Format:
+    """A cache format: what its calls check, and their library entries."""
+
+    def __init__(self, bits, code_dtype, code_bytes, scale_shape):
+        self.bits, self.name = bits, f"kv{bits}"
+        self.code_dtype = code_dtype
+        self.code_bytes = code_bytes    # (head_dim): codes of a row and head
+        self.scale_shape = scale_shape  # (pages, page, heads, head_dim): of the scales
+
+
+_KV4 = _Format(4, torch.uint8, lambda D: D // 2, lambda pages, page, heads, D: (pages, page, heads, D // 32))
+
+
+def _not_tensors(k_cache, v_cache, fmt=_KV4):
     """The error for arguments of which no signature can be formed."""
     for what, c in (("k_cache", k_cache), ("v_cache", v_cache)):
         if not isinstance(c, (tuple, list)) or len(c) != 2 or not (torch.is_tensor(c[0]) and torch.is_tensor(c[1])):
-            return ValueError(f"mtlflashattn_amd: {what} must be a pair (codes, scales), as kv4_cache makes it")
+            return ValueError(f"mtlflashattn_amd: {what} must be a pair (codes, scales), as {fmt.name}_cache makes it")
     return ValueError("mtlflashattn_amd: tensors expected")
 
 
@@ -48,28 +61,36 @@ def kv4_cache(num_pages, page_block_size, num_heads_kv, head_dim, device="cuda")
     kernels read fastest; they take any other order too.  page_block_size: a
     multiple of 64; head_dim: 32, 64, 96 or 128.
     """
-    if page_block_size <= 0 or page_block_size % 64:
-        raise ValueError(f"mtlflashattn_amd: page_block_size {page_block_size} must be a positive multiple of 64")
-    if head_dim <= 0 or head_dim % 32 or head_dim > MAX_HEAD_DIM:
-        raise NotImplementedError(f"mtlflashattn_amd: head_dim {head_dim} of a 4-bit cache must be 32, 64, 96 or 128")
+    _check_page_and_head(page_block_size, head_dim, _KV4)
     return tuple(torch.zeros(num_pages, num_heads_kv, page_block_size, n, dtype=torch.uint8, device=device).transpose(1, 2)
                  for n in (head_dim // 2, head_dim // 32))
 
 
-def _check_cache(cache, D, Hkv, device, what):
+def _check_page_and_head(page, D, fmt):
+    if page <= 0 or page % 64:
+        raise ValueError(f"mtlflashattn_amd: page_block_size {page} must be a positive multiple of 64")
+    if D <= 0 or D % 32 or D > MAX_HEAD_DIM:
+        raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} of a {fmt.bits}-bit cache must be 32, 64, 96 or 128")
+
+
+def _check_cache(cache, D, Hkv, device, what, fmt=_KV4):
     codes, scales = cache
-    if codes.dim() != 4 or scales.dim() != 4 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
-        raise ValueError(f"mtlflashattn_amd: {what}: codes and scales must be 4-D uint8 tensors")
+    dims = len(fmt.scale_shape(0, 64, 0, 32))
+    if codes.dim() != 4 or scales.dim() != dims or codes.dtype != fmt.code_dtype or scales.dtype != torch.uint8:
+        name = str(fmt.code_dtype).replace("torch.", "")
+        raise ValueError(f"mtlflashattn_amd: {what}: codes and scales must be " + (
+            "4-D uint8 tensors" if name == "uint8" else f"a 4-D {name} and a {dims}-D uint8 tensor"))
     page = codes.shape[1]
     if page == 0 or page % 64:
         raise ValueError(f"mtlflashattn_amd: page_block_size {page} must be a positive multiple of 64")
-    if tuple(codes.shape[2:]) != (Hkv, D // 2) or tuple(scales.shape) != (*codes.shape[:3], D // 32):
+    if (tuple(codes.shape[2:]) != (Hkv, fmt.code_bytes(D))
+            or tuple(scales.shape) != fmt.scale_shape(codes.shape[0], page, Hkv, D)):
         raise ValueError(f"mtlflashattn_amd: {what}: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not "
                          f"hold {Hkv} heads of {D} elements")
-    for t, unit in ((codes, 16), (scales, 1)):
+    for t, unit, last in ((codes, 16, True), (scales, 1, dims == 4)):
         if t.device != device:
             raise ValueError(f"mtlflashattn_amd: tensors on different devices ({device} vs {t.device})")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
+        if last and t.shape[-1] > 1 and t.stride(-1) != 1:
             raise ValueError(f"mtlflashattn_amd: {what}: the last dimension must be contiguous")
         if any(s % unit for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1):
             raise ValueError(f"mtlflashattn_amd: {what}: code strides must be multiples of 16 bytes")
@@ -157,21 +178,26 @@ def kv4_append(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, r
     back from the cache (flash_attn_varlen_func(q, k', v', ...)).  Not
     differentiable: inputs that require grad raise.
     """
+    return _append(_KV4, k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, return_values)
+
+
+def _append(fmt, k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, return_values):
     try:
         (kc, ks), (vc, vs) = k_cache, v_cache
-        key = ("append", k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
+        key = ("append", fmt, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
                kc.shape, kc.stride(), kc.dtype, kc.device, ks.shape, ks.stride(), ks.dtype, ks.device,
                vc.shape, vc.stride(), vc.dtype, vc.device, vs.shape, vs.stride(), vs.dtype, vs.device,
                cu_seqlens.shape, cu_seqlens.stride(), cu_seqlens.dtype, cu_seqlens.device,
                cache_seqlens.shape, cache_seqlens.stride(), cache_seqlens.dtype, cache_seqlens.device,
                block_table.shape, block_table.stride(), block_table.dtype, block_table.device)
     except (AttributeError, TypeError, ValueError):
-        raise _not_tensors(k_cache, v_cache) from None
+        raise _not_tensors(k_cache, v_cache, fmt) from None
     _kernel._check_no_tangent(k, v)
     if _kernel._needs_grad(k, v):
-        raise NotImplementedError("mtlflashattn_amd: kv4_append is not differentiable; run it under torch.no_grad() or on "
-                                  "detached rows")
-    plan = _plans.get(key) or _remember(key, _append_plan(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table))
+        raise NotImplementedError(f"mtlflashattn_amd: {fmt.name}_append is not differentiable; run it under "
+                                  "torch.no_grad() or on detached rows")
+    plan = _plans.get(key) or _remember(key, _append_plan(fmt, k, v, k_cache, v_cache, cu_seqlens, cache_seqlens,
+                                                          block_table))
     template, direct = plan
     p = _hip.MfaKv4AppendParams.from_buffer_copy(template)
     kp, vp = k.data_ptr(), v.data_ptr()
@@ -189,17 +215,23 @@ def kv4_append(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, r
     if return_values:
         values = tuple(torch.empty_like(t, memory_format=torch.contiguous_format) for t in (k, v))
         p.k_values, p.v_values = values[0].data_ptr(), values[1].data_ptr()
-    _kernel._launch_on(k.device, _hip.kv4_append, p)
+    _kernel._launch_on(k.device, _hip.kv4_append if fmt is _KV4 else _hip.kv8_append, p)
     _written((kc, ks, vc, vs))
     return values
+
+
+def _check_written(*pools):
+    for c in pools:
+        if any(s == 0 for s, n in zip(c.stride()[:3], c.shape[:3]) if n > 1):
+            raise ValueError("mtlflashattn_amd: an expanded cache (rows that share memory) cannot be written")
 
 
 def _token_strides(x):
     return tuple(s if n > 1 else 0 for s, n in zip(x.stride()[:2], x.shape[:2]))
 
 
-def _append_plan(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table):
-    """(parameters without data pointers, whether the tensors are used in place) of a kv4_append call."""
+def _append_plan(fmt, k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table):
+    """(parameters without data pointers, whether the tensors are used in place) of an append."""
     if k.dim() != 3 or v.dim() != 3 or k.shape != v.shape:
         raise ValueError(f"mtlflashattn_amd: expected k and v [total,H,D], got {tuple(k.shape)} and {tuple(v.shape)}")
     _kernel._check_device(k, v)
@@ -207,18 +239,16 @@ def _append_plan(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table)
         raise NotImplementedError(f"mtlflashattn_amd: dtype {k.dtype} (k/v must match, fp16/bf16/fp32)")
     total, Hkv, D = k.shape
     if D == 0 or D % 32 or D > MAX_HEAD_DIM:
-        raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} of a 4-bit cache must be 32, 64, 96 or 128")
-    _check_cache(k_cache, D, Hkv, k.device, "k_cache")
-    _check_cache(v_cache, D, Hkv, k.device, "v_cache")
+        raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} of a {fmt.bits}-bit cache must be 32, 64, 96 or 128")
+    _check_cache(k_cache, D, Hkv, k.device, "k_cache", fmt)
+    _check_cache(v_cache, D, Hkv, k.device, "v_cache", fmt)
     if k_cache[0].shape != v_cache[0].shape:
         raise ValueError("mtlflashattn_amd: k_cache and v_cache differ in pages")
     batch = cache_seqlens.shape[0] if cache_seqlens.dim() == 1 else 0
     _check_ints(cache_seqlens, batch, k.device, "cache_seqlens")
     _check_ints(cu_seqlens, batch + 1, k.device, "cu_seqlens")
     _check_table(block_table, batch, k.device)
-    for c in (*k_cache, *v_cache):
-        if any(s == 0 for s, n in zip(c.stride()[:3], c.shape[:3]) if n > 1):
-            raise ValueError("mtlflashattn_amd: an expanded cache (rows that share memory) cannot be written")
+    _check_written(*k_cache, *v_cache)
     _kernel._check_sizes(total, Hkv, batch)
     p = _hip.MfaKv4AppendParams()
     _cache_struct(p.cache, k_cache, v_cache, block_table)
@@ -257,7 +287,7 @@ def flash_attn_kv4_func(q, k_cache, v_cache, cache_seqlens, block_table, softmax
     """
     if torch.is_tensor(q) and q.dim() != 4:
         raise ValueError(f"mtlflashattn_amd: expected q [B,Lq,H,D], got {q.dim()}-D")
-    return _attend(q, k_cache, v_cache, None, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap,
+    return _attend(_KV4, q, k_cache, v_cache, None, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap,
                    alibi_slopes, max_seqlen_k, return_softmax_lse)
 
 
@@ -277,23 +307,27 @@ def flash_attn_varlen_kv4_func(q, k_cache, v_cache, cu_seqlens_q, cache_seqlens,
     """
     if torch.is_tensor(q) and q.dim() != 3:
         raise ValueError(f"mtlflashattn_amd: expected q [total,H,D], got {q.dim()}-D")
-    return _attend(q, k_cache, v_cache, cu_seqlens_q, cache_seqlens, block_table, softmax_scale, causal, window_size,
+    return _attend(_KV4, q, k_cache, v_cache, cu_seqlens_q, cache_seqlens, block_table, softmax_scale, causal, window_size,
                    softcap, alibi_slopes, max_seqlen_k, return_softmax_lse)
 
 
-def _attend(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap, alibi_slopes,
-            max_seqlen_k, return_lse):
+def _numbers(softmax_scale, window_size, softcap, alibi_slopes, max_seqlen_k):
+    """The options as numbers, so that a signature holds a value whatever type it came in."""
     _kernel._check_options(window_size, softcap, alibi_slopes)
-    # (numbers, so that the signature holds a value whatever type it came in)
-    softmax_scale = None if softmax_scale is None else float(softmax_scale)
-    # (a window as wide as a 32-bit number is as good as none)
-    most = _kernel._INT32_MAX
-    softcap, window_size = float(softcap), (min(int(window_size[0]), most), min(int(window_size[1]), most))
-    max_seqlen_k = None if max_seqlen_k is None else int(max_seqlen_k)
+    most = _kernel._INT32_MAX  # (a window as wide as a 32-bit number is as good as none)
+    return (None if softmax_scale is None else float(softmax_scale),
+            (min(int(window_size[0]), most), min(int(window_size[1]), most)), float(softcap),
+            None if max_seqlen_k is None else int(max_seqlen_k))
+
+
+def _attend(fmt, q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap,
+            alibi_slopes, max_seqlen_k, return_lse):
+    softmax_scale, window_size, softcap, max_seqlen_k = _numbers(softmax_scale, window_size, softcap, alibi_slopes,
+                                                                 max_seqlen_k)
     try:
         (kc, ks), (vc, vs) = k_cache, v_cache
         varlen = q.dim() == 3
-        key = (q.shape, q.stride(), q.dtype, q.device, kc.shape, kc.stride(), kc.dtype, kc.device,
+        key = (fmt, q.shape, q.stride(), q.dtype, q.device, kc.shape, kc.stride(), kc.dtype, kc.device,
                ks.shape, ks.stride(), ks.dtype, ks.device, vc.shape, vc.stride(), vc.dtype, vc.device,
                vs.shape, vs.stride(), vs.dtype, vs.device,
                cache_seqlens.shape, cache_seqlens.stride(), cache_seqlens.dtype, cache_seqlens.device,
@@ -302,17 +336,17 @@ def _attend(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale
                alibi_slopes is not None and (alibi_slopes.shape, alibi_slopes.device),
                softmax_scale, bool(causal), window_size, softcap, max_seqlen_k)
     except (AttributeError, TypeError, ValueError):
-        raise _not_tensors(k_cache, v_cache) from None
+        raise _not_tensors(k_cache, v_cache, fmt) from None
     _kernel._check_no_tangent(q)
     if q.requires_grad and torch.is_grad_enabled():
-        raise NotImplementedError("mtlflashattn_amd: attention over a 4-bit cache is forward-only; run it under "
+        raise NotImplementedError(f"mtlflashattn_amd: attention over a {fmt.bits}-bit cache is forward-only; run it under "
                                   "torch.no_grad() or without inputs that require grad")
     plan = _plans.get(key) or _remember(key, _attend_plan(
-        q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap, alibi_slopes,
+        fmt, q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap, alibi_slopes,
         max_seqlen_k))
     template, nbytes, direct = plan
     if _kernel._trace_enabled():
-        _kernel._record_trace(q.dtype, q.shape[-1], q.shape[0 if varlen else 1], template.max_seqlen_k, causal, "hip-kv4")
+        _kernel._record_trace(q.dtype, q.shape[-1], q.shape[0 if varlen else 1], template.max_seqlen_k, causal, "hip-" + fmt.name)
     p = _hip.MfaKv4FwdParams.from_buffer_copy(template)
     device, qp = q.device, q.data_ptr()
     if not direct or qp & 15:
@@ -337,23 +371,23 @@ def _attend(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale
     p.q, p.o, p.cache_seqlens = qp, out.data_ptr(), cache_seqlens.data_ptr()
     _cache_pointers(p.cache, kc, ks, vc, vs, block_table)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    _kernel._launch_on(device, _hip.kv4_fwd, p, None if ws is None else ws.data_ptr(), nbytes)
+    _kernel._launch_on(device, _hip.kv4_fwd if fmt is _KV4 else _hip.kv8_fwd, p, None if ws is None else ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 
 
-def _attend_plan(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap,
-                 alibi_slopes, max_seqlen_k):
-    """(parameters without data pointers, workspace bytes, whether the tensors are used in place) of a call."""
+def _attend_params(fmt, q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap,
+                   alibi_slopes, max_seqlen_k):
+    """The parameters of a call without data pointers."""
     varlen = q.dim() == 3
     _kernel._check_device(q)
     if q.dtype not in _ATTEND_DTYPES:
-        raise NotImplementedError(f"mtlflashattn_amd: dtype {q.dtype} (queries over a 4-bit cache are fp16 or bf16)")
+        raise NotImplementedError(f"mtlflashattn_amd: dtype {q.dtype} (queries over a {fmt.bits}-bit cache are fp16 or bf16)")
     Hq, D = q.shape[-2:]
     if D not in (32, 64, 96, 128):
-        raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} of a 4-bit cache must be 32, 64, 96 or 128")
+        raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} of a {fmt.bits}-bit cache must be 32, 64, 96 or 128")
     Hkv = k_cache[0].shape[2] if k_cache[0].dim() == 4 else 0
-    _check_cache(k_cache, D, Hkv, q.device, "k_cache")
-    _check_cache(v_cache, D, Hkv, q.device, "v_cache")
+    _check_cache(k_cache, D, Hkv, q.device, "k_cache", fmt)
+    _check_cache(v_cache, D, Hkv, q.device, "v_cache", fmt)
     if k_cache[0].shape != v_cache[0].shape:
         raise ValueError("mtlflashattn_amd: k_cache and v_cache differ in pages or heads")
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
@@ -392,16 +426,28 @@ def _attend_plan(q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_
     p.window_left, p.window_right = window_size
     p.causal = int(bool(causal))
     p.dtype = _hip.DTYPE_CODES[q.dtype]
+    return p
+
+
+def _attend_direct(q, cu_q, cache_seqlens):
+    """Whether a call takes the tensors in place."""
+    return (_kernel._fits_strides(q) and _i32(cache_seqlens) is cache_seqlens and (q.dim() != 3 or _i32(cu_q) is cu_q))
+
+
+def _attend_plan(fmt, q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale, causal, window_size, softcap,
+                 alibi_slopes, max_seqlen_k):
+    """(parameters without data pointers, workspace bytes, whether the tensors are used in place) of a call."""
+    p = _attend_params(fmt, q, k_cache, v_cache, cu_q, cache_seqlens, block_table, softmax_scale, causal, window_size,
+                       softcap, alibi_slopes, max_seqlen_k)
     # placeholders: sizing the workspace reads no tensor
     sized = _hip.MfaKv4FwdParams.from_buffer_copy(p)
     sized.q = sized.o = sized.cache_seqlens = sized.cache.block_table = 256
     sized.cache.k.codes = sized.cache.k.scales = sized.cache.v.codes = sized.cache.v.scales = 256
-    sized.cu_seqlens_q = 256 if varlen else None
+    sized.cu_seqlens_q = 256 if q.dim() == 3 else None
     sized.q_batch_stride = sized.q_seq_stride = sized.q_head_stride = 0
     with _kernel._on(q.device):
-        nbytes = _hip.kv4_fwd_workspace_bytes(sized)
-    return p, nbytes, (_kernel._fits_strides(q) and _i32(cache_seqlens) is cache_seqlens
-                       and (not varlen or _i32(cu_q) is cu_q))
+        nbytes = (_hip.kv4_fwd_workspace_bytes if fmt is _KV4 else _hip.kv8_fwd_workspace_bytes)(sized)
+    return p, nbytes, _attend_direct(q, cu_q, cache_seqlens)
 
 
 def copy_cache_pages(pools, src, dst):
