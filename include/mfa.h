@@ -493,7 +493,8 @@ typedef mfa_kv4_cache mfa_kv8_cache;
  * of the rows that are written into it; where the block holds rows of the sequence
  * already (cache_seqlens is no multiple of 64), at least the byte that it had, and if
  * the byte rises the codes of those rows are rounded again.  Elements are rounded to
- * the nearest code, ties to the even one; infinities and NaN become NaN.  What stands
+ * the nearest code, ties to the even one (elements beyond 240 * 2^120, which would round
+ * to 2^128, to that); infinities and NaN become NaN.  What stands
  * in a block behind the last row may change its value with the byte.  No two sequences
  * may write into one block.  A negative length counts as 0.  Values of tokens of no
  * sequence are 0; values of rows that are dropped are those of a block that holds
@@ -509,8 +510,8 @@ int mfa_kv8_append_params_size(void);
  * V reaches only the rows whose mask holds its key.  K is exact; V is exact with bf16
  * queries and for at most 32 columns; on the tiles of 128 columns fp16 queries take V
  * rounded to fp16 (elements beyond +/-65504 saturate, those of scales below 2^-15 may
- * lose bits).  scale bytes above 247, which mfa_kv8_append never writes, may stand for
- * values that are not finite.
+ * lose bits).  Codes above 240 with scale bytes from 247 on, which mfa_kv8_append never writes, may
+ * stand for values that are not finite.
  */
 typedef mfa_kv4_fwd_params mfa_kv8_fwd_params;
 int64_t mfa_kv8_fwd_workspace_bytes(const mfa_kv8_fwd_params* params);

@@ -313,6 +313,7 @@ struct MfaKvFormat {
     const char* who;                                // the entry point, for messages
     int rows_wgs[2];                                // workgroups per CU of the kernels of 16 and 32 columns
     int tile_wgs;                                   // ... of 128
+    float least_scale;                              // softmax scales up to here take the path that scales before it masks
     void* (*rows_kernel)(int dp, int cols, bool bf16);   // void(*)(K4Args), for 16 or 32 columns
     void* (*tile_kernel)(int dp, bool bf16, bool bias);  // ... for 128
 };

@@ -365,6 +365,7 @@ int k4_plan(const mfa_kv4_fwd_params* p, const MfaKvFormat& f, K4Plan* plan, int
     const bool varlen = p->cu_seqlens_q != nullptr;
     const int64_t rows = a.rows_q;
     const int D = p->head_dim;
+    a.bias |= !(p->scale > f.least_scale);
 
     // Columns per workgroup: a sequence's, at most 128.  The sequences of a
     // varlen call are known on the device only: one launch takes those of at most
@@ -411,7 +412,7 @@ void* rows_kernel4(int dp, int cols, bool bf16) {
         default: return rows4<128>(cols, bf16);
     }
 }
-const MfaKvFormat kFormat4 = {"mfa_kv4_fwd", {wgs4(1), wgs4(2)}, 2, rows_kernel4, mfa_kv4_tile_kernel_of};
+const MfaKvFormat kFormat4 = {"mfa_kv4_fwd", {wgs4(1), wgs4(2)}, 2, 0.f, rows_kernel4, mfa_kv4_tile_kernel_of};
 
 }  // namespace
 

@@ -17,9 +17,15 @@
 namespace {
 
 constexpr int kKv8Block = MFA_KV8_BLOCK;  // rows per scale
-constexpr float kKv8Top = 448.f;
 
 __device__ __forceinline__ float kv8_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// K's scale as a factor of scores in log2 units before their mask is applied: not below
+// 2^-60, as a factor of 0 (byte 0, which a page outside the pool reads as) times a masked
+// score, -inf, would be NaN.  Scores of smaller scales are 0 to fp32 sums either way
+// (products of |q| < 2^24 with codes stay below 2^-20).
+constexpr float kKv8LeastScale = 0x1p-60f;
+__device__ __forceinline__ float kv8_k_scale(uint32_t byte) { return fmaxf(kv8_scale(byte), kKv8LeastScale); }
 
 // Eight codes (two dwords) as eight bf16: exact while code * s is a normal bf16.
 __device__ __forceinline__ u32x4_t kv8_bf16x8(uint32_t w0, uint32_t w1, float s) {
@@ -74,6 +80,9 @@ __device__ __forceinline__ uint32_t kv8_byte_of(uint32_t max_bits) {
     const int b = (int)(max_bits >> 23) - 8 + ((max_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
     return (uint32_t)max(b, 1);
 }
+// The largest value to write under a byte: 448, or 240 under the largest byte there is
+// (scale 2^120), where 256 would stand for 2^128.
+__device__ __forceinline__ float kv8_top(uint32_t byte) { return byte < 247 ? 448.f : 240.f; }
 // 2^(127 - byte), for bytes 1 .. 253
 __device__ __forceinline__ float kv8_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 

@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kAThreads) mfa_kv8_append_kernel(A8Args a) {
 #pragma unroll
     for (int w = 0; w < kAThreads / 64; ++w) mx = max(mx, max_s[w]);
     const uint32_t byte = max(kv8_byte_of(mx), old);
-    const float inv = kv8_inverse(byte), sc = kv8_scale(byte);
+    const float inv = kv8_inverse(byte), sc = kv8_scale(byte), top = kv8_top(byte);
 
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kAThreads) mfa_kv8_append_kernel(A8Args a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float z = x[i].at(e);
-            y[e] = (__float_as_uint(z) & 0x7fffffffu) < 0x7f800000u ? z * inv : __builtin_nanf("");
+            y[e] = (__float_as_uint(z) & 0x7fffffffu) < 0x7f800000u ? __builtin_amdgcn_fmed3f(z * inv, -top, top) : __builtin_nanf("");
         }
         const u32x2_t c = {kv8_round4(y[0], y[1], y[2], y[3]), kv8_round4(y[4], y[5], y[6], y[7])};
         if (codes) *reinterpret_cast<u32x2_t*>(codes + (int64_t)(lo + r) * p.cr + d) = c;

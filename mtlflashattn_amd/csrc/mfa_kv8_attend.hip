@@ -121,7 +121,7 @@ void* rows_kernel8(int dp, int cols, bool bf16) {
         default: return rows8<128>(cols, bf16);
     }
 }
-const MfaKvFormat kFormat8 = {"mfa_kv8_fwd", {wgs4(1), wgs4(2)}, 2, rows_kernel8, mfa_kv8_tile_kernel_of};
+const MfaKvFormat kFormat8 = {"mfa_kv8_fwd", {wgs4(1), wgs4(2)}, 2, kKv8LeastScale, rows_kernel8, mfa_kv8_tile_kernel_of};
 
 }  // namespace
 

@@ -55,7 +55,7 @@ struct KeyBlock8 {
         return s < 2 * P ? kv8_operand<Op>(k[kk][s >> 1][2 * (s & 1)], k[kk][s >> 1][2 * (s & 1) + 1]) : kv8_operand<Op>(kh[kk][0], kh[kk][1]);
     }
     // what the scores of the block are still to be multiplied by
-    __device__ __forceinline__ float k_scale() const { return kv8_scale(ks); }
+    __device__ __forceinline__ float k_scale() const { return kv8_k_scale(ks); }
 };
 
 }  // namespace

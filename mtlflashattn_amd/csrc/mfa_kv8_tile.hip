@@ -59,7 +59,7 @@ struct Stage8 {
         uint16_t bits[CHUNKS];
     };
     __device__ __forceinline__ void write(uint16_t* tile, Nans& nans, bool part, int half_, int tid) {
-        if (half_ == 0) sk = kv8_scale(ks);
+        if (half_ == 0) sk = kv8_k_scale(ks);
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
             if (i % 2 != half_) continue;

@@ -48,7 +48,8 @@ def kv8_append(k, v, k_cache, v_cache, cu_seqlens, cache_seqlens, block_table, r
 
     A block takes the smallest power of two from 2^-126 on that leaves the largest
     finite magnitude of its rows within 448 times it; elements are rounded to the
-    nearest e4m3 value, ties to the even code; infinities and NaN become NaN.  Rows that
+    nearest e4m3 value, ties to the even code (beyond 240 * 2^120 to that: the next would
+    be infinite in bf16 and fp32); infinities and NaN become NaN.  Rows that
     a block holds already never lower its scale; where new ones raise it, the codes of
     the held rows are rounded again (exact but for the smallest ones).
 
