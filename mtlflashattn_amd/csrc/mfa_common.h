@@ -160,6 +160,12 @@ __device__ __forceinline__ void lds_load16(uint64_t base, uint32_t bytes, uint16
                      : "memory");
 }
 
+// The same from a 64-bit address per lane (global_load_lds_dwordx4).
+__device__ __forceinline__ void lds_load16(const void* src, uint16_t* dst) {
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)dst;
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "{m0}"(lds) : "memory");
+}
+
 // at most N of this wavefront's vector memory operations are still in flight
 template <int N>
 __device__ __forceinline__ void wait_vm() {

@@ -111,22 +111,27 @@ __device__ __forceinline__ Seq4 lane_seq4(const Seq4& s, int l) {
                 __builtin_amdgcn_readlane(s.tiles, l), __builtin_amdgcn_readlane(s.chunks, l)};
 }
 
-// inclusive prefix sum over the wavefront
+// inclusive prefix sum over the wavefront: shifts inside rows of 16 lanes, then the
+// last lanes of rows and of halves to what is behind them
 __device__ __forceinline__ int scan64(int x) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
     return x;
 }
 
 // The items of the call are laid end to end, sequence by sequence (a sequence's:
 // K/V head by K/V head, tile by tile, chunk by chunk); of C items workgroup w
 // takes w C / G to (w + 1) C / G.
-__device__ __forceinline__ int first_item(int w, int C, int G) { return (int)((int64_t)w * C / G); }
-__device__ __forceinline__ int wg_of_item(int x, int C, int G) { return (int)((((int64_t)x + 1) * G - 1) / C); }
+// (Divided in double, a tenth of the code of a 64-bit integer division: numerator and
+// divisor are exact, and a quotient below 2^31 that is no integer is at least 1 / divisor,
+// far more than a rounding, away from the next one: divisors stay below 2^21, or are C
+// with quotients below 2^21.)
+__device__ __forceinline__ int first_item(int w, int C, int G) { return (int)((double)w * C / G); }
+__device__ __forceinline__ int wg_of_item(int x, int C, int G) { return (int)((((double)x + 1) * G - 1) / C); }
 
 // A workgroup's walk over its items.
 struct Walk4 {

@@ -15,9 +15,12 @@
 //    at head dim 128).  A wavefront takes every fourth 32-key block, the next one on
 //    its way into registers;
 //  * more: bound by the exponentials (24 cycles of a SIMD per 64 scores, against 16 of
-//    the products at head dim 128).  A wavefront holds 64 keys as operands and goes
-//    over the columns, 32 at a time; two wavefronts share the keys and two the columns,
-//    64 of which stand in LDS while the next 64 are loaded.
+//    the products at head dim 128).  A wavefront holds 32 keys as operands and goes over
+//    the columns, 128 of which stand in LDS while the next are loaded straight into it;
+//    eight wavefronts share them.  64 rows over two prompts of 12000 to 16384 keys, Hq=32
+//    Hkv=8 D=128: 32 us, of which about 10 pass before the first product (the dealing,
+//    the page, the first queries and keys); 46 us with the pieces of two XCDs on the other
+//    six, 54 with eight-way unrolled loads (their code costs more to fetch than to run).
 #include <math.h>
 #include <stdarg.h>
 #include <stdint.h>
@@ -65,7 +68,10 @@ __device__ __forceinline__ ScoreOf score_of(K4Const& a) {
     return ScoreOf{a.scale, a.scale_log2, a.softcap, a.bias != 0, a.alibi != nullptr};
 }
 
-constexpr int kFewWgs = 4;
+// (32 sequences of 512 to 8192 keys, Hq=32 Hkv=8 D=128 bf16: 35.3 us with three
+// workgroups per CU, 35.5 with five, 51 with six, which spill; two blocks ahead instead
+// of one: 35.7.  Of that about 11 us pass before the stream runs and after it ends.)
+constexpr int kFewWgs = 3;
 template <int DP, bool IS_BF16>
 __global__ void __launch_bounds__(kThreads4) __attribute__((amdgpu_waves_per_eu(kFewWgs)))
 mfa_kv8_weights_few_kernel(K4Args) {
@@ -179,169 +185,215 @@ mfa_kv8_weights_few_kernel(K4Args) {
     }
 }
 
-constexpr int kWCols = 64;     // columns in LDS
-constexpr int kManyWgs = 2;
+constexpr int kManyWgs = 2, kManyThreads = 512;  // (workgroups per CU: what their LDS leaves room for)
+
+// A workgroup's piece of the work: consecutive chunks of one unit (a sequence and K/V
+// head).  The units' chunks are cut into pieces of at most ceil(chunks of all units /
+// G), the same for all of a unit to one chunk, so that no workgroup pays the latency
+// of a second unit's queries and pages.
+struct Piece4 {
+    int b, hkv, c0, nch;
+    Seq4 sq;
+    // pieces of at most `most` chunks of a sequence
+    static __device__ __forceinline__ int pieces(const Seq4& s, int most) { return (s.chunks + most - 1) / most; }
+    __device__ __forceinline__ bool find(K4Const& a) {
+        const int lane = threadIdx.x & 63, B = a.B, H = a.Hkv;
+        auto seq = [&](int b0) { return b0 + lane < B ? seq4(a, b0 + lane) : Seq4{0, 0, 0, 0, 1}; };
+        Seq4 s = seq(0);
+        int all = __builtin_amdgcn_readlane(scan64(s.items(H)), 63);
+        for (int b0 = 64; b0 < B; b0 += 64) all += __builtin_amdgcn_readlane(scan64(seq(b0).items(H)), 63);
+        const int most = max((all + a.G - 1) / a.G, 1);
+        int n = s.tiles * H * pieces(s, most), inc = scan64(n), total = __builtin_amdgcn_readlane(inc, 63);
+        for (int b0 = 64; b0 < B; b0 += 64) {
+            const Seq4 y = seq(b0);
+            total += __builtin_amdgcn_readlane(scan64(y.tiles * H * pieces(y, most)), 63);
+        }
+        // neighbouring pieces, which share their queries, on one XCD
+        const int per = (total + 7) / 8, w = blockIdx.x % 8 * per + blockIdx.x / 8;
+        if ((int)blockIdx.x / 8 >= per || w >= total) return false;
+        for (int b0 = 0, base = 0;;) {
+            const uint64_t past = __ballot(inc + base > w);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                b = b0 + l;
+                sq = lane_seq4(s, l);
+                const int at = w - base - __builtin_amdgcn_readlane(inc - n, l), np = pieces(sq, most);
+                hkv = at / np;
+                const int k = at - hkv * np;
+                c0 = first_item(k, sq.chunks, np);
+                nch = first_item(k + 1, sq.chunks, np) - c0;
+                return true;
+            }
+            base += __builtin_amdgcn_readlane(inc, 63);
+            b0 += 64;
+            if (b0 >= B) return false;
+            s = seq(b0);
+            n = s.tiles * H * pieces(s, most);
+            inc = scan64(n);
+        }
+    }
+};
+
 template <int DP, bool IS_BF16, bool BIAS>
-__global__ void __launch_bounds__(kThreads4) __attribute__((amdgpu_waves_per_eu(kManyWgs)))
+__global__ void __launch_bounds__(kManyThreads) __attribute__((amdgpu_waves_per_eu(2 * kManyWgs)))
 mfa_kv8_weights_many_kernel(K4Args) {
     typedef op_of<IS_BF16> op_t;
-    constexpr int DS = DP / 16, CPR = DP / 8, QST = DP + 8, NQ = kWCols * CPR / kThreads4;
-    static_assert(kWCols * CPR % kThreads4 == 0, "whole rounds of loads");
-    __shared__ __attribute__((aligned(16))) uint16_t q_s[2][kWCols * QST];
-    __shared__ __attribute__((aligned(16))) float nlse_s[2][kWCols], slope_s[2][BIAS ? kWCols : 1];
-    __shared__ __attribute__((aligned(16))) int center_s[2][kWCols];
-    __shared__ float sum_s[2][64];
-    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave & 1, cg = wave >> 1;
-    Walk4 wk;
-    if (!wk.start()) return;
-    while (true) {
-        if (!wk.next(args4())) return;
-        K4Const& a = args4();
-        const int Lk = wk.sq.Lk, dq = Lk - wk.sq.Lq;
-        ScoreOf score = score_of(a);
-        score.bias = BIAS;
-        const int i_last = (int)div4(wk.ncol - 1, a.by_r);
-        const int t_lo = lo4(a.wl, dq), t_hi = hi4(a.causal, a.wr, i_last + dq, Lk);
-        const Chunks4 ch = chunks4(t_lo, t_hi, wk.c0, wk.nch);
+    typedef KeyBlock8<DP> Blk;
+    constexpr int KS = DP / 32, CPR = DP / 8;
+    constexpr int kWCols = 128;             // columns of a tile in LDS
+    constexpr int kWChunks = BIAS ? 2 : 4;  // chunks whose sums are kept in LDS
+    constexpr int NQ = kWCols * CPR / kManyThreads;
+    constexpr int kBlocks = kWChunks * kChunk4 / 32, kWaves = kManyThreads / 64;
+    static_assert(kWCols * CPR % kManyThreads == 0, "whole rounds of loads");
+    // two tiles of queries: 16-byte chunk c of row r is in slot c ^ swz(r) (the loads
+    // straight into LDS leave no room for padding; a read takes a chunk of 16 rows)
+    __shared__ __attribute__((aligned(16))) uint16_t q_s[2][kWCols * DP];
+    auto swz = [](int r) { return DP == 128 ? r & 15 : DP == 64 ? r >> 1 & 7 : r >> 2 & 3; };
+    // of the columns of three tiles: the query's address, the log-sum-exp, the keys that they
+    // see, and for the biases
+    __shared__ const char* row_s[3][kWCols];
+    __shared__ __attribute__((aligned(16))) float nlse_s[3][kWCols], slope_s[3][BIAS ? kWCols : 4];
+    __shared__ __attribute__((aligned(16))) int lo_s[3][kWCols], hi_s[3][kWCols], center_s[3][BIAS ? kWCols : 4];
+    __shared__ float sum_s[4][kBlocks][32];
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, grp = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    K4Const& a = args4();
+    Piece4 wk;
+    if (!wk.find(a)) return;
+    const int Lk = wk.sq.Lk, dq = Lk - wk.sq.Lq, causal = a.causal, wl = a.wl, wr = a.wr;
+    ScoreOf score = score_of(a);
+    score.bias = BIAS;
+    const FastDiv by_r = {a.by_r.d, a.by_r.m, a.by_r.s};
+    const int i_last = wk.sq.Lq - 1;
+    const int t_lo = lo4(wl, dq), t_hi = hi4(causal, wr, i_last + dq, Lk);
+    const Chunks4 ch = chunks4(t_lo, t_hi, wk.c0, wk.nch);
+    for (int c0 = ch.beg; c0 < ch.end; c0 += kWChunks) {
+        // ---- some chunks: blocks of 32 keys, dealt over the wavefronts; where there are
+        // fewer than wavefronts, two or four share one and take every second or fourth 32
+        // columns
+        const int j0 = c0 * kChunk4, jend = min(min(c0 + kWChunks, ch.end) * kChunk4, Lk);
+        const int nb = (jend - j0 + 31) / 32, cw = nb <= kWaves / 4 ? 4 : nb <= kWaves / 2 ? 2 : 1, kw = kWaves / cw;
+        const int cg = wave / kw, b0 = wave - cg * kw;
+        typename Blk::Offsets off;
+        off.init(args4(), lane);
         Pages4<WFormat<DP>> pg;
-        pg.start(a, wk.b, wk.hkv, Lk, ch.beg * kChunk4 + 64 * kg, kChunk4);
-        for (int c = ch.beg; c < ch.end; ++c) {
-            const int j0 = c * kChunk4, j = j0 + 64 * kg;
-            // ---- this wavefront's 64 keys: lane (key l32, half) of tile kt holds elements
-            // 32 p + 16 half + 0..15, steps 2 p and 2 p + 1 of the product
-            op_t kf[2][DS];
-            const int row = pg.row_of(j);
-            const uint32_t at = (uint32_t)((row + lane) * pg.rstride[2]);
-            const float before = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(pg.rs[2], at, 0, 0));
-            const uint8_t ks = __builtin_amdgcn_raw_buffer_load_b8(pg.rs[1], (uint32_t)(row / kKv8Block * pg.rstride[1]), 0, 0);
-            {
-                u32x4_t raw[2][DP / 32];
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int p = 0; p < DP / 32; ++p)
-                        raw[kt][p] = __builtin_amdgcn_raw_buffer_load_b128(
-                            pg.rs[0], (uint32_t)((row + 32 * kt + l32) * pg.rstride[0] + 32 * p + 16 * half), 0, 0);
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int p = 0; p < DP / 32; ++p) {
-                        kf[kt][2 * p] = kv8_operand<op_t>(raw[kt][p][0], raw[kt][p][1]);
-                        kf[kt][2 * p + 1] = kv8_operand<op_t>(raw[kt][p][2], raw[kt][p][3]);
-                    }
-            }
-            const float sk = kv8_scale(ks);
-            // ---- the columns that see any key of the chunk, 64 at a time
-            K4Const& b = args4();
-            const int jl = min(j0 + kChunk4 - 1, Lk - 1);
-            int i0 = 0, i1 = wk.sq.Lq;
-            if (b.causal) i0 = max(i0, j0 - dq);
-            if (b.wr >= 0) i0 = max(i0, (int)max((int64_t)j0 - b.wr - dq, (int64_t)0));
-            if (b.wl >= 0) i1 = (int)min((int64_t)i1, (int64_t)jl + b.wl - dq + 1);
-            const int cbeg = i0 < i1 ? i0 * b.R / kWCols * kWCols : 0, cend = i0 < i1 ? i1 * b.R : 0;
-            u32x4_t qr[NQ];
-            float nl = 0.f, sl = 0.f;
-            auto qload = [&](int col0) {
-                K4Const& e = args4();
-#pragma unroll
-                for (int x = 0; x < NQ; ++x) {
-                    const int u = tid + kThreads4 * x, col = col0 + u / CPR, d = 8 * (u % CPR);
-                    const int i = (int)div4(col, e.by_r), h = wk.hkv * e.R + col - i * e.R;
-                    qr[x] = u32x4_t{0, 0, 0, 0};
-                    if (col < wk.ncol)
-                        qr[x] = *reinterpret_cast<const u32x4_t*>(
-                            e.q + (row_off4(e.cu_q != nullptr, wk.b, wk.sq.q0, i, h, e.qb, e.qs, e.qh) + d) * 2);
-                }
-                if (tid < kWCols) {
-                    const int col = col0 + tid, i = (int)div4(col, e.by_r), h = wk.hkv * e.R + col - i * e.R;
-                    nl = neg_lse2(e, col < wk.ncol, wk.b, wk.sq.q0, i, h);
-                    if (BIAS && score.alibi) sl = col < wk.ncol ? e.alibi[wk.b * e.alibi_bstride + h] : 0.f;
-                }
-            };
-            auto qstore = [&](int to, int col0) {
-#pragma unroll
-                for (int x = 0; x < NQ; ++x) {
-                    const int u = tid + kThreads4 * x;
-                    *reinterpret_cast<u32x4_t*>(q_s[to] + u / CPR * QST + 8 * (u % CPR)) = qr[x];
-                }
-                if (tid < kWCols) {
-                    nlse_s[to][tid] = nl;
-                    if constexpr (BIAS) slope_s[to][tid] = sl;
-                    center_s[to][tid] = (int)div4(col0 + tid, args4().by_r) + dq;
-                }
-            };
-            float acc[2] = {0.f, 0.f};
-            if (cbeg < cend) qload(cbeg);
-            __syncthreads();  // (the last chunk's tiles and sums are read)
-            if (cbeg < cend) qstore(0, cbeg);
+        pg.start(a, wk.b, wk.hkv, Lk, j0 + 32 * b0, 32 * kw);
+        Blk raw;
+        auto kload = [&](int blk) {
+            const int row = pg.row_of(j0 + 32 * min(blk, nb - 1));
+            raw.load(pg.rs, off, (uint32_t)(row * pg.rstride[0]), (uint32_t)(row / kKv8Block * pg.rstride[1]));
+        };
+        kload(b0);
+        auto place = [&](int blk) { return (uint32_t)((pg.row_of(j0 + 32 * blk) + (lane & 31)) * pg.rstride[2]); };
+        // (the first block's weights: where there is no other, nothing waits for them at the end)
+        const float before = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(pg.rs[2], place(min(b0, nb - 1)), 0, 0));
+        for (int blk = b0; blk < nb; blk += kw) sum_s[cg][blk][lane & 31] = 0.f;
+        // the columns that see any of these keys
+        int i0 = 0, i1 = wk.sq.Lq;
+        if (causal) i0 = max(i0, j0 - dq);
+        if (wr >= 0) i0 = (int)max((int64_t)i0, (int64_t)j0 - wr - dq);
+        if (wl >= 0) i1 = (int)min((int64_t)i1, (int64_t)jend + wl - dq);
+        const int cbeg = i0 < i1 ? i0 * a.R / 32 * 32 : 0, cend = i0 < i1 ? i1 * a.R : 0;
+        const int n = (cend - cbeg + kWCols - 1) / kWCols;  // tiles of columns
+        // Step k brings tile k in, works on tile k - 1 and looks up the columns of tile k + 1.
+        // (Every part stands here once: what is run once costs the fetch of its code.)
+        for (int k = -1; k <= n; ++k) {
             __syncthreads();
-            for (int col0 = cbeg, buf = 0; col0 < cend; col0 += kWCols, buf ^= 1) {
-                const bool more = col0 + kWCols < cend;
-                if (more) qload(col0 + kWCols);
-                const int cw = col0 + 32 * cg;  // this wavefront's columns
-                if (cw < wk.ncol) {
-                    f32x16_t s[2];
+            if (k >= 0 && k < n) {
+#pragma unroll 2
+                for (int x = 0; x < NQ; ++x) {
+                    const int first = (kWaves * x + wave) * 64, u = first + lane, r = u / CPR, c = (u - r * CPR) ^ swz(r);
+                    lds_load16(row_s[k % 3][r] + 16 * c, q_s[k & 1] + 8 * first);
+                }
+            }
+            const int at = (k - 1) & 1, col0 = cbeg + (k - 1) * kWCols, as = (k + 2) % 3;
+            const int tiles = k < 1 ? 0 : min((cend - col0 + 31) / 32, kWCols / 32);
+            for (int blk = b0; blk < nb && tiles > 0; blk += kw) {
+                const int j = j0 + 32 * blk;
+                op_t kf[2][KS];  // keys 16 kk + l16
 #pragma unroll
-                    for (int kt = 0; kt < 2; ++kt)
+                for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
+                    for (int s = 0; s < KS; ++s) kf[kk][s] = raw.template k_operand<op_t>(kk, s, grp);
+                const float sk = raw.k_scale();
+                // (the next block, or the first one again for the next columns)
+                if (nb > kw) kload(blk + kw < nb ? blk + kw : b0);
+                float acc[2] = {0.f, 0.f};
+                // 32 columns; masked: some column does not see some key
+                auto tile = [&](int t, auto masked) {
 #pragma unroll
-                    for (int t = 0; t < DS; ++t) {
-                        const op_t qf = *reinterpret_cast<const op_t*>(q_s[buf] + (32 * cg + l32) * QST + 32 * (t >> 1) + 16 * half + 8 * (t & 1));
+                    for (int ct = 0; ct < 2; ++ct) {
+                        const int row = 32 * t + 16 * ct + l16, at0 = 32 * t + 16 * ct + 4 * grp;
+                        f32x4_t s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-                        for (int kt = 0; kt < 2; ++kt) {
-                            if constexpr (IS_BF16) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf, kf[kt][t], s[kt], 0, 0, 0);
-                            else s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qf, kf[kt][t], s[kt], 0, 0, 0);
+                        for (int d = 0; d < KS; ++d) {
+                            const op_t qf = *reinterpret_cast<const op_t*>(q_s[at] + row * DP + 8 * ((Blk::element(grp, d) / 8) ^ swz(row)));
+#pragma unroll
+                            for (int kk = 0; kk < 2; ++kk) {
+                                if constexpr (IS_BF16) s[kk] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf, kf[kk][d], s[kk], 0, 0, 0);
+                                else s[kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf, kf[kk][d], s[kk], 0, 0, 0);
+                            }
                         }
-                    }
-                    // register r is column cw + 8 (r / 4) + 4 half + r % 4
-                    K4Const& e = args4();
-                    const int ca = (int)div4(cw, e.by_r) + dq, cb = (int)div4(min(cw + 31, wk.ncol - 1), e.by_r) + dq;
-                    const bool masked = j < lo4(e.wl, cb) || j + 63 > hi4(e.causal, e.wr, ca, Lk);
-                    const int causal = e.causal, wl = e.wl, wr = e.wr;
+                        // register r is column 32 t + 16 ct + 4 grp + r
+                        const f32x4_t nls = *reinterpret_cast<const f32x4_t*>(nlse_s[as] + at0);
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int at0 = 32 * cg + 8 * g + 4 * half;
-                        const f32x4_t nls = *reinterpret_cast<const f32x4_t*>(nlse_s[buf] + at0);
-                        f32x4_t sls = {0.f, 0.f, 0.f, 0.f};
-                        if (BIAS) sls = *reinterpret_cast<const f32x4_t*>(slope_s[buf] + at0);
-                        int cen[4] = {0, 0, 0, 0};
-                        if (BIAS || masked) {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) cen[r] = center_s[buf][at0 + r];
-                        }
-#pragma unroll
-                        for (int kt = 0; kt < 2; ++kt) {
-                            const int key = j + 32 * kt + l32;
+                        for (int kk = 0; kk < 2; ++kk) {
+                            const int key = j + 16 * kk + l16;
                             float p[4];
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) p[r] = fast_exp2(score(s[kt][4 * g + r], sk, nls[r], sls[r], cen[r] - key));
-                            if (masked) {
+                            for (int r = 0; r < 4; ++r)
+                                p[r] = fast_exp2(score(s[kk][r], sk, nls[r], BIAS ? slope_s[as][at0 + r] : 0.f,
+                                                       BIAS ? center_s[as][at0 + r] - key : 0));
+                            if constexpr (masked.value) {
 #pragma unroll
-                                for (int r = 0; r < 4; ++r) {
-                                    const bool sees = (key >= lo4(wl, cen[r])) & (key <= hi4(causal, wr, cen[r], Lk)) &
-                                                      (nls[r] != -INFINITY);
-                                    p[r] = sees ? p[r] : 0.f;
-                                }
+                                for (int r = 0; r < 4; ++r)
+                                    p[r] = ((key >= lo_s[as][at0 + r]) & (key <= hi_s[as][at0 + r])) ? p[r] : 0.f;
                             }
-                            acc[kt] += (p[0] + p[1]) + (p[2] + p[3]);
+                            acc[kk] += (p[0] + p[1]) + (p[2] + p[3]);
                         }
                     }
+                };
+                for (int t = cg; t < tiles; t += cw) {
+                    const int cw0 = col0 + 32 * t;
+                    const int ca = (int)quotient(cw0, by_r) + dq, cb = (int)quotient(min(cw0 + 31, cend - 1), by_r) + dq;
+                    if (hi4(causal, wr, cb, Lk) < j || lo4(wl, ca) > j + 31) continue;  // (no column sees a key)
+                    if (j < lo4(wl, cb) || j + 31 > hi4(causal, wr, ca, Lk)) tile(t, std::true_type{});
+                    else tile(t, std::false_type{});
                 }
-                if (more) qstore(buf ^ 1, col0 + kWCols);
-                __syncthreads();
+                // lane 16 kk + l16 has the sum of its own key
+                const float s0 = sum_groups4(acc[0]), s1 = sum_groups4(acc[1]);
+                if (lane < 32) sum_s[cg][blk][lane] += grp ? s1 : s0;
             }
-            // lane 32 kt + l32 has the sum of its own key
-            const float s0 = sum_halves(acc[0]), s1 = sum_halves(acc[1]);
-            const float sum = half ? s1 : s0;
-            if (cg == 1) sum_s[kg][lane] = sum;
-            __syncthreads();
-            if (cg == 0) {
-                const float w = (j + lane < dq ? before : 0.f) + (sum + sum_s[kg][lane]);
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(w), pg.rs[2], at, 0, 0);
+            if (k + 1 < n && tid < kWCols) {
+                // (columns behind the last repeat it, with a log-sum-exp that leaves them out)
+                K4Const& e = args4();
+                const int to = (k + 1) % 3, mine = cbeg + (k + 1) * kWCols + tid, col = min(mine, cend - 1);
+                const int i = (int)quotient(col, by_r), h = wk.hkv * e.R + col - i * e.R, c = i + dq;
+                const float nl = neg_lse2(e, mine < cend, wk.b, wk.sq.q0, i, h);
+                row_s[to][tid] = e.q + row_off4(e.cu_q != nullptr, wk.b, wk.sq.q0, i, h, e.qb, e.qs, e.qh) * 2;
+                lo_s[to][tid] = lo4(wl, c);
+                if constexpr (BIAS) {
+                    center_s[to][tid] = c;
+                    slope_s[to][tid] = score.alibi ? e.alibi[wk.b * e.alibi_bstride + h] : 0.f;
+                }
+                nlse_s[to][tid] = nl;
+                hi_s[to][tid] = nl == -INFINITY ? -1 : hi4(causal, wr, c, Lk);
+            }
+            wait_vm<0>();
+        }
+        if (cw > 1) __syncthreads();
+        if (cg == 0) {
+            for (int blk = b0; blk < nb; blk += kw) {
+                // (outside of the condition: a page looked up by some lanes would no longer be uniform)
+                const uint32_t all = place(blk), at = lane < 32 ? all : 0x80000000u;
+                float w = blk == b0 ? before : __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(pg.rs[2], at, 0, 0));
+                w = j0 + 32 * blk + lane < dq ? w : 0.f;
+                float sum = sum_s[0][blk][lane & 31];
+                for (int z = 1; z < cw; ++z) sum += sum_s[z][blk][lane & 31];
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(w + sum), pg.rs[2], at, 0, 0);
             }
         }
+        if (cw > 1) __syncthreads();  // (the sums are read)
     }
 }
 
@@ -410,9 +462,12 @@ int mfa_kv8_weights(const mfa_kv8_weights_params* p, void* stream) {
         a.min_cols = few ? 1 : 17;
         a.max_cols = few ? 16 : 0x7fffffff;
         a.G = (int32_t)std::min<int64_t>(units * chunks, (int64_t)cus * (few ? kFewWgs : kManyWgs));
-        a.xcds = !few && a.G % 8 == 0 ? 8 : 1;  // (neighbouring chunks of a K/V head share its queries in their XCD's L2)
+        // (pieces: at most one more of each unit than its share)
+        int64_t grid = few ? a.G : std::min<int64_t>(units * chunks, a.G + units);
+        if (!few) grid = (grid + 7) / 8 * 8;
+        a.xcds = 1;
         const w8_fn fn = weights_of(f.head_dim, few != 0, f.dtype == MFA_DTYPE_BF16, a.bias != 0);
-        hipLaunchKernelGGL(fn, dim3(a.G), dim3(kThreads4), 0, static_cast<hipStream_t>(stream), a);
+        hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(few ? kThreads4 : kManyThreads), 0, static_cast<hipStream_t>(stream), a);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return w8err(MFA_ERR_LAUNCH, "%s: launch failed: %s", who, hipGetErrorString(e));
