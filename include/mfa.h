@@ -550,8 +550,9 @@ int mfa_kv8_weights_params_size(void);
  * and weights.  n = min(cache_seqlens, max_seqlen_k, what the table can name), max_seqlen_k
  * 0 leaving that bound out; new_seqlens [batch] (may be cache_seqlens itself) receives
  * min(n, budget).  A row on a page id outside the pool reads as zeros with weight 0 and
- * drops what is written.  budget and recent >= 0.  `workspace`: 256-byte aligned, at least
- * mfa_kv8_evict_workspace_bytes bytes.  Three kernels; never synchronizes, never allocates.
+ * drops what is written.  budget and recent >= 0; the pool has less than 2^31 rows.
+ * `workspace`: 256-byte aligned, at least mfa_kv8_evict_workspace_bytes bytes.  Three
+ * kernels; never synchronizes, never allocates.
  */
 typedef struct mfa_kv8_evict_params {
     mfa_kv8_cache cache;

@@ -5,29 +5,31 @@
 //  * select: one workgroup per (sequence, head) finds the weight of the last row that
 //    stays and lists the rows that stay in order.  Weights become unsigned keys of the
 //    same order; the threshold, the largest key that as many candidates reach as are
-//    to stay, is found two bits at a time by counting with ballots (no histogram:
-//    weights crowd into a few exponents, where counters in LDS would collide).  Keys
-//    stay in registers where a sequence fits (64 K rows), else they are read again.
+//    to stay, is found 11, 11 and 10 bits at a time from histograms in LDS (weights
+//    crowd into few exponents: lanes of a wavefront that agree count once together).
+//    Keys stay in LDS where a sequence fits (32768 rows), else they are read again.
 //  * save: rows only move down, and no block behind the one that holds row budget - 1
 //    is written to; the rows that stay and lie in front are what another block's new
 //    rows, or its new scale, may overwrite.  They go to the workspace as they are.
 //  * gather: a workgroup per block of 64 new rows of a head, in K or in V, collects
 //    its rows from the workspace and the cache, takes their largest magnitude, and
 //    writes them with a new scale.
-// Bound by the latency of the selection for one sequence, by the bytes of save and
-// gather for a batch.
+// One sequence (2048 of 2176 rows stay, 8 heads of 128) takes 20 us, of which the kernels
+// have 8.6, 5.2 and 6.4: the latency of a few dependent passes each.  Sixteen sequences
+// (4001 of 4096 to 16384 rows stay) take 138 us: 22, 43 and 68, the last two by the bytes.  Selecting by 32 passes over one bit took 41 us of the sixteen, and
+// workgroups of 512 threads for save and gather 158 us against 140 of 256.
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
 
 #include <algorithm>
 
+#include "mfa_kv4_attend.h"
 #include "mfa_kv8.h"
 
 namespace {
 
 constexpr int kSThreads = 1024, kSWaves = kSThreads / 64;
-constexpr int kSKeys = 64;  // keys of a thread in registers, at most
 constexpr int kEThreads = 256;
 constexpr int kStay = 0x7fffffff;
 
@@ -35,6 +37,8 @@ constexpr int kStay = 0x7fffffff;
 struct Head8 {
     int32_t first;  // first row that moves (kStay: none)
     int32_t n;      // rows of the sequence afterwards
+    int32_t low;    // rows that stay and lie in front of `safe`
+    int32_t pad;
 };
 
 struct E8Args {
@@ -49,9 +53,10 @@ struct E8Args {
     int32_t rows;    // of the workspace per (sequence, head): the budget, or none where no sequence is longer
     int32_t blocks;  // of 64 new rows per (sequence, head), at least 1
     int32_t safe;    // rows from here on are read where they are
+    int32_t four;    // weights of four adjacent rows may be loaded at once
     FastDiv by_page, by_blocks;
     Head8* head;      // [B H]
-    int32_t* idx;     // [B H rows] rows that stay, ascending
+    int32_t* idx;     // [B H rows] rows that stay, in order: their places in the pool (page page_block_size + row), or -1
     float* sw;        // [B H rows] saved weights
     uint8_t* codes;   // [2][B H rows][D] saved rows
     uint8_t* scales;  // [2][B H rows]
@@ -65,6 +70,11 @@ __device__ __forceinline__ Place8 place8(const E8Args& a, const int32_t* bt, int
     const int i = (int)quotient((uint32_t)j, a.by_page), id = bt[i];
     return Place8{(uint32_t)id < (uint32_t)a.npages ? id : -1, j - i * a.page};
 }
+__device__ __forceinline__ int packed8(const E8Args& a, const Place8& p) { return p.id < 0 ? -1 : p.id * a.page + p.row; }
+__device__ __forceinline__ Place8 unpacked8(const E8Args& a, int x) {
+    const int id = (int)quotient((uint32_t)x, a.by_page);
+    return Place8{id, x - id * a.page};
+}
 __device__ __forceinline__ float* weight_at(const E8Args& a, const Place8& p, int h) {
     return a.w + p.id * a.wp + p.row * a.wr + h * a.wh;
 }
@@ -77,182 +87,219 @@ __device__ __forceinline__ uint32_t key_of(float w) {
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// N: keys of a thread, row ((i kSWaves + wavefront) 64 + lane) of a segment of 1024 N
-template <int N>
+constexpr int kBins = 2048;
+static_assert(kBins == 2 * kSThreads, "two bins per thread");
+
+// KEYS: keys that LDS holds, 0: none
+template <int KEYS>
 __global__ void __launch_bounds__(kSThreads) mfa_kv8_select_kernel(E8Args a) {
-    constexpr int kSegment = kSThreads * N, kGroups = kSWaves * N;  // groups of 64 rows
-    static_assert(kGroups <= kSThreads, "a thread per group");
-    __shared__ int count_s[16][4];
-    __shared__ int gt_s[kGroups], eq_s[kGroups];
-    __shared__ int2 part_s[kSWaves];
-    __shared__ int first_s;
+    __shared__ __attribute__((aligned(16))) uint32_t key_s[KEYS > 0 ? KEYS : 4];
+    __shared__ int count_s[kBins];
+    __shared__ int sum_s[kSWaves], found_s[3];
+    __shared__ int gt_s[kSWaves], eq_s[kSWaves];
+    __shared__ int first_s, low_s;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int bh = blockIdx.x, b = bh / a.H, h = bh - b * a.H;
     const int n = min(max(a.lens[b], 0), a.max_k);
     if (n <= a.budget) {
-        if (tid == 0) a.head[bh] = Head8{kStay, n};
+        if (tid == 0) a.head[bh] = Head8{kStay, n, 0, 0};
         return;
     }
     const int tail = min(a.recent, a.budget), m = n - tail, need = a.budget - tail;  // need < m
     const int32_t* bt = a.bt + b * a.bt_b;
     int32_t* const idx = a.idx + (int64_t)bh * a.rows;
-    if (tid < 64) count_s[tid >> 2][tid & 3] = 0;
-    if (tid == 0) first_s = m;
-    uint32_t key[N];
-    auto load = [&](int seg) {
+    if (tid == 0) {
+        first_s = m;
+        low_s = max(0, min(tail, a.safe - m));
+    }
+
+    // the keys of rows j .. j + 3 (j a multiple of 4), 0 for rows from m on
+    auto read4 = [&](int j) {
+        float w[4] = {0.f, 0.f, 0.f, 0.f};
+        if (j < m) {
+            const Place8 p = place8(a, bt, j);  // (of all four)
+            if (p.id >= 0) {
+                const float* at = weight_at(a, p, h);
+                if (a.four) {
+                    const float4 y = *reinterpret_cast<const float4*>(at);
+                    w[0] = y.x; w[1] = y.y; w[2] = y.z; w[3] = y.w;
+                } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            // (64 rows of a wavefront lie in one page)
-            const int j0 = seg + (i * kSWaves + wave) * 64;
-            float w = 0.f;
-            if (j0 < m) {
-                const Place8 p = place8(a, bt, j0);
-                if (p.id >= 0 && j0 + lane < m) w = a.w[p.id * a.wp + (p.row + lane) * a.wr + h * a.wh];
+                    for (int i = 0; i < 4; ++i) w[i] = at[i * a.wr];
+                }
             }
-            key[i] = __float_as_uint(w);
         }
+        u32x4_t k;
 #pragma unroll
-        for (int i = 0; i < N; ++i) key[i] = seg + (i * kSWaves + wave) * 64 + lane < m ? key_of(__uint_as_float(key[i])) : 0u;
+        for (int i = 0; i < 4; ++i) k[i] = j + i < m ? key_of(w[i]) : 0u;
+        return k;
     };
-    const bool once = m <= kSegment;
-    if (once) load(0);
+    auto keys4 = [&](int j) {
+        if constexpr (KEYS > 0) return *reinterpret_cast<const u32x4_t*>(key_s + j);
+        else return read4(j);
+    };
+    const int end4 = (m + 4 * kSThreads - 1) / (4 * kSThreads) * (4 * kSThreads);  // whole rounds of the workgroup
+    if constexpr (KEYS > 0) {
+        static_assert(KEYS % (4 * kSThreads) == 0, "whole rounds");
+#pragma unroll 2
+        for (int j = 4 * tid; j < end4; j += 4 * kSThreads) *reinterpret_cast<u32x4_t*>(key_s + j) = read4(j);
+    }
     __syncthreads();
 
-    // ---- the largest key that `need` candidates reach (need = 0: none stays but the tail)
+    // ---- the threshold t: candidates above it stay, and of those at it the first `spare`
     uint32_t t = 0;
-    if (need > 0) {
-        for (int step = 0; step < 16; ++step) {
-            const int shift = 30 - 2 * step;
-            const uint32_t t1 = t | 1u << shift, t2 = t | 2u << shift, t3 = t | 3u << shift;
-            int c1 = 0, c2 = 0, c3 = 0;
-            for (int seg = 0; seg < m; seg += kSegment) {
-                if (!once) load(seg);
+    bool met = need == 0;  // (none but the tail stays)
+    for (int pass = 0, left = need; pass < 3 && !met; ++pass) {  // left: to stay of those that begin with t's bits
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, known = pass == 0 ? 0 : pass == 1 ? 21 : 10;
+        const uint32_t mask = pass < 2 ? kBins - 1 : kBins / 2 - 1;
+        count_s[tid] = count_s[tid + kSThreads] = 0;
+        __syncthreads();
+        for (int j = 4 * tid; j < end4; j += 4 * kSThreads) {
+            const u32x4_t k = keys4(j);
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    c1 += __builtin_popcountll(__ballot(key[i] >= t1));
-                    c2 += __builtin_popcountll(__ballot(key[i] >= t2));
-                    c3 += __builtin_popcountll(__ballot(key[i] >= t3));
+            for (int i = 0; i < 4; ++i) {
+                const bool on = j + i < m && (pass == 0 || (k[i] ^ t) >> known == 0);
+                const uint64_t any = __ballot(on);
+                if (any == 0) continue;
+                const int bin = (int)(k[i] >> shift & mask), one = __builtin_amdgcn_readlane(bin, __builtin_ctzll(any));
+                if (__ballot(on && bin == one) == any) {  // (all the same)
+                    if (lane == __builtin_ctzll(any)) atomicAdd(&count_s[one], __builtin_popcountll(any));
+                } else if (on) {
+                    atomicAdd(&count_s[bin], 1);
                 }
             }
-            if (lane == 0) {
-                atomicAdd(&count_s[step][0], c1);
-                atomicAdd(&count_s[step][1], c2);
-                atomicAdd(&count_s[step][2], c3);
-            }
-            __syncthreads();
-            if (count_s[step][2] >= need) t = t3;
-            else if (count_s[step][1] >= need) t = t2;
-            else if (count_s[step][0] >= need) t = t1;
         }
+        __syncthreads();
+        // sums from the top: thread i holds the two bins of its place counted from above
+        const int top = kBins - 1 - 2 * tid, c0 = count_s[top], c1 = count_s[top - 1];
+        const int inc = scan64(c0 + c1);
+        if (lane == 63) sum_s[wave] = inc;
+        __syncthreads();
+        int above = inc - c0 - c1;
+#pragma unroll
+        for (int w = 0; w < kSWaves; ++w) above += w < wave ? sum_s[w] : 0;
+        if (above < left && left <= above + c0 + c1) {  // (one thread)
+            const bool first = left <= above + c0;
+            found_s[0] = first ? top : top - 1;
+            found_s[1] = left - above - (first ? 0 : c0);  // to stay of this bin
+            found_s[2] = first ? c0 : c1;                  // and what it holds
+        }
+        __syncthreads();
+        t |= (uint32_t)found_s[0] << shift;
+        left = found_s[1];
+        met = found_s[2] == left;
     }
+    // (met: all that reach t stay; with need = 0 none)
+    if (met) t -= 1;
 
-    // ---- the rows that stay, in order: those above t, and of those at t the first
-    int base_gt = 0, base_eq = 0, spare = 0;
-    if (need > 0) {
-        // (how many at t: need less those above it, counted on the way below)
-        int gt = 0;
-        for (int seg = 0; seg < m; seg += kSegment) {
-            if (!once) load(seg);
+    // ---- the rows that stay, in order: those above t, and of those at t the first.  Each
+    // wavefront takes consecutive rows.
+    const int per = ((m + kSWaves - 1) / kSWaves + 255) / 256 * 256, w0 = wave * per, w1 = min(w0 + per, m);
+    int gt = 0, eq = 0;
+    for (int j = w0; j < w1; j += 256) {
+        const u32x4_t k = j + 4 * lane < end4 ? keys4(j + 4 * lane) : u32x4_t{0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < N; ++i) gt += __builtin_popcountll(__ballot(key[i] > t));
+        for (int i = 0; i < 4; ++i) {
+            gt += __builtin_popcountll(__ballot(k[i] > t));
+            eq += __builtin_popcountll(__ballot(k[i] == t));
         }
-        if (lane == 0) atomicAdd(&count_s[0][3], gt);
-        __syncthreads();
-        spare = need - count_s[0][3];
-        for (int seg = 0; seg < m; seg += kSegment) {
-            if (!once) load(seg);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const uint64_t g = __ballot(key[i] > t), e = __ballot(key[i] == t);
-                if (lane == 0) {
-                    gt_s[i * kSWaves + wave] = __builtin_popcountll(g);
-                    eq_s[i * kSWaves + wave] = __builtin_popcountll(e);
-                }
-            }
-            __syncthreads();
-            // exclusive prefix sums over the groups
-            const int g0 = tid < kGroups ? gt_s[tid] : 0, e0 = tid < kGroups ? eq_s[tid] : 0;
-            int g = g0, e = e0;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int yg = __shfl_up(g, o), ye = __shfl_up(e, o);
-                if (lane >= o) {
-                    g += yg;
-                    e += ye;
-                }
-            }
-            if (lane == 63) part_s[wave] = make_int2(g, e);
-            __syncthreads();
-            int all_g = 0, all_e = 0;
-#pragma unroll
-            for (int w = 0; w < kSWaves; ++w) {
-                const int2 p = part_s[w];
-                if (w < wave) {
-                    g += p.x;
-                    e += p.y;
-                }
-                all_g += p.x;
-                all_e += p.y;
-            }
-            if (tid < kGroups) {
-                gt_s[tid] = base_gt + g - g0;
-                eq_s[tid] = base_eq + e - e0;
-            }
-            __syncthreads();
-            int gone = m;  // the first row that goes
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int row = seg + (i * kSWaves + wave) * 64 + lane;
-                const bool is_gt = key[i] > t, is_eq = key[i] == t;
-                const uint64_t gb = __ballot(is_gt), eb = __ballot(is_eq), below = (1ull << lane) - 1;
-                const int eq = eq_s[i * kSWaves + wave] + __builtin_popcountll(eb & below);
-                const bool stays = is_gt || (is_eq && eq < spare);
-                if (stays) idx[gt_s[i * kSWaves + wave] + __builtin_popcountll(gb & below) + min(eq, spare)] = row;
-                else if (row < gone) gone = row;
-            }
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) gone = min(gone, __shfl_xor(gone, o));
-            if (lane == 0 && gone < m) atomicMin(&first_s, gone);
-            base_gt += all_g;
-            base_eq += all_e;
-            __syncthreads();
-        }
-    } else {
-        if (tid == 0) first_s = 0;
-        __syncthreads();
     }
-    for (int r = tid; r < tail; r += kSThreads) idx[need + r] = m + r;
+    if (lane == 0) {
+        gt_s[wave] = gt;
+        eq_s[wave] = eq;
+    }
+    __syncthreads();
+    int all_gt = 0, base_gt = 0, base_eq = 0;
+#pragma unroll
+    for (int w = 0; w < kSWaves; ++w) {
+        all_gt += gt_s[w];
+        base_gt += w < wave ? gt_s[w] : 0;
+        base_eq += w < wave ? eq_s[w] : 0;
+    }
+    const int spare = need - all_gt;  // (of those at t; none where all that reach it stay)
+    int gone = m, low = 0;            // the first row that goes; rows that stay in front of `safe`
+    for (int j = w0; j < w1; j += 256) {
+        const u32x4_t k = j + 4 * lane < end4 ? keys4(j + 4 * lane) : u32x4_t{0, 0, 0, 0};
+        // a lane's four rows are adjacent: sums of the lanes below
+        int g = 0, e = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            g += k[i] > t;
+            e += k[i] == t;
+        }
+        const int both = g | e << 16, inc = scan64(both), last = __builtin_amdgcn_readlane(inc, 63);
+        int at_g = base_gt + ((inc - both) & 0xffff), at_e = base_eq + ((inc - both) >> 16);
+        const Place8 p = both ? place8(a, bt, j + 4 * lane) : Place8{-1, 0};  // (of all four)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = j + 4 * lane + i;
+            const bool is_gt = k[i] > t, is_eq = k[i] == t;
+            if (is_gt || (is_eq && at_e < spare)) {
+                idx[at_g + min(at_e, spare)] = packed8(a, Place8{p.id, p.row + i});
+                low += row < a.safe;
+            } else {
+                gone = min(gone, row);
+            }
+            at_g += is_gt;
+            at_e += is_eq;
+        }
+        base_gt += last & 0xffff;
+        base_eq += last >> 16;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        gone = min(gone, __shfl_xor(gone, o));
+        low += __shfl_xor(low, o);
+    }
+    if (lane == 0) {
+        if (gone < m) atomicMin(&first_s, gone);
+        atomicAdd(&low_s, low);
+    }
+    for (int r = tid; r < tail; r += kSThreads) idx[need + r] = packed8(a, place8(a, bt, m + r));
+    __syncthreads();
     // (first_s = budget: the rows that stay are the first ones)
-    if (tid == 0) a.head[bh] = Head8{first_s < a.budget ? first_s : kStay, a.budget};
+    if (tid == 0) a.head[bh] = Head8{first_s < a.budget ? first_s : kStay, a.budget, low_s, 0};
 }
 
 // Rows of changing blocks that stay and lie in front of `safe`, into the workspace: 64
-// per workgroup.
+// per workgroup, in K (blockIdx.y 0) or V.
+template <int D>
 __global__ void __launch_bounds__(kEThreads) mfa_kv8_save_kernel(E8Args a) {
-    const int bh = (int)quotient(blockIdx.x, a.by_blocks), b = bh / a.H, h = bh - b * a.H;
+    constexpr int CPR = D / 16, NI = (kKv8Block * CPR + kEThreads - 1) / kEThreads;
+    const int bh = (int)quotient(blockIdx.x, a.by_blocks), h = bh % a.H, which = blockIdx.y;
     const int i0 = ((int)blockIdx.x - bh * a.blocks) * kKv8Block;
-    const int first = a.head[bh].first;
-    const int from = first / kKv8Block * kKv8Block;  // (a block that changes takes all of its rows)
-    if (first == kStay || i0 + kKv8Block <= from) return;
-    const int32_t* bt = a.bt + b * a.bt_b;
+    const Head8 head = a.head[bh];
+    // (a block that changes takes all of its rows)
+    if (head.first == kStay || i0 + kKv8Block <= head.first || i0 >= head.low) return;
     const int32_t* idx = a.idx + (int64_t)bh * a.rows;
-    const int tid = threadIdx.x, cpr = a.D / 16;
-    for (int u = tid; u < kKv8Block * cpr; u += kEThreads) {
-        const int r = u / cpr, c = u - r * cpr, i = i0 + r;
-        if (i >= a.budget) break;
-        const int j = idx[i];
-        if (j >= a.safe) break;  // (ascending)
-        const Place8 p = place8(a, bt, j);
-        if (p.id < 0) continue;
-        const int64_t at = (int64_t)bh * a.rows + i, pools = (int64_t)a.B * a.H * a.rows;
+    const Kv4Pool& q = a.pool[which];
+    const int64_t pools = (int64_t)a.B * a.H * a.rows, saved = (int64_t)bh * a.rows;
+    const int rows = min(head.low - i0, kKv8Block);
+    u32x4_t w[NI];
+    uint8_t s[NI];
+    float weight[NI];
+    bool on[NI];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const Kv4Pool& q = a.pool[x];
-            *reinterpret_cast<u32x4_t*>(a.codes + (x * pools + at) * a.D + 16 * c) =
-                *reinterpret_cast<const u32x4_t*>(q.codes + p.id * q.cp + p.row * q.cr + h * q.ch + 16 * c);
-            if (c == 0) a.scales[x * pools + at] = q.scales[p.id * q.sp + p.row / kKv8Block * q.sr + h * q.sh];
-        }
-        if (c == 0) a.sw[at] = *weight_at(a, p, h);
+    for (int x = 0; x < NI; ++x) {
+        const int u = (int)threadIdx.x + kEThreads * x, r = u / CPR, c = u - r * CPR;
+        on[x] = false;
+        if (r >= rows) continue;
+        const int j = idx[i0 + r];
+        on[x] = j >= 0;
+        if (!on[x]) continue;
+        const Place8 p = unpacked8(a, j);
+        w[x] = *reinterpret_cast<const u32x4_t*>(q.codes + p.id * q.cp + p.row * q.cr + h * q.ch + 16 * c);
+        if (c == 0) s[x] = q.scales[p.id * q.sp + p.row / kKv8Block * q.sr + h * q.sh];
+        if (which == 0 && c == 0) weight[x] = *weight_at(a, p, h);
+    }
+#pragma unroll
+    for (int x = 0; x < NI; ++x) {
+        const int u = (int)threadIdx.x + kEThreads * x, r = u / CPR, c = u - r * CPR;
+        if (!on[x]) continue;
+        const int64_t at = saved + i0 + r;
+        *reinterpret_cast<u32x4_t*>(a.codes + (which * pools + at) * D + 16 * c) = w[x];
+        if (c == 0) a.scales[which * pools + at] = s[x];
+        if (which == 0 && c == 0) a.sw[at] = weight[x];
     }
 }
 
@@ -281,9 +328,9 @@ __global__ void __launch_bounds__(kEThreads) mfa_kv8_gather_kernel(E8Args a) {
         s[x] = weight[x] = 0.f;
         if (r >= rows) continue;
         const int j = idx[i0 + r];
-        const Place8 p = place8(a, bt, j);
-        if (p.id < 0) continue;  // (zeros)
-        if (j < a.safe) {
+        if (j < 0) continue;  // (zeros)
+        const Place8 p = unpacked8(a, j);
+        if (i0 + r < head.low) {
             const int64_t at = saved + i0 + r;
             w[x] = *reinterpret_cast<const u32x4_t*>(a.codes + (which * pools + at) * D + 16 * c);
             s[x] = kv8_scale(a.scales[which * pools + at]);
@@ -372,12 +419,14 @@ int e8_plan(const mfa_kv8_evict_params* p, E8Args* out, int64_t* bytes) {
     a.pool[1] = kv4_pool(p->cache.v);
     a.w = p->weights;
     a.wp = p->weight_page_stride; a.wr = p->weight_row_stride; a.wh = p->weight_head_stride;
+    a.four = a.wr == 1 && a.wp % 4 == 0 && a.wh % 4 == 0 && (reinterpret_cast<uintptr_t>(a.w) & 15) == 0;
     a.bt = p->cache.block_table;
     a.bt_b = p->cache.block_table_batch_stride;
     a.lens = p->cache_seqlens;
     a.new_lens = p->new_seqlens;
     a.B = p->batch; a.H = p->heads_kv; a.D = p->head_dim;
     a.page = p->cache.page_block_size; a.npages = p->cache.num_pages;
+    if ((int64_t)a.page * a.npages > 0x7fffffffLL) return e8err(MFA_ERR_INVALID, "%s: a pool of more than 2^31 - 1 rows", who);
     a.budget = p->budget; a.recent = p->recent;
     a.by_page = fast_div(a.page);
     const int64_t units = (int64_t)a.B * a.H;
@@ -429,15 +478,19 @@ int mfa_kv8_evict(const mfa_kv8_evict_params* p, void* workspace, int64_t worksp
     a.sw = reinterpret_cast<float*>(a.idx + rows);
     a.scales = reinterpret_cast<uint8_t*>(a.sw + rows);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    // keys in registers: as few as hold the longest sequence
-    const auto select = a.max_k <= 4 * kSThreads    ? mfa_kv8_select_kernel<4>
-                        : a.max_k <= 16 * kSThreads ? mfa_kv8_select_kernel<16>
-                                                    : mfa_kv8_select_kernel<kSKeys>;
+    const auto select = a.max_k <= 4096    ? mfa_kv8_select_kernel<4096>
+                        : a.max_k <= 32768 ? mfa_kv8_select_kernel<32768>
+                                           : mfa_kv8_select_kernel<0>;
     hipLaunchKernelGGL(select, dim3((unsigned)units), dim3(kSThreads), 0, st, a);
     const unsigned grid = (unsigned)(units * a.blocks);
-    if (a.rows > 0) hipLaunchKernelGGL(mfa_kv8_save_kernel, dim3(grid), dim3(kEThreads), 0, st, a);
-    const auto gather = a.D == 32 ? mfa_kv8_gather_kernel<32> : a.D == 64 ? mfa_kv8_gather_kernel<64>
-                        : a.D == 96 ? mfa_kv8_gather_kernel<96> : mfa_kv8_gather_kernel<128>;
+    typedef void (*fn)(E8Args);
+    const auto of = [&](auto pick) { return a.D == 32 ? pick(std::integral_constant<int, 32>{}) : a.D == 64 ? pick(std::integral_constant<int, 64>{})
+                                          : a.D == 96 ? pick(std::integral_constant<int, 96>{}) : pick(std::integral_constant<int, 128>{}); };
+    if (a.rows > 0) {
+        const fn save = of([](auto d) { return (fn)mfa_kv8_save_kernel<decltype(d)::value>; });
+        hipLaunchKernelGGL(save, dim3(grid, 2), dim3(kEThreads), 0, st, a);
+    }
+    const fn gather = of([](auto d) { return (fn)mfa_kv8_gather_kernel<decltype(d)::value>; });
     hipLaunchKernelGGL(gather, dim3(grid, 2), dim3(kEThreads), 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e8err(MFA_ERR_LAUNCH, "mfa_kv8_evict: launch failed: %s", hipGetErrorString(e));

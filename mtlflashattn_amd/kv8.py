@@ -214,7 +214,8 @@ def kv8_evict(k_cache, v_cache, weights, cache_seqlens, block_table, budget, rec
     captured into a graph).  A sequence has at most max_seqlen_k rows (None: as many as
     the table names); a tight bound keeps the selection short and, where the budget is
     not below it, the workspace empty.  A row on a page id outside the pool reads as
-    zeros with weight 0.  No two sequences may share a page that changes.
+    zeros with weight 0.  The pool has less than 2^31 rows.  No two sequences may share a page that
+    changes.
     """
     budget, recent = int(budget), int(recent)
     max_seqlen_k = None if max_seqlen_k is None else int(max_seqlen_k)
@@ -256,7 +257,7 @@ def _evict_plan(k_cache, v_cache, weights, cache_seqlens, block_table, budget, r
         raise ValueError("mtlflashattn_amd: k_cache: codes must be 4-D")
     Hkv, D = codes.shape[2:]
     if D not in (32, 64, 96, 128):
-        raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} of a 8-bit cache must be 32, 64, 96 or 128")
+        raise NotImplementedError(f"mtlflashattn_amd: head_dim {D} of an 8-bit cache must be 32, 64, 96 or 128")
     kv4._check_cache(k_cache, D, Hkv, codes.device, "k_cache", _KV8)
     kv4._check_cache(v_cache, D, Hkv, codes.device, "v_cache", _KV8)
     if k_cache[0].shape != v_cache[0].shape:

@@ -389,6 +389,9 @@ def test_c_evict(lib):
         refused(lib, lib.mfa_kv8_evict(ctypes.byref(p), None, 0, None), code, text)
         refused(lib, lib.mfa_kv8_evict_workspace_bytes(ctypes.byref(p)), code, text)
     p = params()
+    p.cache.num_pages = (1 << 31) // p.cache.page_block_size
+    refused(lib, lib.mfa_kv8_evict_workspace_bytes(ctypes.byref(p)), -1, "2^31 - 1 rows")
+    p = params()
     refused(lib, lib.mfa_kv8_evict(ctypes.byref(p), None, need, None), -1, "workspace")
     refused(lib, lib.mfa_kv8_evict(ctypes.byref(p), 4096 + 16, need, None), -1, "aligned")
     refused(lib, lib.mfa_kv8_evict(ctypes.byref(p), 4096, need - 1, None), -1, "needed")
