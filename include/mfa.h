@@ -551,8 +551,9 @@ int mfa_kv8_weights_params_size(void);
  * 0 leaving that bound out; new_seqlens [batch] (may be cache_seqlens itself) receives
  * min(n, budget).  A row on a page id outside the pool reads as zeros with weight 0 and
  * drops what is written.  budget and recent >= 0; the pool has less than 2^31 rows.
- * `workspace`: 256-byte aligned, at least mfa_kv8_evict_workspace_bytes bytes.  Three
- * kernels; never synchronizes, never allocates.
+ * K and V do not share memory.  `workspace`: 256-byte aligned, at least
+ * mfa_kv8_evict_workspace_bytes bytes.  Two or three kernels; never synchronizes, never
+ * allocates.
  */
 typedef struct mfa_kv8_evict_params {
     mfa_kv8_cache cache;

@@ -1,23 +1,26 @@
 // mfa_kv8_evict.hip -- eviction from a paged 8-bit K/V cache by accumulated weight
 // (mfa_kv8_evict in include/mfa.h).
 //
-// Three kernels:
 //  * select: one workgroup per (sequence, head) finds the weight of the last row that
 //    stays and lists the rows that stay in order.  Weights become unsigned keys of the
 //    same order; the threshold, the largest key that as many candidates reach as are
 //    to stay, is found 11, 11 and 10 bits at a time from histograms in LDS (weights
 //    crowd into few exponents: lanes of a wavefront that agree count once together).
 //    Keys stay in LDS where a sequence fits (32768 rows), else they are read again.
+// Then, with many heads in the batch:
+//  * walk: a workgroup per head, for K and for V, moves the rows block by block, in place.
+// With few, a workgroup per block:
 //  * save: rows only move down, and no block behind the one that holds row budget - 1
 //    is written to; the rows that stay and lie in front are what another block's new
 //    rows, or its new scale, may overwrite.  They go to the workspace as they are.
 //  * gather: a workgroup per block of 64 new rows of a head, in K or in V, collects
 //    its rows from the workspace and the cache, takes their largest magnitude, and
 //    writes them with a new scale.
-// One sequence (2048 of 2176 rows stay, 8 heads of 128) takes 20 us, of which the kernels
-// have 8.6, 5.2 and 6.4: the latency of a few dependent passes each.  Sixteen sequences
-// (4001 of 4096 to 16384 rows stay) take 138 us: 22, 43 and 68, the last two by the bytes.  Selecting by 32 passes over one bit took 41 us of the sixteen, and
-// workgroups of 512 threads for save and gather 158 us against 140 of 256.
+// One sequence (2048 of 2176 rows stay, 8 heads of 128) takes 19 us, of which select, save
+// and gather have 8.6, 5.2 and 6.0: the latency of a few dependent passes each.  Sixteen
+// sequences (4001 of 4096 to 16384 rows stay) take 98 us, select 22 of them and the rest
+// the bytes and the conversions of the walk (save and gather: 111).  Selecting by 32 passes
+// over one bit took 41 us, and save and gather by 512 threads instead of 256 18 us more.
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -31,6 +34,11 @@ namespace {
 
 constexpr int kSThreads = 1024, kSWaves = kSThreads / 64;
 constexpr int kEThreads = 256;
+// Sequences times heads from which on one workgroup moves all rows of a head.  (64 heads of
+// 128, 2067 of 2176 rows: 47 us against 53 by save and gather; 32 heads 41 against 37, 128
+// heads 55 against 81, 8 heads 39 against 24.  128 heads, 4275 of 9500: 98 against 128.)
+constexpr int kWalk = 64;
+constexpr int walk_threads(int d) { return d == 96 ? 768 : 1024; }  // (whole blocks per step)
 constexpr int kStay = 0x7fffffff;
 
 // What select leaves for the kernels behind it.
@@ -53,6 +61,7 @@ struct E8Args {
     int32_t rows;    // of the workspace per (sequence, head): the budget, or none where no sequence is longer
     int32_t blocks;  // of 64 new rows per (sequence, head), at least 1
     int32_t safe;    // rows from here on are read where they are
+    int32_t walk;    // one workgroup moves all rows of a head
     int32_t four;    // weights of four adjacent rows may be loaded at once
     FastDiv by_page, by_blocks;
     Head8* head;      // [B H]
@@ -303,6 +312,53 @@ __global__ void __launch_bounds__(kEThreads) mfa_kv8_save_kernel(E8Args a) {
     }
 }
 
+// The largest finite magnitude of 16 codes at scale s, as bits.  Magnitudes of codes have
+// the order of their values: one more than each (NaN: 0) compares in halves of a dword.
+__device__ __forceinline__ uint32_t largest8(const u32x4_t& w, float s) {
+    if (s >= 0x1p120f) {  // (some codes stand for values that are not finite)
+        uint32_t mx = 0;
+#pragma unroll 1
+        for (int e = 0; e < 16; ++e) {
+            const uint32_t z = __float_as_uint(__builtin_amdgcn_cvt_f32_fp8((int)(w[e >> 2] >> 8 * (e & 3)), 0) * s) & 0x7fffffffu;
+            mx = max(mx, z < 0x7f800000u ? z : 0u);
+        }
+        return mx;
+    }
+    typedef __attribute__((__vector_size__(2 * sizeof(uint16_t)))) uint16_t u16x2_t;
+    u16x2_t m = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t y = ((w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x7f7f7f7fu;
+        m = __builtin_elementwise_max(m, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, y & 0x00ff00ffu),
+                                                                   __builtin_bit_cast(u16x2_t, y >> 8 & 0x00ff00ffu)));
+    }
+    const uint32_t code = max(max((uint32_t)m[0], (uint32_t)m[1]), 1u) - 1;
+    return __float_as_uint(__builtin_amdgcn_cvt_f32_fp8((int)code, 0) * s);
+}
+// Unsigned maximum of a wavefront, in lane 63
+__device__ __forceinline__ uint32_t max64(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false));  // row_shr:1, 2, 4, 8
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false));  // row_bcast:15 to rows 1 and 3
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false));  // row_bcast:31 to rows 2 and 3
+    return x;
+}
+// 16 codes of scale s under a new byte.  Above 2^18 the factor only meets zeros and NaN (a
+// code is at least 2^-9, a new one at most 448), and an infinite one would make them NaN.
+__device__ __forceinline__ u32x4_t rounded8(const u32x4_t& w, float s, uint32_t byte) {
+    const float f = fminf(s * kv8_inverse(byte), 0x1p18f);
+    typedef __attribute__((__vector_size__(2 * sizeof(float)))) float f2;
+    u32x4_t z;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const f2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[e], f, false), y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[e], f, true);
+        z[e] = kv8_round4(x[0], x[1], y[0], y[1]);
+    }
+    return z;
+}
+
 // 64 new rows of a head, in K (blockIdx.y 0) or V
 template <int D>
 __global__ void __launch_bounds__(kEThreads) mfa_kv8_gather_kernel(E8Args a) {
@@ -341,29 +397,15 @@ __global__ void __launch_bounds__(kEThreads) mfa_kv8_gather_kernel(E8Args a) {
             if (which == 0 && c == 0) weight[x] = *weight_at(a, p, h);
         }
     }
-    // the largest finite magnitude
     uint32_t mx = 0;
 #pragma unroll
-    for (int x = 0; x < NI; ++x) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float y[4];
-            kv8_values4(w[x][e], s[x], y);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t z = __float_as_uint(y[i]) & 0x7fffffffu;
-                mx = max(mx, z < 0x7f800000u ? z : 0u);
-            }
-        }
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o));
-    if (lane == 0) max_s[tid >> 6] = mx;
+    for (int x = 0; x < NI; ++x) mx = max(mx, largest8(w[x], s[x]));
+    mx = max64(mx);
+    if (lane == 63) max_s[tid >> 6] = mx;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kEThreads / 64; ++i) mx = max(mx, max_s[i]);
     const uint32_t byte = kv8_byte_of(mx);
-    const float inv = kv8_inverse(byte);
     const Place8 to = place8(a, bt, i0);  // (64 rows lie in one page)
     if (to.id < 0) return;
     uint8_t* const dst = q.codes + to.id * q.cp + to.row * q.cr + h * q.ch;
@@ -372,17 +414,115 @@ __global__ void __launch_bounds__(kEThreads) mfa_kv8_gather_kernel(E8Args a) {
     for (int x = 0; x < NI; ++x) {
         const int u = tid + kEThreads * x, r = u / CPR, c = u - r * CPR;
         if (r >= rows) continue;
-        u32x4_t z;
-        const float f = s[x] * inv;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float y[4];
-            kv8_values4(w[x][e], f, y);
-            z[e] = kv8_round4(y[0], y[1], y[2], y[3]);
-        }
-        *reinterpret_cast<u32x4_t*>(dst + r * q.cr + 16 * c) = z;
+        *reinterpret_cast<u32x4_t*>(dst + r * q.cr + 16 * c) = rounded8(w[x], s[x], byte);
         if (which == 0 && c == 0) a.w[to.id * a.wp + (to.row + r) * a.wr + h * a.wh] = weight[x];
     }
+}
+
+// All new rows of a head, in K or in V, by one workgroup, blocks in order: row i comes from
+// a row >= i, so what a step writes lies in front of all that later steps read, and the
+// rows of the next two steps are on their way while this one's are rounded.  Loads have no
+// branches (a row that is none reads the pool's first), so that waits can be counted.
+template <int D, bool IS_K>
+__device__ __forceinline__ void walk8(const E8Args& a, const Head8& head, int b, int h) {
+    constexpr int THREADS = walk_threads(D), CPR = D / 16, NI = 2;
+    constexpr int UNITS = THREADS / 64 * NI;  // wavefront loads per step, CPR of them a block
+    constexpr int ROWS = UNITS / CPR * kKv8Block;
+    static_assert(UNITS % CPR == 0, "whole blocks");
+    __shared__ uint32_t max_s[2][UNITS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int32_t* bt = a.bt + b * a.bt_b;
+    const int32_t* idx = a.idx + (int64_t)(b * a.H + h) * a.rows;
+    const Kv4Pool& q = a.pool[IS_K ? 0 : 1];
+    int row[NI], col[NI];  // of a step
+#pragma unroll
+    for (int x = 0; x < NI; ++x) {
+        const int u = tid + THREADS * x;
+        row[x] = u / CPR;
+        col[x] = u - row[x] * CPR;
+    }
+    struct Places {
+        int from[NI], to[NI];  // place of a row, page id of its new one
+    };
+    struct Rows {
+        u32x4_t w[NI];
+        uint32_t s[NI];
+        float weight[NI];
+        bool on[NI];
+        int to[NI];
+    };
+    auto places = [&](int base, Places& j) {
+#pragma unroll
+        for (int x = 0; x < NI; ++x) {
+            const int i = min(base + row[x], a.budget - 1);
+            j.from[x] = idx[i];
+            j.to[x] = bt[quotient((uint32_t)i, a.by_page)];
+        }
+    };
+    auto load = [&](int base, const Places& j, Rows& y) {
+#pragma unroll
+        for (int x = 0; x < NI; ++x) {
+            y.on[x] = j.from[x] >= 0 && base + row[x] < a.budget;
+            y.to[x] = j.to[x];
+            const Place8 p = unpacked8(a, max(j.from[x], 0));
+            y.w[x] = *reinterpret_cast<const u32x4_t*>(q.codes + p.id * q.cp + p.row * q.cr + h * q.ch + 16 * col[x]);
+            y.s[x] = q.scales[p.id * q.sp + p.row / kKv8Block * q.sr + h * q.sh];
+            if (IS_K) y.weight[x] = *weight_at(a, p, h);
+        }
+    };
+    int base = head.first / kKv8Block * kKv8Block, turn = 0;
+    // rows `now` are written; `last`, two steps on, are loaded from `j`, and the places
+    // after them into `fill`
+    auto step = [&](Rows& now, Rows& last, const Places& j, Places& fill) {
+        places(base + 3 * ROWS, fill);
+        load(base + 2 * ROWS, j, last);
+        float s[NI];
+#pragma unroll
+        for (int x = 0; x < NI; ++x) {
+            if (!now.on[x]) now.w[x] = u32x4_t{0, 0, 0, 0};
+            s[x] = kv8_scale(now.s[x]);
+            const uint32_t mx = max64(largest8(now.w[x], s[x]));
+            if (lane == 63) max_s[turn][wave + THREADS / 64 * x] = mx;
+        }
+        __syncthreads();  // (and this step's rows are all read)
+#pragma unroll
+        for (int x = 0; x < NI; ++x) {
+            const int block = (wave + THREADS / 64 * x) / CPR, i = base + row[x], id = now.to[x];
+            if (i >= a.budget || (uint32_t)id >= (uint32_t)a.npages) continue;
+            uint32_t mx = 0;
+#pragma unroll
+            for (int i = 0; i < CPR; ++i) mx = max(mx, max_s[turn][block * CPR + i]);
+            const uint32_t byte = kv8_byte_of(mx);
+            const int r = i - (int)quotient((uint32_t)i, a.by_page) * a.page;
+            *reinterpret_cast<u32x4_t*>(q.codes + id * q.cp + r * q.cr + h * q.ch + 16 * col[x]) =
+                rounded8(now.w[x], s[x], byte);
+            if (col[x] != 0) continue;
+            if (r % kKv8Block == 0) q.scales[id * q.sp + r / kKv8Block * q.sr + h * q.sh] = (uint8_t)byte;
+            if (IS_K) a.w[id * a.wp + r * a.wr + h * a.wh] = now.on[x] ? now.weight[x] : 0.f;
+        }
+        base += ROWS;
+        turn ^= 1;
+        return base < a.budget;
+    };
+    Places j0, j1, j2;
+    Rows r0, r1, r2;
+    places(base, j0);
+    places(base + ROWS, j1);
+    load(base, j0, r0);
+    places(base + 2 * ROWS, j2);
+    load(base + ROWS, j1, r1);
+    while (step(r0, r2, j2, j0) && step(r1, r0, j0, j1) && step(r2, r1, j1, j2)) {
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(walk_threads(D)) mfa_kv8_walk_kernel(E8Args a) {
+    const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H;
+    const Head8 head = a.head[blockIdx.x];
+    if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.new_lens[b] = head.n;
+    if (head.first == kStay || a.npages == 0) return;
+    if (blockIdx.y == 0) walk8<D, true>(a, head, b, h);
+    else walk8<D, false>(a, head, b, h);
 }
 
 int e8err(int code, const char* fmt, ...) {
@@ -438,8 +578,9 @@ int e8_plan(const mfa_kv8_evict_params* p, E8Args* out, int64_t* bytes) {
     a.blocks = (int32_t)blocks;
     a.safe = a.rows > 0 ? (int32_t)(blocks * kKv8Block) : 0;
     a.by_blocks = fast_div(a.blocks);
+    a.walk = units >= kWalk;
     const int64_t rows = units * a.rows;
-    *bytes = (units * (int64_t)sizeof(Head8) + 255) / 256 * 256 + rows * (8 + 2 * a.D + 2) + 64;
+    *bytes = (units * (int64_t)sizeof(Head8) + 255) / 256 * 256 + rows * (a.walk ? 4 : 8 + 2 * a.D + 2) + 64;
     return MFA_OK;
 }
 
@@ -468,30 +609,40 @@ int mfa_kv8_evict(const mfa_kv8_evict_params* p, void* workspace, int64_t worksp
     if (workspace_bytes < bytes)
         return e8err(MFA_ERR_INVALID, "mfa_kv8_evict: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                      (long long)bytes);
+    if (a.npages > 0 && p->cache.k.codes == p->cache.v.codes)
+        return e8err(MFA_ERR_INVALID, "mfa_kv8_evict: K and V are the same memory");
     const int64_t units = (int64_t)a.B * a.H, rows = units * a.rows;
     char* ws = static_cast<char*>(workspace);
     a.head = reinterpret_cast<Head8*>(ws);
     ws += (units * (int64_t)sizeof(Head8) + 255) / 256 * 256;
-    a.codes = reinterpret_cast<uint8_t*>(ws);  // (16-byte aligned: rows of 32, 64, 96 or 128 bytes)
-    ws += 2 * rows * a.D;
+    if (!a.walk) {
+        a.codes = reinterpret_cast<uint8_t*>(ws);  // (16-byte aligned: rows of 32, 64, 96 or 128 bytes)
+        ws += 2 * rows * a.D;
+        a.sw = reinterpret_cast<float*>(ws);
+        ws += 4 * rows;
+    }
     a.idx = reinterpret_cast<int32_t*>(ws);
-    a.sw = reinterpret_cast<float*>(a.idx + rows);
-    a.scales = reinterpret_cast<uint8_t*>(a.sw + rows);
+    if (!a.walk) a.scales = reinterpret_cast<uint8_t*>(a.idx + rows);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const auto select = a.max_k <= 4096    ? mfa_kv8_select_kernel<4096>
                         : a.max_k <= 32768 ? mfa_kv8_select_kernel<32768>
                                            : mfa_kv8_select_kernel<0>;
     hipLaunchKernelGGL(select, dim3((unsigned)units), dim3(kSThreads), 0, st, a);
-    const unsigned grid = (unsigned)(units * a.blocks);
     typedef void (*fn)(E8Args);
     const auto of = [&](auto pick) { return a.D == 32 ? pick(std::integral_constant<int, 32>{}) : a.D == 64 ? pick(std::integral_constant<int, 64>{})
                                           : a.D == 96 ? pick(std::integral_constant<int, 96>{}) : pick(std::integral_constant<int, 128>{}); };
-    if (a.rows > 0) {
-        const fn save = of([](auto d) { return (fn)mfa_kv8_save_kernel<decltype(d)::value>; });
-        hipLaunchKernelGGL(save, dim3(grid, 2), dim3(kEThreads), 0, st, a);
+    if (a.walk) {
+        const fn walk = of([](auto d) { return (fn)mfa_kv8_walk_kernel<decltype(d)::value>; });
+        hipLaunchKernelGGL(walk, dim3((unsigned)units, 2), dim3(walk_threads(a.D)), 0, st, a);
+    } else {
+        const dim3 grid((unsigned)(units * a.blocks), 2);
+        if (a.rows > 0) {
+            const fn save = of([](auto d) { return (fn)mfa_kv8_save_kernel<decltype(d)::value>; });
+            hipLaunchKernelGGL(save, grid, dim3(kEThreads), 0, st, a);
+        }
+        const fn gather = of([](auto d) { return (fn)mfa_kv8_gather_kernel<decltype(d)::value>; });
+        hipLaunchKernelGGL(gather, grid, dim3(kEThreads), 0, st, a);
     }
-    const fn gather = of([](auto d) { return (fn)mfa_kv8_gather_kernel<decltype(d)::value>; });
-    hipLaunchKernelGGL(gather, dim3(grid, 2), dim3(kEThreads), 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e8err(MFA_ERR_LAUNCH, "mfa_kv8_evict: launch failed: %s", hipGetErrorString(e));
     return MFA_OK;

@@ -215,7 +215,7 @@ def kv8_evict(k_cache, v_cache, weights, cache_seqlens, block_table, budget, rec
     the table names); a tight bound keeps the selection short and, where the budget is
     not below it, the workspace empty.  A row on a page id outside the pool reads as
     zeros with weight 0.  The pool has less than 2^31 rows.  No two sequences may share a page that
-    changes.
+    changes; k_cache and v_cache are two caches.
     """
     budget, recent = int(budget), int(recent)
     max_seqlen_k = None if max_seqlen_k is None else int(max_seqlen_k)

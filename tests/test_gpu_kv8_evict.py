@@ -112,6 +112,37 @@ def test_nan_codes_move():
     check(kc, vc, w, lens, table, 130, 40)
 
 
+def test_zeros_of_large_scales():
+    """Rows of zeros from blocks of any scale make a block of the smallest scale: zeros still."""
+    kc, vc, w, lens, table = state([400, 130], 64, 2, 64)
+    for c in (kc, vc):
+        codes = c[0].view(torch.uint8)
+        codes &= 0x80
+        codes[:, ::9] = 0x70
+        c[1].copy_(torch.tensor([1, 100, 129, 200, 247], dtype=torch.uint8, device=DEV).repeat(99)[: c[1].shape[0]].view(-1, 1, 1))
+    w[:, ::9] = 0
+    check(kc, vc, w, lens, table, 128, 0)
+
+
+@pytest.mark.parametrize("batch", [16, 24])
+@pytest.mark.parametrize("D,page", [(32, 192), (64, 64), (96, 128), (128, 256)])
+def test_batches(batch, D, page):
+    """Many heads with much to move: ragged, some untouched, an odd budget, missing pages, odd weights."""
+    g = torch.Generator().manual_seed(batch + D)
+    lens = torch.randint(0, 1500, (batch,), generator=g).tolist()
+    for layout, kind in (("heads", "odd"), ("rows", "random")):
+        kc, vc, w, n, table = state(lens, page, 8, D, layout=layout, kind=kind)
+        table[1, :2], table[2, 1] = -1, 1 << 30
+        check(kc, vc, w, n, table, 611, 40)
+
+
+@pytest.mark.parametrize("kind", ["random", "ties", "falling"])
+@pytest.mark.parametrize("budget,recent", [(0, 0), (1, 1), (63, 5), (64, 0), (65, 64), (100, 100), (257, 20), (299, 1), (300, 0)])
+def test_budgets_of_batches(budget, recent, kind):
+    lens = [300, 1, 0, 64, 65, 129, 200, 299, 301, 270] * 4
+    check(*state(lens, 64, 2, 32, kind=kind), budget, recent)
+
+
 def test_again_on_a_stream_and_captured():
     """An eviction of what an eviction left; the same bits on another stream and in a graph."""
     args = state([900, 64, 500], 64, 2, 64, seed=3)

@@ -395,6 +395,7 @@ def test_c_evict(lib):
     refused(lib, lib.mfa_kv8_evict(ctypes.byref(p), None, need, None), -1, "workspace")
     refused(lib, lib.mfa_kv8_evict(ctypes.byref(p), 4096 + 16, need, None), -1, "aligned")
     refused(lib, lib.mfa_kv8_evict(ctypes.byref(p), 4096, need - 1, None), -1, "needed")
+    refused(lib, lib.mfa_kv8_evict(ctypes.byref(p), 4096, need, None), -1, "same memory")
     refused(lib, lib.mfa_kv8_evict(None, None, 0, None), -1, "NULL")
     p.batch = 0
     assert lib.mfa_kv8_evict(ctypes.byref(p), None, 0, None) == 0
