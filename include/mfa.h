@@ -525,7 +525,8 @@ int mfa_kv8_fwd_params_size(void);
  *                  + sum over query rows i and query heads h of hkv of exp(score_ihj - lse_ih)
  * for the keys j < Lk of every sequence with queries, Lq of them: keys before the
  * queries' own rows add to what they had, the queries' own start from 0.  What a row's
- * mask leaves out, and rows whose lse is -inf, add nothing.  weights: fp32
+ * mask leaves out, and rows whose lse is -inf, add nothing.  Sequences with queries must
+ * not share pages.  weights: fp32
  * [num_pages, page_block_size, heads_kv] by element strides (row and head strides >= 0),
  * addressed with the cache's block table; a page id outside the pool drops what is
  * written.  Sums in fp32, in an order that sizes alone decide; every key has one

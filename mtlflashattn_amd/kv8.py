@@ -120,11 +120,12 @@ def kv8_key_weights(q, k_cache, softmax_lse, weights, cache_seqlens, block_table
                 query rows i and the query heads of h,
     so keys before the queries' own rows add to what they had and the queries' own, new
     in this step, start from 0: the pool needs no clearing.  What a row's mask leaves out
-    adds nothing, and sequences without queries keep their weights.  The weights that the
+    adds nothing, and sequences without queries keep their weights.  Sequences with queries
+    must not share pages (a fork's weights need pages of their own).  The weights that the
     last rows of a prompt alone give come from a call with those rows and their
     log-sum-exps: then only those rows' own keys start from 0.
 
-    Sums in fp32, every key summed by one wavefront pair in an order that sizes alone
+    Sums in fp32, every key by one owner in an order that sizes and lengths alone
     decide; no synchronisation.  Any strides; each head's rows of a page side by side are
     read fastest.  Not differentiable: tensors that require grad raise.
     """
