@@ -100,4 +100,16 @@ __device__ __forceinline__ uint32_t quotient(uint32_t j, const FastDiv& f) {
     return f.d <= 1 ? j : __umulhi(j, f.m) >> f.s;
 }
 
+// inclusive prefix sum over the wavefront: shifts inside rows of 16 lanes, then the
+// last lanes of rows and of halves to what is behind them
+__device__ __forceinline__ int scan64(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
+    return x;
+}
+
 }  // namespace

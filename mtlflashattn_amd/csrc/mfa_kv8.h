@@ -86,6 +86,17 @@ __device__ __forceinline__ float kv8_top(uint32_t byte) { return byte < 247 ? 44
 // 2^(127 - byte), for bytes 1 .. 253
 __device__ __forceinline__ float kv8_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
+// Unsigned maximum of a wavefront, in lane 63
+__device__ __forceinline__ uint32_t max64(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false));  // row_shr:1, 2, 4, 8
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false));  // row_bcast:15 to rows 1 and 3
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false));  // row_bcast:31 to rows 2 and 3
+    return x;
+}
+
 // Four floats, at most 448 in magnitude or NaN, as four codes: the nearest values,
 // ties to the even code.
 __device__ __forceinline__ uint32_t kv8_round4(float a, float b, float c, float d) {

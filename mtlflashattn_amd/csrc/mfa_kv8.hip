@@ -1,10 +1,13 @@
 // mfa_kv8.hip -- writing a paged 8-bit K/V cache (mfa_kv8_append in include/mfa.h).
 //
-// Bound by memory for prompts, by the latency of dependent loads (prefix sums, page
-// id, old scale) for decoding steps.  A workgroup owns one block of 64 cache rows of
-// one head, in K or in V: it holds all of the call's rows that fall into the block in
-// registers (8 elements of a thread per load), takes their largest magnitude, and
-// writes codes, values and the scale; so no two workgroups share a scale.  Where the
+// Bound by memory for prompts (8 prompts of 256 to 4096 rows, 8 heads of 128, fp16: 39 us,
+// the copy rate), by the latency of dependent loads (prefix sums, page id, old scale) for
+// decoding steps (24 rows: 5 us, half of what the call takes on the host).  A workgroup
+// owns one block of 64 cache rows of one head, in K or in V: it takes the largest
+// magnitude of all of the call's rows that fall into the block (held in registers where
+// they fit, else read twice) and writes codes, values and the scale; so no two workgroups
+// share a scale.  Four wavefronts where blocks fill, one for the few rows of steps, whose
+// blocks are mostly latency: four times as many are on their way at once.  Where the
 // block holds rows already and the new ones raise its scale, their codes are rounded
 // again, at most 64 rows.  The scale comes from the maximum's exponent and mantissa
 // bits and the elements are multiplied by its inverse, a power of two, before the
@@ -22,7 +25,14 @@
 
 namespace {
 
-constexpr int kAThreads = 256;
+
+// A block is one wavefront's where a call has at most this many new rows per sequence on
+// average, and at least this many heads of sequences: fewer are on their way at once in
+// either form, and a full block takes a wavefront 12 us.
+// (8 K/V heads of 128, bf16, 256 sequences of 1, 16, 32 rows: 7.5, 13.1, 23.9 us against
+// 12.0, 21.5, 29.2; 64 sequences of 1 and 5: 4.9 and 5.2 against 5.5 and 7.0; 31 single
+// rows beside 400: 12.5 against 6.3, 255 beside 3000: 19.1 against 19.9.)
+constexpr int kStepRows = 16, kStepHeads = 2048;
 
 struct A8Args {
     const char* x[2];  // k, v
@@ -96,10 +106,11 @@ __device__ __forceinline__ void store_values8(char* p, u32x2_t codes, float s) {
     }
 }
 
-template <int DT, int D>
-__global__ void __launch_bounds__(kAThreads) mfa_kv8_append_kernel(A8Args a) {
-    constexpr int ES = DT == MFA_DTYPE_F32 ? 4 : 2, CPR = D / 8, NI = kKv8Block * CPR / kAThreads;
-    __shared__ uint32_t max_s[kAThreads / 64];
+template <int DT, int D, int T>
+__global__ void __launch_bounds__(T) mfa_kv8_append_kernel(A8Args a) {
+    constexpr int ES = DT == MFA_DTYPE_F32 ? 4 : 2, CPR = D / 8;
+    constexpr int ALL = kKv8Block * CPR / T, NI = ALL < 4 ? ALL : 4;  // loads of 64 rows, and of those held at once
+    __shared__ uint32_t max_s[T / 64];
     const int tid = threadIdx.x, lane = tid & 63, which = blockIdx.y;
     const int blk = (int)quotient(blockIdx.x, a.by_heads), h = (int)blockIdx.x - blk * a.H;
     char* const val = a.val[which] ? a.val[which] + (int64_t)h * D * ES : nullptr;
@@ -120,13 +131,7 @@ __global__ void __launch_bounds__(kAThreads) mfa_kv8_append_kernel(A8Args a) {
     // the sequence of block `blk`
     int b = -1, off = 0;
     for (int b0 = 0, base = 0; b0 < a.B && b < 0; b0 += 64) {
-        const int n = b0 + lane < a.B ? new_rows(a, b0 + lane).blocks() : 0;
-        int inc = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(inc, o);
-            if (lane >= o) inc += y;
-        }
+        const int n = b0 + lane < a.B ? new_rows(a, b0 + lane).blocks() : 0, inc = scan64(n);
         const uint64_t past = __ballot(inc + base > blk);
         if (past) {
             const int l = __builtin_ctzll(past);
@@ -145,11 +150,14 @@ __global__ void __launch_bounds__(kAThreads) mfa_kv8_append_kernel(A8Args a) {
     Raw8<DT> x[NI];
     uint32_t mx = 0;
     const char* const src = a.x[which] + (t0 * a.ts[which] + h * a.hs[which]) * ES;
+    auto load = [&](int first) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        const int u = tid + kAThreads * i, r = u / CPR, d = 8 * (u - r * CPR);
-        if (r < n) x[i].load(src + (r * a.ts[which] + d) * ES);
-    }
+        for (int i = 0; i < NI; ++i) {
+            const int u = first + tid + T * i, r = u / CPR, d = 8 * (u - r * CPR);
+            if (r < n) x[i].load(src + (r * a.ts[which] + d) * ES);
+        }
+    };
+    load(0);
     // the block's place (none: behind the table or on a page outside the pool)
     const Kv4Pool& p = a.pool[which];
     uint8_t *codes = nullptr, *scale = nullptr;
@@ -164,44 +172,51 @@ __global__ void __launch_bounds__(kAThreads) mfa_kv8_append_kernel(A8Args a) {
         }
     }
     // the largest finite magnitude
+    for (int first = 0; first < n * CPR; first += T * NI) {
+        if (first > 0) load(first);
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        if ((tid + kAThreads * i) / CPR < n) {
+        for (int i = 0; i < NI; ++i) {
+            if ((first + tid + T * i) / CPR < n) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t y = __float_as_uint(x[i].at(e)) & 0x7fffffffu;
-                mx = max(mx, y < 0x7f800000u ? y : 0u);
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t y = __float_as_uint(x[i].at(e)) & 0x7fffffffu;
+                    mx = max(mx, y < 0x7f800000u ? y : 0u);
+                }
             }
         }
+        if (NI == ALL) break;
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o));
-    if (lane == 0) max_s[tid >> 6] = mx;
+    mx = max64(mx);
+    if (lane == 63) max_s[tid >> 6] = mx;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kAThreads / 64; ++w) mx = max(mx, max_s[w]);
+    for (int w = 0; w < T / 64; ++w) mx = max(mx, max_s[w]);
     const uint32_t byte = max(kv8_byte_of(mx), old);
     const float inv = kv8_inverse(byte), sc = kv8_scale(byte), top = kv8_top(byte);
 
+    for (int first = 0; first < n * CPR; first += T * NI) {
+        if (n * CPR > T * NI) load(first);  // (else still held)
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        const int u = tid + kAThreads * i, r = u / CPR, d = 8 * (u - r * CPR);
-        if (r >= n) continue;
-        float y[8];
+        for (int i = 0; i < NI; ++i) {
+            const int u = first + tid + T * i, r = u / CPR, d = 8 * (u - r * CPR);
+            if (r >= n) continue;
+            float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float z = x[i].at(e);
-            y[e] = (__float_as_uint(z) & 0x7fffffffu) < 0x7f800000u ? __builtin_amdgcn_fmed3f(z * inv, -top, top) : __builtin_nanf("");
+            for (int e = 0; e < 8; ++e) {
+                const float z = x[i].at(e);
+                y[e] = (__float_as_uint(z) & 0x7fffffffu) < 0x7f800000u ? __builtin_amdgcn_fmed3f(z * inv, -top, top) : __builtin_nanf("");
+            }
+            const u32x2_t c = {kv8_round4(y[0], y[1], y[2], y[3]), kv8_round4(y[4], y[5], y[6], y[7])};
+            if (codes) *reinterpret_cast<u32x2_t*>(codes + (int64_t)(lo + r) * p.cr + d) = c;
+            if (val) store_values8<DT>(val + (t0 + r) * row_bytes + d * ES, c, sc);
         }
-        const u32x2_t c = {kv8_round4(y[0], y[1], y[2], y[3]), kv8_round4(y[4], y[5], y[6], y[7])};
-        if (codes) *reinterpret_cast<u32x2_t*>(codes + (int64_t)(lo + r) * p.cr + d) = c;
-        if (val) store_values8<DT>(val + (t0 + r) * row_bytes + d * ES, c, sc);
+        if (NI == ALL) break;
     }
     if (!codes) return;
     if (tid == 0) *scale = (uint8_t)byte;
     if (lo > 0 && byte > old) {  // the rows that were there, by the new scale
         const float f = kv8_scale(old) * inv;
-        for (int u = tid; u < lo * CPR; u += kAThreads) {
+        for (int u = tid; u < lo * CPR; u += T) {
             const int r = u / CPR;
             u32x2_t* q = reinterpret_cast<u32x2_t*>(codes + (int64_t)r * p.cr + 8 * (u - r * CPR));
             const u32x2_t c = *q;
@@ -222,10 +237,16 @@ int a8err(int code, const char* fmt, ...) {
 }
 
 typedef void (*a8_fn)(A8Args);
-template <int DT>
+template <int DT, int T>
 a8_fn append_of(int d) {
-    return d == 32 ? mfa_kv8_append_kernel<DT, 32> : d == 64 ? mfa_kv8_append_kernel<DT, 64>
-           : d == 96 ? mfa_kv8_append_kernel<DT, 96> : mfa_kv8_append_kernel<DT, 128>;
+    return d == 32 ? mfa_kv8_append_kernel<DT, 32, T> : d == 64 ? mfa_kv8_append_kernel<DT, 64, T>
+           : d == 96 ? mfa_kv8_append_kernel<DT, 96, T> : mfa_kv8_append_kernel<DT, 128, T>;
+}
+template <int T>
+a8_fn append_of(int dtype, int d) {
+    return dtype == MFA_DTYPE_F32    ? append_of<MFA_DTYPE_F32, T>(d)
+           : dtype == MFA_DTYPE_BF16 ? append_of<MFA_DTYPE_BF16, T>(d)
+                                     : append_of<MFA_DTYPE_F16, T>(d);
 }
 
 }  // namespace
@@ -277,10 +298,10 @@ int mfa_kv8_append(const mfa_kv8_append_params* p, void* stream) {
     const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(p->total, p->total / kKv8Block + 2 * (int64_t)p->batch));
     if (blocks * p->heads_kv > 0x7fffff) return a8err(MFA_ERR_INVALID, "mfa_kv8_append: problem too large");
     a.blocks = (int32_t)blocks;
-    const a8_fn fn = p->dtype == MFA_DTYPE_F32    ? append_of<MFA_DTYPE_F32>(p->head_dim)
-                     : p->dtype == MFA_DTYPE_BF16 ? append_of<MFA_DTYPE_BF16>(p->head_dim)
-                                                  : append_of<MFA_DTYPE_F16>(p->head_dim);
-    hipLaunchKernelGGL(fn, dim3((unsigned)(blocks * p->heads_kv), 2), dim3(kAThreads), 0, static_cast<hipStream_t>(stream), a);
+    const bool step = p->total <= kStepRows * (int64_t)p->batch && (int64_t)p->batch * p->heads_kv >= kStepHeads;
+    const int threads = step ? 64 : 256;
+    const a8_fn fn = step ? append_of<64>(p->dtype, p->head_dim) : append_of<256>(p->dtype, p->head_dim);
+    hipLaunchKernelGGL(fn, dim3((unsigned)(blocks * p->heads_kv), 2), dim3(threads), 0, static_cast<hipStream_t>(stream), a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return a8err(MFA_ERR_LAUNCH, "mfa_kv8_append: launch failed: %s", hipGetErrorString(e));
     return MFA_OK;

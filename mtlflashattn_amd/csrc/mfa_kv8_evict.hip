@@ -335,16 +335,6 @@ __device__ __forceinline__ uint32_t largest8(const u32x4_t& w, float s) {
     const uint32_t code = max(max((uint32_t)m[0], (uint32_t)m[1]), 1u) - 1;
     return __float_as_uint(__builtin_amdgcn_cvt_f32_fp8((int)code, 0) * s);
 }
-// Unsigned maximum of a wavefront, in lane 63
-__device__ __forceinline__ uint32_t max64(uint32_t x) {
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false));  // row_shr:1, 2, 4, 8
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false));
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false));
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false));
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false));  // row_bcast:15 to rows 1 and 3
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false));  // row_bcast:31 to rows 2 and 3
-    return x;
-}
 // 16 codes of scale s under a new byte.  Above 2^18 the factor only meets zeros and NaN (a
 // code is at least 2^-9, a new one at most 448), and an infinite one would make them NaN.
 __device__ __forceinline__ u32x4_t rounded8(const u32x4_t& w, float s, uint32_t byte) {

@@ -154,6 +154,26 @@ def test_many_sequences(nseq):
     mfa.kv8_append(k[:0], v[:0], *pools, cu_of([0] * nseq), i32(*old), table)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("H", [28, 30])
+def test_steps_of_many_heads(H, D, dtype):
+    """A block is a wavefront's from 2048 heads of sequences on: full blocks, few rows, rows that
+    raise the scale of those held, tokens of no sequence, missing pages, empty sequences."""
+    g = torch.Generator().manual_seed(D + H)
+    new = [3, 0, 70, 1, 130, 1, 2, 200, 17, 33] + [1, 0, 2, 1, 5, 1] * 10
+    old = torch.randint(0, 130, (len(new),), generator=g).tolist()
+    k, v = (torch.randn(sum(new) + 9, H, D, generator=g).mul(torch.exp(2 * torch.randn(sum(new) + 9, H, 1, generator=g))).to(DEV, dtype)
+            for _ in range(2))
+    pools = [filled_cache(g, 240, 64, H, D) for _ in range(2)]
+    table = table_of([a + b for a, b in zip(new, old)], 64, 240)
+    table[2, 0], table[4, 1], table[20, 0] = -1, 1 << 30, 240
+    cu = cu_of(new)
+    cu = cu + 4  # (rows in front and behind)
+    kv = check(pools, k, v, cu, i32(*old), table)
+    assert not kv[0][:4].any() and not kv[1][-5:].any()
+
+
 def test_input_and_cache_layouts():
     """Views of a packed projection, unaligned rows, expanded heads; caches with rows or pages in any order."""
     g = torch.Generator().manual_seed(4)
