@@ -11,9 +11,9 @@
 //
 // Two kernels, by the columns of a sequence, over chunks of 128 keys that are dealt as
 // in the attention (mfa_kv4_attend.hip):
-//  * at most 16: bound by the stream of K and the weights (136 bytes per key and head
+//  * at most 32: bound by the stream of K and the weights (136 bytes per key and head
 //    at head dim 128).  A wavefront takes every fourth 32-key block, the next one on
-//    its way into registers;
+//    its way into registers, and multiplies one or two tiles of 16 columns;
 //  * more: bound by the exponentials (24 cycles of a SIMD per 64 scores, against 16 of
 //    the products at head dim 128).  A wavefront holds 32 keys as operands and goes over
 //    the columns, 128 of which stand in LDS while the next are loaded straight into it;
@@ -53,27 +53,30 @@ __device__ __forceinline__ float neg_lse2(K4Const& a, bool in, int b, int q0, in
 
 // Scores to log2 units less the log-sum-exp, from the products s of one column.
 struct ScoreOf {
-    float scale, scale_log2, softcap;
+    float scale, scale_log2, softcap, softcap_sk;
     bool bias, alibi;
     __device__ __forceinline__ float operator()(float s, float sk, float nlse, float slope, int dist) const {
         if (!bias) return fmaf(s, scale_log2 * sk, nlse);
+        // (the soft-cap as the attention forms it, off by up to softcap 2^-21; tanh to the last
+        // bits made a chunk of 1024 rows over 8192 keys take 306 us instead of 199)
         float x = s * (scale * sk);
-        // (tanh to the last bits: the sums are fp32 results)
-        if (softcap > 0.f) x = softcap * precise_tanh(x / softcap);
+        if (softcap > 0.f) x = fmaf(-2.f * softcap, __builtin_amdgcn_rcpf(fast_exp2(s * (softcap_sk * sk)) + 1.f), softcap);
         if (alibi) x = fmaf(-slope, fabsf((float)dist), x);
         return fmaf(x, kLog2e, nlse);
     }
 };
 __device__ __forceinline__ ScoreOf score_of(K4Const& a) {
-    return ScoreOf{a.scale, a.scale_log2, a.softcap, a.bias != 0, a.alibi != nullptr};
+    return ScoreOf{a.scale, a.scale_log2, a.softcap, a.softcap_sk, a.bias != 0, a.alibi != nullptr};
 }
 
-// (32 sequences of 512 to 8192 keys, Hq=32 Hkv=8 D=128 bf16: 35.3 us with three
-// workgroups per CU, 35.5 with five, 51 with six, which spill; two blocks ahead instead
-// of one: 35.7.  Of that about 11 us pass before the stream runs and after it ends.)
-constexpr int kFewWgs = 3;
-template <int DP, bool IS_BF16>
-__global__ void __launch_bounds__(kThreads4) __attribute__((amdgpu_waves_per_eu(kFewWgs)))
+// (32 sequences of 512 to 8192 keys, Hq=32 Hkv=8 D=128 bf16: 34.9 us with three
+// workgroups per CU, 37.4 with two, 35.5 with five; two blocks ahead instead of one: 35.7.
+// Of that about 11 us pass before the stream runs and after it ends.  64 sequences of 5 rows
+// over 8192: two tiles of columns 122 us, 133 with three workgroups, 198 by the kernel for
+// more columns.)
+constexpr int few_wgs(int nt) { return nt == 1 ? 3 : 2; }
+template <int DP, bool IS_BF16, int NT>
+__global__ void __launch_bounds__(kThreads4) __attribute__((amdgpu_waves_per_eu(few_wgs(NT))))
 mfa_kv8_weights_few_kernel(K4Args) {
     typedef op_of<IS_BF16> op_t;
     typedef KeyBlock8<DP> Blk;
@@ -113,52 +116,60 @@ mfa_kv8_weights_few_kernel(K4Args) {
             blk.w = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(pg.rs[2], blk.at, 0, 0));
             blk.rs = pg.rs[2];
         };
-        // queries: lane (column l16, group grp) holds elements Blk::element(grp, s) .. + 7;
-        // the products' registers are columns 4 grp + e
-        op_t qf[KS];
-        float nlse[4], slope[4];
-        int lo[4], hi[4], center[4];
-        {
-            const int i = (int)div4(l16, a.by_r), h = wk.hkv * a.R + l16 - i * a.R;
-            const bool in = l16 < wk.ncol;
+        // queries: lane (column 16 t + l16, group grp) holds elements Blk::element(grp, s) .. + 7;
+        // the products' registers are columns 16 t + 4 grp + e
+        op_t qf[NT][KS];
+        float nlse[NT][4], slope[NT][4];
+        int lo[NT][4], hi[NT][4], center[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int mine = 16 * t + l16, i = (int)div4(mine, a.by_r), h = wk.hkv * a.R + mine - i * a.R;
+            const bool in = mine < wk.ncol;
             const char* q = a.q + row_off4(a.cu_q != nullptr, wk.b, wk.sq.q0, in ? i : 0, in ? h : 0, a.qb, a.qs, a.qh) * 2;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 u32x4_t w = {0, 0, 0, 0};
                 if (in) w = *reinterpret_cast<const u32x4_t*>(q + Blk::element(grp, s) * 2);
-                qf[s] = __builtin_bit_cast(op_t, w);
+                qf[t][s] = __builtin_bit_cast(op_t, w);
             }
-        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int col = 4 * grp + e, i = (int)div4(col, a.by_r), h = wk.hkv * a.R + col - i * a.R;
-            const bool in = col < wk.ncol;
-            center[e] = i + dq;
-            lo[e] = lo4(a.wl, center[e]);
-            hi[e] = in ? hi4(a.causal, a.wr, center[e], Lk) : -1;
-            nlse[e] = neg_lse2(a, in, wk.b, wk.sq.q0, i, h);
-            slope[e] = score.alibi && in ? a.alibi[wk.b * a.alibi_bstride + h] : 0.f;
+            for (int e = 0; e < 4; ++e) {
+                const int col = 16 * t + 4 * grp + e, ie = (int)div4(col, a.by_r), he = wk.hkv * a.R + col - ie * a.R;
+                const bool some = col < wk.ncol;
+                center[t][e] = ie + dq;
+                lo[t][e] = lo4(a.wl, center[t][e]);
+                hi[t][e] = some ? hi4(a.causal, a.wr, center[t][e], Lk) : -1;
+                nlse[t][e] = neg_lse2(a, some, wk.b, wk.sq.q0, ie, he);
+                slope[t][e] = score.alibi && some ? a.alibi[wk.b * a.alibi_bstride + he] : 0.f;
+            }
         }
         load(0);
         // (waited for here: a wait inside the loop would drain the codes' loads too)
 #pragma unroll
-        for (int s = 0; s < KS; ++s) pin(qf[s]);
+        for (int t = 0; t < NT; ++t) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            pin(nlse[e]);
-            pin(slope[e]);
+            for (int s = 0; s < KS; ++s) pin(qf[t][s]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                pin(nlse[t][e]);
+                pin(slope[t][e]);
+            }
         }
         for (int n = 0; n < n1; ++n) {
             const int j = key0 + n * kChunk4;
-            f32x4_t st[2];
+            f32x4_t st[NT][2];
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
-                st[kk] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int t = 0; t < NT; ++t) st[t][kk] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
                     const op_t kf = blk.k.template k_operand<op_t>(kk, s, grp);
-                    if constexpr (IS_BF16) st[kk] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[s], kf, st[kk], 0, 0, 0);
-                    else st[kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[s], kf, st[kk], 0, 0, 0);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        if constexpr (IS_BF16) st[t][kk] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qf[t][s], kf, st[t][kk], 0, 0, 0);
+                        else st[t][kk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qf[t][s], kf, st[t][kk], 0, 0, 0);
+                    }
                 }
             }
             const float sk = blk.k.k_scale(), old = j + lane < dq ? blk.w : 0.f;
@@ -170,13 +181,18 @@ mfa_kv8_weights_few_kernel(K4Args) {
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
                 const int key = j + 16 * kk + l16;
-                float p[4];
+                float all = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    p[e] = fast_exp2(score(st[kk][e], sk, nlse[e], slope[e], center[e] - key));
-                    if (masked) p[e] = ((key >= lo[e]) & (key <= hi[e])) ? p[e] : 0.f;
+                for (int t = 0; t < NT; ++t) {
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        p[e] = fast_exp2(score(st[t][kk][e], sk, nlse[t][e], slope[t][e], center[t][e] - key));
+                        if (masked) p[e] = ((key >= lo[t][e]) & (key <= hi[t][e])) ? p[e] : 0.f;
+                    }
+                    all += (p[0] + p[1]) + (p[2] + p[3]);
                 }
-                sum[kk] = sum_groups4((p[0] + p[1]) + (p[2] + p[3]));
+                sum[kk] = sum_groups4(all);
             }
             // lane 16 kk + l16 has the sum of its own key
             const float w = old + (grp & 1 ? sum[1] : sum[0]);
@@ -398,18 +414,19 @@ mfa_kv8_weights_many_kernel(K4Args) {
 }
 
 typedef void (*w8_fn)(K4Args);
-template <int DP>
-w8_fn weights_of(bool few, bool bf16, bool bias) {
-    if (few) return bf16 ? (w8_fn)mfa_kv8_weights_few_kernel<DP, true> : (w8_fn)mfa_kv8_weights_few_kernel<DP, false>;
-    if (bias) return bf16 ? (w8_fn)mfa_kv8_weights_many_kernel<DP, true, true> : (w8_fn)mfa_kv8_weights_many_kernel<DP, false, true>;
-    return bf16 ? (w8_fn)mfa_kv8_weights_many_kernel<DP, true, false> : (w8_fn)mfa_kv8_weights_many_kernel<DP, false, false>;
+// few: 16-column tiles of the kernel for few columns, 0: the other
+template <int DP, bool IS_BF16>
+w8_fn weights_of(int few, bool bias) {
+    return few == 1 ? mfa_kv8_weights_few_kernel<DP, IS_BF16, 1> : few == 2 ? mfa_kv8_weights_few_kernel<DP, IS_BF16, 2>
+           : bias   ? mfa_kv8_weights_many_kernel<DP, IS_BF16, true> : mfa_kv8_weights_many_kernel<DP, IS_BF16, false>;
 }
-w8_fn weights_of(int dp, bool few, bool bf16, bool bias) {
+template <bool IS_BF16>
+w8_fn weights_of(int dp, int few, bool bias) {
     switch (dp) {
-        case 32: return weights_of<32>(few, bf16, bias);
-        case 64: return weights_of<64>(few, bf16, bias);
-        case 96: return weights_of<96>(few, bf16, bias);
-        default: return weights_of<128>(few, bf16, bias);
+        case 32: return weights_of<32, IS_BF16>(few, bias);
+        case 64: return weights_of<64, IS_BF16>(few, bias);
+        case 96: return weights_of<96, IS_BF16>(few, bias);
+        default: return weights_of<128, IS_BF16>(few, bias);
     }
 }
 
@@ -447,8 +464,8 @@ int mfa_kv8_weights(const mfa_kv8_weights_params* p, void* stream) {
         return w8err(MFA_ERR_INVALID, "%s: the rows of a page must span less than 2 GiB", who);
     a.v = Kv4Pool{reinterpret_cast<uint8_t*>(p->weights), nullptr, p->weight_page_stride * 4, p->weight_row_stride * 4,
                   p->weight_head_stride * 4, 0, 0, 0};
-    // Sequences of at most 16 columns, then those of more (a varlen call's are known on
-    // the device only: both)
+    // Sequences of few columns, then those of more (a varlen call's are known on the device
+    // only: both)
     const bool varlen = f.cu_seqlens_q != nullptr;
     const int64_t cols = (varlen ? (int64_t)a.rows_q : f.seqlen_q) * (int64_t)a.R;
     const int64_t chunks = std::max<int64_t>(1, ((int64_t)a.max_k + kChunk4 - 1) / kChunk4);
@@ -456,17 +473,20 @@ int mfa_kv8_weights(const mfa_kv8_weights_params* p, void* stream) {
     if (cols > 0x3fffffff || units > 0x3fffffff || units * chunks > 0x7fffffffLL)
         return w8err(MFA_ERR_INVALID, "%s: problem too large", who);
     const int cus = mfa_chip_cus(stream);
-    for (int few = 1; few >= 0; --few) {
-        if (few ? !varlen && cols > 16 : cols <= 16) continue;
-        a.cols = few ? 16 : 0x3fffffff;  // (one unit per sequence and K/V head)
-        a.min_cols = few ? 1 : 17;
-        a.max_cols = few ? 16 : 0x7fffffff;
-        a.G = (int32_t)std::min<int64_t>(units * chunks, (int64_t)cus * (few ? kFewWgs : kManyWgs));
+    // (a varlen call's tiles by the mean of its sequences)
+    const int nt = (varlen ? cols > 16 * (int64_t)f.batch : cols > 16) ? 2 : 1;
+    for (int few = nt; few >= 0; few -= nt) {
+        if (few ? !varlen && cols > 16 * nt : cols <= 16 * nt) continue;
+        a.cols = few ? 16 * few : 0x3fffffff;  // (one unit per sequence and K/V head)
+        a.min_cols = few ? 1 : 16 * nt + 1;
+        a.max_cols = few ? 16 * few : 0x7fffffff;
+        a.G = (int32_t)std::min<int64_t>(units * chunks, (int64_t)cus * (few ? few_wgs(few) : kManyWgs));
         // (pieces: at most one more of each unit than its share)
         int64_t grid = few ? a.G : std::min<int64_t>(units * chunks, a.G + units);
         if (!few) grid = (grid + 7) / 8 * 8;
         a.xcds = 1;
-        const w8_fn fn = weights_of(f.head_dim, few != 0, f.dtype == MFA_DTYPE_BF16, a.bias != 0);
+        const bool bias = a.bias != 0;
+        const w8_fn fn = f.dtype == MFA_DTYPE_BF16 ? weights_of<true>(f.head_dim, few, bias) : weights_of<false>(f.head_dim, few, bias);
         hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(few ? kThreads4 : kManyThreads), 0, static_cast<hipStream_t>(stream), a);
     }
     const hipError_t e = hipGetLastError();

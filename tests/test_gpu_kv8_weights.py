@@ -3,8 +3,8 @@
 Bounds: a probability exp(s - lse) is off by its exponent's error, and the sums by theirs.
 Scores are fp32 sums of exact products (|ds| <= 2^-22 sum |q k| scale, the sum below 100:
 2.4e-5); lse in log2 units, the score's scaling and their difference round three numbers
-below 64 to 2^-24 each (1.2e-5 together); the soft-cap adds 2^-22 of its bound (at most
-8: 2e-6) and ALiBi two roundings of terms below 256 (3.1e-5); exp2 is within 2^-23.  That is less than
+below 64 to 2^-24 each (1.2e-5 together); the soft-cap adds 2^-21 of its bound (at most
+8: 4e-6) and ALiBi two roundings of terms below 256 (3.1e-5); exp2 is within 2^-23.  That is less than
 8e-5 of every probability, hence of their sum; adding n of them in fp32 costs at most n
 2^-24 of it, the old weight one more rounding.
 """
@@ -99,6 +99,16 @@ def test_alibi(lq, per_batch):
     if per_batch:
         slopes = torch.stack((slopes, slopes.flip(0)))
     run_and_check([400, 77], [lq] * 2, 64, 4, 2, 128, torch.float16, causal=True, slopes=slopes)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(causal=True), dict(causal=True, window_size=(100, -1)), dict(window_size=(30, 20)), dict(causal=True, softcap=2.0),
+    dict(causal=True, slopes=torch.tensor([0.5, 0.01, 0.3, 0.0, 0.1, 0.2])),
+])
+@pytest.mark.parametrize("D,dtype", [(32, torch.float16), (64, torch.bfloat16), (96, torch.bfloat16), (128, torch.float16)])
+def test_two_tiles_of_columns(D, dtype, kw):
+    run_and_check([7, 900, 513], [7] * 3, 64, 6, 2, D, dtype, **kw)
+    run_and_check([10, 900, 513, 64, 33, 300], [10, 11, 1, 0, 33, 8], 64, 6, 2, D, dtype, **kw)
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.2, 0.3])
