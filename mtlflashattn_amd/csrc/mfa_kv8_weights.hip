@@ -206,12 +206,17 @@ constexpr int kManyWgs = 2, kManyThreads = 512;  // (workgroups per CU: what the
 // A workgroup's piece of the work: consecutive chunks of one unit (a sequence and K/V
 // head).  The units' chunks are cut into pieces of at most ceil(chunks of all units /
 // G), the same for all of a unit to one chunk, so that no workgroup pays the latency
-// of a second unit's queries and pages.
+// of a second unit's queries and pages.  Where all chunks leave half of the workgroups
+// without one, pieces of sequences with many columns are halves of a chunk (a prompt of
+// 2048 rows over themselves, Hq=32 Hkv=8 D=128: 158 us by chunks, 118 by halves, 120 by
+// quarters; 4 sequences of 9 rows over 1000: 8.1 and 10.6).
+constexpr int kHalfCols = 256;
 struct Piece4 {
-    int b, hkv, c0, nch;
+    int b, hkv, c0, nch, part, parts;  // part: of `parts` of one chunk
     Seq4 sq;
-    // pieces of at most `most` chunks of a sequence
+    // pieces of at most `most` chunks of a sequence, a chunk in `parts`
     static __device__ __forceinline__ int pieces(const Seq4& s, int most) { return (s.chunks + most - 1) / most; }
+    static __device__ __forceinline__ int parts_of(const Seq4& s, int R, bool half) { return half && s.Lq * R >= kHalfCols ? 2 : 1; }
     __device__ __forceinline__ bool find(K4Const& a) {
         const int lane = threadIdx.x & 63, B = a.B, H = a.Hkv;
         auto seq = [&](int b0) { return b0 + lane < B ? seq4(a, b0 + lane) : Seq4{0, 0, 0, 0, 1}; };
@@ -219,10 +224,11 @@ struct Piece4 {
         int all = __builtin_amdgcn_readlane(scan64(s.items(H)), 63);
         for (int b0 = 64; b0 < B; b0 += 64) all += __builtin_amdgcn_readlane(scan64(seq(b0).items(H)), 63);
         const int most = max((all + a.G - 1) / a.G, 1);
-        int n = s.tiles * H * pieces(s, most), inc = scan64(n), total = __builtin_amdgcn_readlane(inc, 63);
+        const bool half = all <= a.G / 2;
+        auto of = [&](const Seq4& y) { return y.tiles * H * pieces(y, most) * parts_of(y, a.R, half); };
+        int n = of(s), inc = scan64(n), total = __builtin_amdgcn_readlane(inc, 63);
         for (int b0 = 64; b0 < B; b0 += 64) {
-            const Seq4 y = seq(b0);
-            total += __builtin_amdgcn_readlane(scan64(y.tiles * H * pieces(y, most)), 63);
+            total += __builtin_amdgcn_readlane(scan64(of(seq(b0))), 63);
         }
         // neighbouring pieces, which share their queries, on one XCD
         const int per = (total + 7) / 8, w = blockIdx.x % 8 * per + blockIdx.x / 8;
@@ -233,9 +239,11 @@ struct Piece4 {
                 const int l = __builtin_ctzll(past);
                 b = b0 + l;
                 sq = lane_seq4(s, l);
-                const int at = w - base - __builtin_amdgcn_readlane(inc - n, l), np = pieces(sq, most);
-                hkv = at / np;
-                const int k = at - hkv * np;
+                parts = parts_of(sq, a.R, half);
+                const int at = w - base - __builtin_amdgcn_readlane(inc - n, l), np = pieces(sq, most), nx = np * parts;
+                hkv = at / nx;
+                const int kx = at - hkv * nx, k = kx / parts;
+                part = kx - k * parts;
                 c0 = first_item(k, sq.chunks, np);
                 nch = first_item(k + 1, sq.chunks, np) - c0;
                 return true;
@@ -244,7 +252,7 @@ struct Piece4 {
             b0 += 64;
             if (b0 >= B) return false;
             s = seq(b0);
-            n = s.tiles * H * pieces(s, most);
+            n = of(s);
             inc = scan64(n);
         }
     }
@@ -287,7 +295,9 @@ mfa_kv8_weights_many_kernel(K4Args) {
         // ---- some chunks: blocks of 32 keys, dealt over the wavefronts; where there are
         // fewer than wavefronts, two or four share one and take every second or fourth 32
         // columns
-        const int j0 = c0 * kChunk4, jend = min(min(c0 + kWChunks, ch.end) * kChunk4, Lk);
+        const int keys = wk.parts > 1 ? kChunk4 / 2 : kWChunks * kChunk4;
+        const int j0 = c0 * kChunk4 + wk.part * keys, jend = min(min(ch.end * kChunk4, j0 + keys), Lk);
+        if (j0 >= jend) break;
         const int nb = (jend - j0 + 31) / 32, cw = nb <= kWaves / 4 ? 4 : nb <= kWaves / 2 ? 2 : 1, kw = kWaves / cw;
         const int cg = wave / kw, b0 = wave - cg * kw;
         typename Blk::Offsets off;
@@ -480,9 +490,10 @@ int mfa_kv8_weights(const mfa_kv8_weights_params* p, void* stream) {
         a.cols = few ? 16 * few : 0x3fffffff;  // (one unit per sequence and K/V head)
         a.min_cols = few ? 1 : 16 * nt + 1;
         a.max_cols = few ? 16 * few : 0x7fffffff;
-        a.G = (int32_t)std::min<int64_t>(units * chunks, (int64_t)cus * (few ? few_wgs(few) : kManyWgs));
+        const int64_t most = units * chunks * (few ? 1 : 2);  // (halves of chunks)
+        a.G = (int32_t)std::min<int64_t>(most, (int64_t)cus * (few ? few_wgs(few) : kManyWgs));
         // (pieces: at most one more of each unit than its share)
-        int64_t grid = few ? a.G : std::min<int64_t>(units * chunks, a.G + units);
+        int64_t grid = few ? a.G : std::min<int64_t>(most, a.G + units);
         if (!few) grid = (grid + 7) / 8 * 8;
         a.xcds = 1;
         const bool bias = a.bias != 0;
