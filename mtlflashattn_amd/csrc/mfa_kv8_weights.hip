@@ -208,7 +208,7 @@ constexpr int kManyWgs = 2, kManyThreads = 512;  // (workgroups per CU: what the
 // G), the same for all of a unit to one chunk, so that no workgroup pays the latency
 // of a second unit's queries and pages.  Where all chunks leave half of the workgroups
 // without one, pieces of sequences with many columns are halves of a chunk (a prompt of
-// 2048 rows over themselves, Hq=32 Hkv=8 D=128: 158 us by chunks, 118 by halves, 120 by
+// 2048 rows over themselves, Hq=32 Hkv=8 D=128: 158 us by chunks, 108 by halves, 110 by
 // quarters; 4 sequences of 9 rows over 1000: 8.1 and 10.6).
 constexpr int kHalfCols = 256;
 struct Piece4 {
@@ -288,6 +288,12 @@ mfa_kv8_weights_many_kernel(K4Args) {
     ScoreOf score = score_of(a);
     score.bias = BIAS;
     const FastDiv by_r = {a.by_r.d, a.by_r.m, a.by_r.s};
+    // (what columns are looked up with: read from the arguments in the loop, each is a latency)
+    const int R = a.R;
+    const char* const q_0 = a.q + row_off4(a.cu_q != nullptr, wk.b, wk.sq.q0, 0, wk.hkv * R, a.qb, a.qs, a.qh) * 2;
+    const int64_t q_i = a.qs * 2, q_h = a.qh * 2, lse_h = a.lse_h;
+    const float* const lse_0 = a.lse + (a.cu_q ? (int64_t)wk.sq.q0 : wk.b * a.lse_b) + wk.hkv * R * lse_h;
+    const float* const alibi_0 = BIAS && a.alibi ? a.alibi + wk.b * a.alibi_bstride + wk.hkv * R : nullptr;
     const int i_last = wk.sq.Lq - 1;
     const int t_lo = lo4(wl, dq), t_hi = hi4(causal, wr, i_last + dq, Lk);
     const Chunks4 ch = chunks4(t_lo, t_hi, wk.c0, wk.nch);
@@ -319,7 +325,7 @@ mfa_kv8_weights_many_kernel(K4Args) {
         if (causal) i0 = max(i0, j0 - dq);
         if (wr >= 0) i0 = (int)max((int64_t)i0, (int64_t)j0 - wr - dq);
         if (wl >= 0) i1 = (int)min((int64_t)i1, (int64_t)jend + wl - dq);
-        const int cbeg = i0 < i1 ? i0 * a.R / 32 * 32 : 0, cend = i0 < i1 ? i1 * a.R : 0;
+        const int cbeg = i0 < i1 ? i0 * R / 32 * 32 : 0, cend = i0 < i1 ? i1 * R : 0;
         const int n = (cend - cbeg + kWCols - 1) / kWCols;  // tiles of columns
         // Step k brings tile k in, works on tile k - 1 and looks up the columns of tile k + 1.
         // (Every part stands here once: what is run once costs the fetch of its code.)
@@ -392,18 +398,18 @@ mfa_kv8_weights_many_kernel(K4Args) {
             }
             if (k + 1 < n && tid < kWCols) {
                 // (columns behind the last repeat it, with a log-sum-exp that leaves them out)
-                K4Const& e = args4();
                 const int to = (k + 1) % 3, mine = cbeg + (k + 1) * kWCols + tid, col = min(mine, cend - 1);
-                const int i = (int)quotient(col, by_r), h = wk.hkv * e.R + col - i * e.R, c = i + dq;
-                const float nl = neg_lse2(e, mine < cend, wk.b, wk.sq.q0, i, h);
-                row_s[to][tid] = e.q + row_off4(e.cu_q != nullptr, wk.b, wk.sq.q0, i, h, e.qb, e.qs, e.qh) * 2;
+                const int i = (int)quotient(col, by_r), h = col - i * R, c = i + dq;
+                const float l = lse_0[i + h * lse_h];
+                row_s[to][tid] = q_0 + (i * q_i + h * q_h);
                 lo_s[to][tid] = lo4(wl, c);
                 if constexpr (BIAS) {
                     center_s[to][tid] = c;
-                    slope_s[to][tid] = score.alibi ? e.alibi[wk.b * e.alibi_bstride + h] : 0.f;
+                    slope_s[to][tid] = score.alibi ? alibi_0[h] : 0.f;
                 }
-                nlse_s[to][tid] = nl;
-                hi_s[to][tid] = nl == -INFINITY ? -1 : hi4(causal, wr, c, Lk);
+                const bool sees = mine < cend && l != -INFINITY;
+                nlse_s[to][tid] = sees ? -l * kLog2e : -INFINITY;
+                hi_s[to][tid] = sees ? hi4(causal, wr, c, Lk) : -1;
             }
             wait_vm<0>();
         }
