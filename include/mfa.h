@@ -506,7 +506,9 @@ int mfa_kv8_append(const mfa_kv8_append_params* params, void* stream);
 int mfa_kv8_append_params_size(void);
 
 /*
- * Attention over the cache: the parameters and rules of mfa_kv4_fwd.  A NaN element of
+ * Attention over the cache: the parameters and rules of mfa_kv4_fwd; a varlen call whose
+ * sequences have 17 to 32 columns on average takes those of up to 32 as a fixed call
+ * does, so with two terms of the probabilities.  A NaN element of
  * V reaches only the rows whose mask holds its key.  K is exact; V is exact with bf16
  * queries and for at most 32 columns; on the tiles of 128 columns fp16 queries take V
  * rounded to fp16 (elements beyond +/-65504 saturate, those of scales below 2^-15 may

@@ -307,6 +307,7 @@ struct MfaKvFormat {
     int rows_wgs[2];                                // workgroups per CU of the kernels of 16 and 32 columns
     int tile_wgs;                                   // ... of 128
     float least_scale;                              // softmax scales up to here take the path that scales before it masks
+    bool varlen32;                                  // varlen calls of 17 to 32 columns per sequence on average take the kernel of 32
     void* (*rows_kernel)(int dp, int cols, bool bf16);   // void(*)(K4Args), for 16 or 32 columns
     void* (*tile_kernel)(int dp, bool bf16, bool bias);  // ... for 128
 };

@@ -369,20 +369,21 @@ int k4_plan(const mfa_kv4_fwd_params* p, const MfaKvFormat& f, K4Plan* plan, int
 
     // Columns per workgroup: a sequence's, at most 128.  The sequences of a
     // varlen call are known on the device only: one launch takes those of at most
-    // 16 columns, another the longer ones.
+    // 16 columns (32 by the mean, where the format says so), another the longer ones.
     // (no sequences: the launch only clears the rows)
     const int64_t cols = p->batch == 0 ? 1 : (varlen ? rows : p->seqlen_q) * (int64_t)a.R;
     plan->n = varlen && cols > 16 ? 2 : 1;
+    const int few = f.varlen32 && cols > 16 * (int64_t)p->batch && cols <= 32 * (int64_t)p->batch ? 32 : 16;
     const int64_t chunks = p->batch == 0 ? 1 : std::max<int64_t>(1, ((int64_t)a.max_k + kChunk4 - 1) / kChunk4);
     for (int i = 0; i < plan->n; ++i) {
         K4Launch& l = plan->l[i];
         l.a = a;
-        l.a.cols = unit_cols(plan->n == 2 && i == 0 ? 16 : cols);
-        l.a.min_cols = i == 0 ? 1 : 17;
-        l.a.max_cols = plan->n == 2 && i == 0 ? 16 : 0x7fffffff;
+        l.a.cols = unit_cols(plan->n == 2 && i == 0 ? few : cols);
+        l.a.min_cols = i == 0 ? 1 : few + 1;
+        l.a.max_cols = plan->n == 2 && i == 0 ? few : 0x7fffffff;
         // (a bound on the items, which are counted on the device in int32)
         const int64_t tiles = !varlen       ? p->batch * ((cols + l.a.cols - 1) / l.a.cols)
-                              : l.a.max_cols == 16 ? std::min<int64_t>(p->batch, rows)
+                              : l.a.max_cols == few ? std::min<int64_t>(p->batch, rows)
                                                    : (cols + l.a.cols - 1) / l.a.cols + std::min<int64_t>(p->batch, rows);
         const int64_t units = tiles * a.Hkv;
         if (units > 0x3fffffff || units * chunks > 0x7fffffffLL) return k4err(MFA_ERR_INVALID, "%s: problem too large", f.who);
@@ -412,7 +413,7 @@ void* rows_kernel4(int dp, int cols, bool bf16) {
         default: return rows4<128>(cols, bf16);
     }
 }
-const MfaKvFormat kFormat4 = {"mfa_kv4_fwd", {wgs4(1), wgs4(2)}, 2, 0.f, rows_kernel4, mfa_kv4_tile_kernel_of};
+const MfaKvFormat kFormat4 = {"mfa_kv4_fwd", {wgs4(1), wgs4(2)}, 2, 0.f, false, rows_kernel4, mfa_kv4_tile_kernel_of};
 
 }  // namespace
 

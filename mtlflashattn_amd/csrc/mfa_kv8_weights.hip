@@ -208,8 +208,8 @@ constexpr int kManyWgs = 2, kManyThreads = 512;  // (workgroups per CU: what the
 // G), the same for all of a unit to one chunk, so that no workgroup pays the latency
 // of a second unit's queries and pages.  Where all chunks leave half of the workgroups
 // without one, pieces of sequences with many columns are halves of a chunk (a prompt of
-// 2048 rows over themselves, Hq=32 Hkv=8 D=128: 158 us by chunks, 108 by halves, 110 by
-// quarters; 4 sequences of 9 rows over 1000: 8.1 and 10.6).
+// 2048 rows over themselves, Hq=32 Hkv=8 D=128: 158 us by chunks, 118 by halves, now 108,
+// and 120 by quarters; 4 sequences of 9 rows over 1000: 8.1 by chunks, 10.6 by halves).
 constexpr int kHalfCols = 256;
 struct Piece4 {
     int b, hkv, c0, nch, part, parts;  // part: of `parts` of one chunk

@@ -69,7 +69,8 @@ def flash_attn_kv8_func(q, k_cache, v_cache, cache_seqlens, block_table, softmax
     over another format, with its arguments, masks, limits and results.
 
     K is exact; so is V, except on the tiles of 128 columns (sequences of more than 32
-    columns) with fp16 queries, where it is rounded to fp16 (beyond 65504 it saturates;
+    columns; in a varlen call of more than 32 in total, of more than 16, but not where its
+    sequences have 17 to 32 on average) with fp16 queries, where it is rounded to fp16 (beyond 65504 it saturates;
     scales below 2^-15 may lose bits).  NaN elements reach only the rows whose mask
     holds their key.
     """

@@ -73,6 +73,21 @@ def test_drafted_tokens(D, lq, dtype):
     run_and_check([lq, 300, 41, 1000], [lq] * 4, 128, 6, 2, D, dtype, causal=True)
 
 
+@pytest.mark.parametrize("D,dtype", [(32, torch.float16), (64, torch.bfloat16), (96, torch.float16), (128, torch.bfloat16)])
+def test_drafts_in_a_varlen_call(D, dtype):
+    """17 to 32 columns per sequence on average: the kernel of 32 columns, with the bits of the fixed
+    call; longer sequences among them run on tiles of 128."""
+    lq, R = 5, 4
+    lens = [5, 300, 41, 1000, 2000, 64]
+    q, kc, vc, lens_t, table = make(lens, 64, 8, 2, D, dtype, [lq] * 6)
+    fixed = mfa.flash_attn_kv8_func(q.view(6, lq, 8, D), kc, vc, lens_t, table, causal=True)
+    packed = mfa.flash_attn_varlen_kv8_func(q, kc, vc, cu_of([lq] * 6), lens_t, table, causal=True)
+    assert torch.equal(fixed.flatten(0, 1), packed)
+    for mixed in ([5, 8, 0, 1, 9, 12, 5], [8, 8, 8], [1, 15], [5, 5, 5, 5, 1, 20]):
+        assert 16 < sum(mixed) * R / len(mixed) <= 32
+        run_and_check([max(n, 1) + 333 * (i % 3) for i, n in enumerate(mixed)], mixed, 64, 8, 2, D, dtype, causal=True)
+
+
 @pytest.mark.parametrize("kw", [
     dict(), dict(causal=True), dict(causal=True, window_size=(100, -1)), dict(window_size=(30, 20)),
     dict(window_size=(0, 0)), dict(window_size=(-1, 3)), dict(causal=True, softcap=2.0),
