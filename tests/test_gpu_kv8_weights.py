@@ -247,3 +247,50 @@ def test_page_ids_outside_the_pool():
     used[table[0, 1], :36] = True
     used[table[1, 0]] = True
     assert bool((w[~used] == 1).all()) and bool((w[used] != 1).any())
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(softcap=4.0), dict(window_size=(2500, -1))])
+@pytest.mark.parametrize("D", [32, 96])
+def test_many_chunks_of_many_heads(D, kw):
+    """More chunks than workgroups: several per workgroup, several blocks of keys per wavefront, the
+    sums of some chunks after those of others; beside a sequence of few columns."""
+    run_and_check([6400, 3001], [40, 24], 64, 48, 48, D, torch.bfloat16, causal=True, **kw)
+    run_and_check([6400, 3001], [40, 3], 64, 48, 48, D, torch.bfloat16, causal=True, **kw)
+
+
+@pytest.mark.parametrize("lq", [1, 6, 70])
+def test_max_seqlen_k(lq):
+    """It cuts a sequence as its length would; 0 leaves every weight as it was."""
+    q, kc, _, lens_t, table = make([900, 500], 64, 8, 2, 64, torch.bfloat16, [lq] * 2)
+    q = q.view(2, lq, 8, 64)
+    lse = torch.randn(2, 8, lq, device=DEV) + 6
+    w0 = pool_like(kc, torch.Generator().manual_seed(1))
+    cut, short, none = w0.clone(), w0.clone(), w0.clone()
+    mfa.kv8_key_weights(q, kc, lse, cut, lens_t, table, causal=True, max_seqlen_k=450)
+    mfa.kv8_key_weights(q, kc, lse, short, i32(450, 450), table, causal=True)
+    mfa.kv8_key_weights(q, kc, lse, none, lens_t, table, causal=True, max_seqlen_k=0)
+    assert torch.equal(cut, short) and not torch.equal(cut, w0) and torch.equal(none, w0)
+    mfa.kv8_key_weights(q, kc, lse, none, i32(0, -3), table, causal=True)
+    mfa.kv8_key_weights(q[:0], kc, lse[:0], none, lens_t[:0], table[:0], causal=True)
+    mfa.kv8_key_weights(q[:, :0], kc, lse[:, :, :0], none, lens_t, table, causal=True)
+    assert torch.equal(none, w0)
+
+
+@pytest.mark.parametrize("heads", [2, 40])
+def test_weights_past_32_bits(heads):
+    """Pages 4 GiB apart: the weights of a step, and an eviction that moves them."""
+    lens, lq, page = [170, 120], [1, 40], 64
+    q, kc, vc, lens_t, table = make(lens, page, 4 * heads, heads, 32, torch.bfloat16, lq)
+    pages = kc[0].shape[0]
+    near = pool_like(kc, torch.Generator().manual_seed(2))
+    far = torch.empty(((pages - 1) << 30) + heads * page, device=DEV).as_strided((pages, page, heads), (1 << 30, 1, page))
+    far.copy_(near)
+    vc2, kc2 = (tuple(x.clone() for x in c) for c in (vc, kc))
+    lse = torch.randn(4 * heads, sum(lq), device=DEV) + 5
+    for w in (near, far):
+        mfa.kv8_key_weights(q, kc, lse, w, lens_t, table, cu_of(lq), causal=True)
+    assert torch.equal(near, far)
+    n = [mfa.kv8_evict(k, v, w, lens_t, table, 100, 10) for k, v, w in ((kc, vc, near), (kc2, vc2, far))]
+    assert n[0].tolist() == n[1].tolist() == [100, 100] and torch.equal(near, far)
+    for a, b in zip((*kc, *vc), (*kc2, *vc2)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
