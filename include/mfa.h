@@ -555,8 +555,8 @@ int mfa_kv8_weights_params_size(void);
  * min(n, budget).  A row on a page id outside the pool reads as zeros with weight 0 and
  * drops what is written.  budget and recent >= 0; the pool has less than 2^31 rows.
  * K and V do not share memory.  `workspace`: 256-byte aligned, at least
- * mfa_kv8_evict_workspace_bytes bytes.  Two or three kernels; never synchronizes, never
- * allocates.
+ * mfa_kv8_evict_workspace_bytes bytes (0, where no row can move: may be NULL).  One to
+ * three kernels; never synchronizes, never allocates.
  */
 typedef struct mfa_kv8_evict_params {
     mfa_kv8_cache cache;

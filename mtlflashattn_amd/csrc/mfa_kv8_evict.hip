@@ -7,7 +7,8 @@
 //    to stay, is found 11, 11 and 10 bits at a time from histograms in LDS (weights
 //    crowd into few exponents: lanes of a wavefront that agree count once together).
 //    Keys stay in LDS where a sequence fits (32768 rows), else they are read again.
-// Then, with many heads in the batch:
+// (Where the bound on the lengths or the budget says that no row moves, one kernel writes the
+// lengths.)  Then, with many heads in the batch:
 //  * walk: a workgroup per head, for K and for V, moves the rows block by block, in place.
 // With few, a workgroup per block:
 //  * save: rows only move down, and no block behind the one that holds row budget - 1
@@ -58,8 +59,8 @@ struct E8Args {
     const int32_t* lens;
     int32_t* new_lens;
     int32_t B, H, D, page, npages, max_k, budget, recent;
-    int32_t rows;    // of the workspace per (sequence, head): the budget, or none where no sequence is longer
-    int32_t blocks;  // of 64 new rows per (sequence, head), at least 1
+    int32_t rows;    // of the workspace per (sequence, head): the budget, or none where no row moves
+    int32_t blocks;  // of 64 new rows per (sequence, head)
     int32_t safe;    // rows from here on are read where they are
     int32_t walk;    // one workgroup moves all rows of a head
     int32_t four;    // weights of four adjacent rows may be loaded at once
@@ -515,6 +516,12 @@ __global__ void __launch_bounds__(walk_threads(D)) mfa_kv8_walk_kernel(E8Args a)
     else walk8<D, false>(a, head, b, h);
 }
 
+// No row moves: no sequence is longer than its budget, or none keeps a row
+__global__ void __launch_bounds__(kEThreads) mfa_kv8_lengths_kernel(E8Args a) {
+    const int b = blockIdx.x * kEThreads + threadIdx.x;
+    if (b < a.B) a.new_lens[b] = min(max(a.lens[b], 0), min(a.max_k, a.budget));
+}
+
 int e8err(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
@@ -560,17 +567,17 @@ int e8_plan(const mfa_kv8_evict_params* p, E8Args* out, int64_t* bytes) {
     a.budget = p->budget; a.recent = p->recent;
     a.by_page = fast_div(a.page);
     const int64_t units = (int64_t)a.B * a.H;
-    // (no sequence is longer than its budget: no rows to hold)
+    // (none: no row moves)
     a.rows = a.budget < a.max_k ? a.budget : 0;
-    const int64_t blocks = std::max<int64_t>(((int64_t)a.rows + kKv8Block - 1) / kKv8Block, 1);
+    const int64_t blocks = ((int64_t)a.rows + kKv8Block - 1) / kKv8Block;
     // (a launch has less than 2^32 threads)
     if (units > 0x3fffff || units * blocks > 0x7fffff) return e8err(MFA_ERR_INVALID, "%s: problem too large", who);
     a.blocks = (int32_t)blocks;
-    a.safe = a.rows > 0 ? (int32_t)(blocks * kKv8Block) : 0;
+    a.safe = (int32_t)(blocks * kKv8Block);
     a.by_blocks = fast_div(a.blocks);
     a.walk = units >= kWalk;
     const int64_t rows = units * a.rows;
-    *bytes = (units * (int64_t)sizeof(Head8) + 255) / 256 * 256 + rows * (a.walk ? 4 : 8 + 2 * a.D + 2) + 64;
+    *bytes = a.rows == 0 ? 0 : (units * (int64_t)sizeof(Head8) + 255) / 256 * 256 + rows * (a.walk ? 4 : 8 + 2 * a.D + 2) + 64;
     return MFA_OK;
 }
 
@@ -594,6 +601,13 @@ int mfa_kv8_evict(const mfa_kv8_evict_params* p, void* workspace, int64_t worksp
     int64_t bytes;
     const int rc = e8_plan(p, &a, &bytes);
     if (rc != MFA_OK || a.B == 0) return rc;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (a.rows == 0) {
+        hipLaunchKernelGGL(mfa_kv8_lengths_kernel, dim3((unsigned)((a.B + kEThreads - 1) / kEThreads)), dim3(kEThreads), 0, st, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e8err(MFA_ERR_LAUNCH, "mfa_kv8_evict: launch failed: %s", hipGetErrorString(e));
+        return MFA_OK;
+    }
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u))
         return e8err(MFA_ERR_INVALID, "mfa_kv8_evict: workspace must be a 256-byte aligned device pointer");
     if (workspace_bytes < bytes)
@@ -613,7 +627,6 @@ int mfa_kv8_evict(const mfa_kv8_evict_params* p, void* workspace, int64_t worksp
     }
     a.idx = reinterpret_cast<int32_t*>(ws);
     if (!a.walk) a.scales = reinterpret_cast<uint8_t*>(a.idx + rows);
-    const hipStream_t st = static_cast<hipStream_t>(stream);
     const auto select = a.max_k <= 4096    ? mfa_kv8_select_kernel<4096>
                         : a.max_k <= 32768 ? mfa_kv8_select_kernel<32768>
                                            : mfa_kv8_select_kernel<0>;
@@ -626,10 +639,8 @@ int mfa_kv8_evict(const mfa_kv8_evict_params* p, void* workspace, int64_t worksp
         hipLaunchKernelGGL(walk, dim3((unsigned)units, 2), dim3(walk_threads(a.D)), 0, st, a);
     } else {
         const dim3 grid((unsigned)(units * a.blocks), 2);
-        if (a.rows > 0) {
-            const fn save = of([](auto d) { return (fn)mfa_kv8_save_kernel<decltype(d)::value>; });
-            hipLaunchKernelGGL(save, grid, dim3(kEThreads), 0, st, a);
-        }
+        const fn save = of([](auto d) { return (fn)mfa_kv8_save_kernel<decltype(d)::value>; });
+        hipLaunchKernelGGL(save, grid, dim3(kEThreads), 0, st, a);
         const fn gather = of([](auto d) { return (fn)mfa_kv8_gather_kernel<decltype(d)::value>; });
         hipLaunchKernelGGL(gather, grid, dim3(kEThreads), 0, st, a);
     }

@@ -245,8 +245,8 @@ def kv8_evict(k_cache, v_cache, weights, cache_seqlens, block_table, budget, rec
     new_seqlens = torch.empty_like(cache_seqlens)
     p.cache_seqlens, p.new_seqlens, p.weights = cache_seqlens.data_ptr(), new_seqlens.data_ptr(), weights.data_ptr()
     kv4._cache_pointers(p.cache, kc, ks, vc, vs, block_table)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _launch_on(device, _hip.kv8_evict, p, ws.data_ptr(), nbytes)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _launch_on(device, _hip.kv8_evict, p, None if ws is None else ws.data_ptr(), nbytes)
     kv4._written((kc, ks, vc, vs, weights))
     return new_seqlens
 

@@ -389,6 +389,12 @@ def test_c_evict(lib):
         refused(lib, lib.mfa_kv8_evict(ctypes.byref(p), None, 0, None), code, text)
         refused(lib, lib.mfa_kv8_evict_workspace_bytes(ctypes.byref(p)), code, text)
     p = params()
+    for change in (dict(budget=0), dict(budget=256), dict(max_seqlen_k=100), dict(max_seqlen_k=7)):  # (no row moves)
+        p = params()
+        for k, v in change.items():
+            setattr(p, k, v)
+        assert lib.mfa_kv8_evict_workspace_bytes(ctypes.byref(p)) == 0
+    p = params()
     p.cache.num_pages = (1 << 31) // p.cache.page_block_size
     refused(lib, lib.mfa_kv8_evict_workspace_bytes(ctypes.byref(p)), -1, "2^31 - 1 rows")
     p = params()
