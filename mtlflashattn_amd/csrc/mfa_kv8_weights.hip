@@ -489,8 +489,10 @@ int mfa_kv8_weights(const mfa_kv8_weights_params* p, void* stream) {
     if (cols > 0x3fffffff || units > 0x3fffffff || units * chunks > 0x7fffffffLL)
         return w8err(MFA_ERR_INVALID, "%s: problem too large", who);
     const int cus = mfa_chip_cus(stream);
-    // (a varlen call's tiles by the mean of its sequences)
-    const int nt = (varlen ? cols > 16 * (int64_t)f.batch : cols > 16) ? 2 : 1;
+    // (a varlen call's tiles by the mean of its sequences; beyond 32 columns they are single rows
+    // beside chunks, as a rule)
+    const int64_t mean = varlen ? (cols + f.batch - 1) / f.batch : cols;
+    const int nt = mean > 16 && mean <= 32 ? 2 : 1;
     for (int few = nt; few >= 0; few -= nt) {
         if (few ? !varlen && cols > 16 * nt : cols <= 16 * nt) continue;
         a.cols = few ? 16 * few : 0x3fffffff;  // (one unit per sequence and K/V head)
