@@ -43,6 +43,7 @@ struct K4Args {
     int32_t min_cols, max_cols;  // a sequence with fewer or more columns is another launch's
     float* ws_o;     // [G][2][cols][D]
     float* ws_ml;    // [G][2][cols][2] exponent reference, sum of p
+    float* ws_le;    // [G][2][cols] sum of p before its rounding, NULL: that of ws_ml is of exact ones
     Merge4* ws_merge;  // [G], NULL: no unit is walked by more than one workgroup
 };
 
@@ -309,7 +310,7 @@ struct MfaKvFormat {
     float least_scale;                              // softmax scales up to here take the path that scales before it masks
     bool varlen32;                                  // varlen calls of 17 to 32 columns per sequence on average take the kernel of 32
     void* (*rows_kernel)(int dp, int cols, bool bf16);   // void(*)(K4Args), for 16 or 32 columns
-    void* (*tile_kernel)(int dp, bool bf16, bool bias);  // ... for 128
+    void* (*tile_kernel)(int dp, bool bf16, bool bias, bool lse);  // ... for 128
 };
 // mfa_kv4_attend.hip; the parameters mean what include/mfa.h says of mfa_kv4_fwd.
 // mfa_kv_args: checks them and fills K4Args with what does not depend on how the work
@@ -319,5 +320,5 @@ __attribute__((visibility("hidden"))) int64_t mfa_kv_fwd_workspace_bytes(const m
 __attribute__((visibility("hidden"))) int mfa_kv_fwd(const mfa_kv4_fwd_params* p, const MfaKvFormat& f, void* workspace,
                                                      int64_t workspace_bytes, void* stream);
 // mfa_kv4_tile.hip, mfa_kv8_tile.hip
-__attribute__((visibility("hidden"))) void* mfa_kv4_tile_kernel_of(int dp, bool bf16, bool bias);
-__attribute__((visibility("hidden"))) void* mfa_kv8_tile_kernel_of(int dp, bool bf16, bool bias);
+__attribute__((visibility("hidden"))) void* mfa_kv4_tile_kernel_of(int dp, bool bf16, bool bias, bool lse);
+__attribute__((visibility("hidden"))) void* mfa_kv8_tile_kernel_of(int dp, bool bf16, bool bias, bool lse);

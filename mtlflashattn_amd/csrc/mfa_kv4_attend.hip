@@ -172,11 +172,13 @@ struct Block4 {
 // where some have many (13.6 us for the step above, 18.8 with 512).
 constexpr int kMergeFew = 512, kMergeMany = 256;
 constexpr int merge_cols(int threads) { return threads / (MFA_MAX_HEAD_DIM / 4); }
-template <int DP, bool IS_BF16, int T>
+// LE: some parts have a sum for the log-sum-exp of their own (ws_le).
+template <int DP, bool IS_BF16, int T, bool LE>
 __global__ void __launch_bounds__(T) mfa_kv_merge_kernel(K4Args, K4Args) {
     constexpr int kMergeCols = merge_cols(T);
     __shared__ f32x4_t o_s[T];
     __shared__ float2 ml_s[T];
+    __shared__ float le_s[LE ? T : 1];
     const int tid = threadIdx.x;
     const int first = args4(0).ws_merge ? args4(0).G * (args4(0).cols / kMergeCols) : 0;
     const int which = __builtin_amdgcn_readfirstlane((int)blockIdx.x >= first);
@@ -194,11 +196,14 @@ __global__ void __launch_bounds__(T) mfa_kv_merge_kernel(K4Args, K4Args) {
     const int r = in ? it / (DP / 4) : 0, d = in ? 4 * (it - r * (DP / 4)) : 0;
     const float* ws_o = a.ws_o;
     const float* ws_ml = a.ws_ml;
-    float m = -INFINITY, l = 0.f;
+    const float* ws_le = a.ws_le ? a.ws_le : ws_ml + 1;  // (by le_step)
+    const int le_step = a.ws_le ? 1 : 2;
+    float m = -INFINITY, l = 0.f, le = 0.f;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-    auto add = [&](float mw, float lw, const f32x4_t& y) {
+    auto add = [&](float mw, float lw, float lew, const f32x4_t& y) {
         const float mn = fmax_nn(m, mw), e0 = pow2_diff(m, mn), e1 = pow2_diff(mw, mn);
         l = fmaf(lw, e1, l * e0);
+        if constexpr (LE) le = fmaf(lew, e1, le * e0);
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[k] = fmaf(y[k], e1, acc[k] * e0);
         m = mn;
@@ -207,16 +212,18 @@ __global__ void __launch_bounds__(T) mfa_kv_merge_kernel(K4Args, K4Args) {
         constexpr int N = decltype(ahead)::value;
         for (int v0 = w0 + g; v0 <= w1; v0 += P * N) {
             float2 ml[N];
+            float lw[N];
             f32x4_t y[N];
 #pragma unroll
             for (int z = 0; z < N; ++z) {
                 const int64_t row = at(min(v0 + P * z, w1)) + r;
                 ml[z] = *reinterpret_cast<const float2*>(ws_ml + 2 * row);
+                lw[z] = LE ? ws_le[le_step * row] : 0.f;
                 y[z] = *reinterpret_cast<const f32x4_t*>(ws_o + row * DP + d);
             }
 #pragma unroll
             for (int z = 0; z < N; ++z)
-                if (v0 + P * z <= w1) add(ml[z].x, ml[z].y, y[z]);
+                if (v0 + P * z <= w1) add(ml[z].x, ml[z].y, lw[z], y[z]);
         }
     };
     if (w1 - w0 + 1 <= 2 * P)
@@ -228,14 +235,15 @@ __global__ void __launch_bounds__(T) mfa_kv_merge_kernel(K4Args, K4Args) {
     if (P > 1) {
         o_s[tid] = acc;
         ml_s[tid] = make_float2(m, l);
+        if constexpr (LE) le_s[tid] = le;
         __syncthreads();
         if (g > 0) return;
-        for (int z = 1; z < P; ++z) add(ml_s[tid + z * S].x, ml_s[tid + z * S].y, o_s[tid + z * S]);
+        for (int z = 1; z < P; ++z) add(ml_s[tid + z * S].x, ml_s[tid + z * S].y, LE ? le_s[tid + z * S] : 0.f, o_s[tid + z * S]);
     }
     if (in) {
         const int col = g4.col0 + cbeg + r, i = (int)div4(col, a.by_r), h = g4.hkv * a.R + col - i * a.R;
         store_row4<IS_BF16>(a.o + row_off4(a.cu_q != nullptr, g4.b, g4.q0, i, h, a.ob, a.os, a.oh) * 2, d, acc, l);
-        if (d == 0) store_lse4(a, g4.b, g4.q0, i, h, m, l);
+        if (d == 0) store_lse4(a, g4.b, g4.q0, i, h, m, LE ? le : l);
     }
 }
 static_assert(16 % merge_cols(kMergeFew) == 0 && kTileCols4 % merge_cols(kMergeMany) == 0, "whole blocks per unit");
@@ -244,16 +252,18 @@ typedef void (*k4_fn)(K4Args);
 typedef void (*k4_merge_fn)(K4Args, K4Args);
 // threads: of the merge's blocks
 template <int DP, bool IS_BF16>
-k4_merge_fn merge4(int threads) {
-    return threads == kMergeFew ? mfa_kv_merge_kernel<DP, IS_BF16, kMergeFew> : mfa_kv_merge_kernel<DP, IS_BF16, kMergeMany>;
+k4_merge_fn merge4(int threads, bool le) {
+    return threads == kMergeFew ? mfa_kv_merge_kernel<DP, IS_BF16, kMergeFew, false>  // (no tiles of 128 columns)
+           : le                 ? mfa_kv_merge_kernel<DP, IS_BF16, kMergeMany, true>
+                                : mfa_kv_merge_kernel<DP, IS_BF16, kMergeMany, false>;
 }
 template <bool IS_BF16>
-k4_merge_fn merge4(int dp, int threads) {
+k4_merge_fn merge4(int dp, int threads, bool le) {
     switch (dp) {
-        case 32: return merge4<32, IS_BF16>(threads);
-        case 64: return merge4<64, IS_BF16>(threads);
-        case 96: return merge4<96, IS_BF16>(threads);
-        default: return merge4<128, IS_BF16>(threads);
+        case 32: return merge4<32, IS_BF16>(threads, le);
+        case 64: return merge4<64, IS_BF16>(threads, le);
+        case 96: return merge4<96, IS_BF16>(threads, le);
+        default: return merge4<128, IS_BF16>(threads, le);
     }
 }
 
@@ -276,9 +286,11 @@ struct K4Launch {
     K4Args a;
     int64_t parts;  // rows of its partial results, 0: no merge
 };
-// workspace of a launch: parts, their references and sums, what is merged
+// workspace of a launch: parts, their references and sums (of 128 columns one more, for the
+// log-sum-exp, whether it is asked for or not), what is merged
 int64_t part_bytes(const K4Launch& l, int D) {
-    return l.parts ? (l.parts * (D * 4 + 8) + (int64_t)l.a.G * sizeof(Merge4) + 255) / 256 * 256 : 0;
+    const int64_t row = D * 4 + (l.a.cols == kTileCols4 ? 12 : 8);
+    return l.parts ? (l.parts * row + (int64_t)l.a.G * sizeof(Merge4) + 255) / 256 * 256 : 0;
 }
 struct K4Plan {
     K4Launch l[2];
@@ -443,19 +455,21 @@ int mfa_kv_fwd(const mfa_kv4_fwd_params* p, const MfaKvFormat& f, void* workspac
     const int threads = plan.l[plan.n - 1].a.cols == kTileCols4 ? kMergeMany : kMergeFew;
     for (int i = 0; i < plan.n; ++i) {
         K4Launch& l = plan.l[i];
-        const k4_fn attend = (k4_fn)(l.a.cols == kTileCols4 ? f.tile_kernel(p->head_dim, bf16, l.a.bias != 0)
+        const k4_fn attend = (k4_fn)(l.a.cols == kTileCols4 ? f.tile_kernel(p->head_dim, bf16, l.a.bias != 0, l.a.lse != nullptr)
                                                             : f.rows_kernel(p->head_dim, l.a.cols, bf16));
         if (l.parts) {
             l.a.ws_o = reinterpret_cast<float*>(ws);
             l.a.ws_ml = l.a.ws_o + l.parts * p->head_dim;
             l.a.ws_merge = reinterpret_cast<Merge4*>(l.a.ws_ml + l.parts * 2);
+            if (l.a.cols == kTileCols4 && l.a.lse) l.a.ws_le = reinterpret_cast<float*>(l.a.ws_merge + l.a.G);
             ws += part_bytes(l, p->head_dim);
             merge += l.a.G * (l.a.cols / merge_cols(threads));
         }
         hipLaunchKernelGGL(attend, dim3(l.a.G), dim3(kThreads4), 0, st, l.a);
     }
     if (merge) {
-        const k4_merge_fn fn = bf16 ? merge4<true>(p->head_dim, threads) : merge4<false>(p->head_dim, threads);
+        const bool le = plan.l[plan.n - 1].a.ws_le != nullptr;
+        const k4_merge_fn fn = bf16 ? merge4<true>(p->head_dim, threads, le) : merge4<false>(p->head_dim, threads, le);
         hipLaunchKernelGGL(fn, dim3(merge), dim3(threads), 0, st, plan.l[0].a, plan.l[plan.n - 1].a);
     }
     const hipError_t e = hipGetLastError();

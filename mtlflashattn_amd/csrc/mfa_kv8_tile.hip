@@ -113,20 +113,24 @@ struct Stage8 {
     }
 };
 
-template <int DP>
-void* tile_of(bool bf16, bool bias) {
+template <class Stage>
+void* tile_of(bool bias, bool lse) {
     typedef void (*fn)(K4Args);
-    return bf16 ? (void*)(bias ? (fn)mfa_kv_tile_kernel<Stage8<DP, true>, true> : (fn)mfa_kv_tile_kernel<Stage8<DP, true>, false>)
-                : (void*)(bias ? (fn)mfa_kv_tile_kernel<Stage8<DP, false>, true> : (fn)mfa_kv_tile_kernel<Stage8<DP, false>, false>);
+    return (void*)(bias ? (lse ? (fn)mfa_kv_tile_kernel<Stage, true, true> : (fn)mfa_kv_tile_kernel<Stage, true, false>)
+                        : (lse ? (fn)mfa_kv_tile_kernel<Stage, false, true> : (fn)mfa_kv_tile_kernel<Stage, false, false>));
+}
+template <int DP>
+void* tile_of(bool bf16, bool bias, bool lse) {
+    return bf16 ? tile_of<Stage8<DP, true>>(bias, lse) : tile_of<Stage8<DP, false>>(bias, lse);
 }
 
 }  // namespace
 
-void* mfa_kv8_tile_kernel_of(int dp, bool bf16, bool bias) {
+void* mfa_kv8_tile_kernel_of(int dp, bool bf16, bool bias, bool lse) {
     switch (dp) {
-        case 32: return tile_of<32>(bf16, bias);
-        case 64: return tile_of<64>(bf16, bias);
-        case 96: return tile_of<96>(bf16, bias);
-        default: return tile_of<128>(bf16, bias);
+        case 32: return tile_of<32>(bf16, bias, lse);
+        case 64: return tile_of<64>(bf16, bias, lse);
+        case 96: return tile_of<96>(bf16, bias, lse);
+        default: return tile_of<128>(bf16, bias, lse);
     }
 }

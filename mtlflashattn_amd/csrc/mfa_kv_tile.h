@@ -37,7 +37,11 @@ __device__ __forceinline__ int vswz4(int r) {
     return DP == 128 ? 5 * (r & 3) : DP == 64 ? 4 * ((r >> 1) & 1) + ((r >> 1) & 3) : DP == 96 ? r & 3 : (r >> 2) & 3;
 }
 
-template <class Stage, bool BIAS>
+// LSE: the log-sum-exp is asked for.  Its sum is of the probabilities before they are
+// rounded, beside that of the rounded ones, which the result is divided by: what the
+// roundings of a row's weights have in common cancels there, but would leave the
+// log-sum-exp off by up to 2^-8 in bf16 and 2^-11 in fp16.
+template <class Stage, bool BIAS, bool LSE>
 __global__ void __launch_bounds__(kThreads4) __attribute__((amdgpu_waves_per_eu(2)))
 mfa_kv_tile_kernel(K4Args) {
     constexpr int DP = Stage::D;
@@ -105,7 +109,7 @@ mfa_kv_tile_kernel(K4Args) {
         // these run between the products of the other tile)
         auto swrite = [&](bool part, int to, int half_) { stage.write(smem + to * T_ELEMS, nan_s[to], part, half_, tid); };
 
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY, l = 0.f, l_exact = 0.f;  // (l_exact: with LSE)
         f32x16_t o[DB];
 #pragma unroll
         for (int db = 0; db < DB; ++db)
@@ -226,6 +230,7 @@ mfa_kv_tile_kernel(K4Args) {
                 float alpha = pow2_diff(m, mn);
                 asm volatile("" : "+v"(alpha));  // (keeps the products inside the branch)
                 l *= alpha;
+                if constexpr (LSE) l_exact *= alpha;
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -239,7 +244,7 @@ mfa_kv_tile_kernel(K4Args) {
             // result: 4.3e-5 rms against 3.1e-5 for results of 1.8e-2 over 8192 keys in
             // bf16, 5.4e-6 against 3.8e-6 in fp16; two have the latter.)  The second 32
             // keys' are formed while the first's products run.
-            float acc[2] = {0.f, 0.f};
+            float acc[2] = {0.f, 0.f}, exact = 0.f;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 u32x4_t pw[2];
@@ -249,6 +254,7 @@ mfa_kv_tile_kernel(K4Args) {
                     for (int w = 0; w < 4; ++w) {
                         const float p0 = fast_exp2(fmaf(s[kb][8 * st + 2 * w], c, -mu));
                         const float p1 = fast_exp2(fmaf(s[kb][8 * st + 2 * w + 1], c, -mu));
+                        if constexpr (LSE) exact += p0 + p1;
                         if constexpr (IS_BF16) {
                             const k4_bf16x2_t pk = {(__bf16)p0, (__bf16)p1}, one = {(__bf16)1.f, (__bf16)1.f};
                             acc[w & 1] = __builtin_amdgcn_fdot2_f32_bf16(pk, one, acc[w & 1], false);
@@ -269,6 +275,7 @@ mfa_kv_tile_kernel(K4Args) {
                 if (kb == 0) load_v(1);
             }
             l += acc[0] + acc[1];
+            if constexpr (LSE) l_exact += exact;
         };
 
         if (jbeg < jend) gload(jbeg);
@@ -309,6 +316,8 @@ mfa_kv_tile_kernel(K4Args) {
         // ---- results: lane (column, half) holds elements 32 db + 8 g + 4 half + 0..3
         K4Const& e = args4();
         const float lt = sum_halves(l);
+        float le = lt;
+        if constexpr (LSE) le = sum_halves(l_exact);
         const int col = wcol + l32, qi = (int)div4(col, e.by_r), h = wk.hkv * e.R + col - qi * e.R;
         const bool in = col <= wlast;
         if (live && wk.whole) {
@@ -327,7 +336,7 @@ mfa_kv_tile_kernel(K4Args) {
                     }
                     *reinterpret_cast<u32x2_t*>(rows + l32 * KST + 32 * db + 8 * g + 4 * half) = w;
                 }
-            if (in && half == 0) store_lse4(e, wk.b, wk.sq.q0, qi, h, m, lt);
+            if (in && half == 0) store_lse4(e, wk.b, wk.sq.q0, qi, h, m, le);
             for (int x = lane; x < (wlast - wcol + 1) * CPR; x += 64) {
                 const int r = x / CPR, d = 8 * (x - r * CPR);
                 const int ri = (int)div4(wcol + r, e.by_r), rh = wk.hkv * e.R + wcol + r - ri * e.R;
@@ -343,7 +352,10 @@ mfa_kv_tile_kernel(K4Args) {
                 for (int g = 0; g < 4; ++g)
                     *reinterpret_cast<f32x4_t*>(p + 32 * db + 8 * g + 4 * half) =
                         f32x4_t{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
-            if (half == 0) *reinterpret_cast<float2*>(e.ws_ml + 2 * row) = make_float2(m, lt);
+            if (half == 0) {
+                *reinterpret_cast<float2*>(e.ws_ml + 2 * row) = make_float2(m, lt);
+                if constexpr (LSE) e.ws_le[row] = le;
+            }
         }
         __syncthreads();  // (the result rows are read before the next unit's tiles are written)
     }
