@@ -123,11 +123,13 @@ __global__ void __launch_bounds__(kSThreads) mfa_kv8_select_kernel(E8Args a) {
         low_s = max(0, min(tail, a.safe - m));
     }
 
+    // (rows are counted without a sign: whole rounds behind m may pass 2^31)
+    const uint32_t rows = (uint32_t)m;
     // the keys of rows j .. j + 3 (j a multiple of 4), 0 for rows from m on
-    auto read4 = [&](int j) {
+    auto read4 = [&](uint32_t j) {
         float w[4] = {0.f, 0.f, 0.f, 0.f};
-        if (j < m) {
-            const Place8 p = place8(a, bt, j);  // (of all four)
+        if (j < rows) {
+            const Place8 p = place8(a, bt, (int)j);  // (of all four)
             if (p.id >= 0) {
                 const float* at = weight_at(a, p, h);
                 if (a.four) {
@@ -141,18 +143,18 @@ __global__ void __launch_bounds__(kSThreads) mfa_kv8_select_kernel(E8Args a) {
         }
         u32x4_t k;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k[i] = j + i < m ? key_of(w[i]) : 0u;
+        for (int i = 0; i < 4; ++i) k[i] = j + i < rows ? key_of(w[i]) : 0u;
         return k;
     };
-    auto keys4 = [&](int j) {
+    auto keys4 = [&](uint32_t j) {
         if constexpr (KEYS > 0) return *reinterpret_cast<const u32x4_t*>(key_s + j);
         else return read4(j);
     };
-    const int end4 = (m + 4 * kSThreads - 1) / (4 * kSThreads) * (4 * kSThreads);  // whole rounds of the workgroup
+    const uint32_t end4 = (rows + 4 * kSThreads - 1) / (4 * kSThreads) * (4 * kSThreads);  // whole rounds of the workgroup
     if constexpr (KEYS > 0) {
         static_assert(KEYS % (4 * kSThreads) == 0, "whole rounds");
 #pragma unroll 2
-        for (int j = 4 * tid; j < end4; j += 4 * kSThreads) *reinterpret_cast<u32x4_t*>(key_s + j) = read4(j);
+        for (uint32_t j = 4 * tid; j < end4; j += 4 * kSThreads) *reinterpret_cast<u32x4_t*>(key_s + j) = read4(j);
     }
     __syncthreads();
 
@@ -164,11 +166,11 @@ __global__ void __launch_bounds__(kSThreads) mfa_kv8_select_kernel(E8Args a) {
         const uint32_t mask = pass < 2 ? kBins - 1 : kBins / 2 - 1;
         count_s[tid] = count_s[tid + kSThreads] = 0;
         __syncthreads();
-        for (int j = 4 * tid; j < end4; j += 4 * kSThreads) {
+        for (uint32_t j = 4 * tid; j < end4; j += 4 * kSThreads) {
             const u32x4_t k = keys4(j);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool on = j + i < m && (pass == 0 || (k[i] ^ t) >> known == 0);
+                const bool on = j + i < rows && (pass == 0 || (k[i] ^ t) >> known == 0);
                 const uint64_t any = __ballot(on);
                 if (any == 0) continue;
                 const int bin = (int)(k[i] >> shift & mask), one = __builtin_amdgcn_readlane(bin, __builtin_ctzll(any));
@@ -204,9 +206,9 @@ __global__ void __launch_bounds__(kSThreads) mfa_kv8_select_kernel(E8Args a) {
 
     // ---- the rows that stay, in order: those above t, and of those at t the first.  Each
     // wavefront takes consecutive rows.
-    const int per = ((m + kSWaves - 1) / kSWaves + 255) / 256 * 256, w0 = wave * per, w1 = min(w0 + per, m);
+    const uint32_t per = ((rows + kSWaves - 1) / kSWaves + 255) / 256 * 256, w0 = wave * per, w1 = min(w0 + per, rows);
     int gt = 0, eq = 0;
-    for (int j = w0; j < w1; j += 256) {
+    for (uint32_t j = w0; j < w1; j += 256) {
         const u32x4_t k = j + 4 * lane < end4 ? keys4(j + 4 * lane) : u32x4_t{0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -227,8 +229,9 @@ __global__ void __launch_bounds__(kSThreads) mfa_kv8_select_kernel(E8Args a) {
         base_eq += w < wave ? eq_s[w] : 0;
     }
     const int spare = need - all_gt;  // (of those at t; none where all that reach it stay)
-    int gone = m, low = 0;            // the first row that goes; rows that stay in front of `safe`
-    for (int j = w0; j < w1; j += 256) {
+    uint32_t gone = rows;  // the first row that goes
+    int low = 0;           // rows that stay in front of `safe`
+    for (uint32_t j = w0; j < w1; j += 256) {
         const u32x4_t k = j + 4 * lane < end4 ? keys4(j + 4 * lane) : u32x4_t{0, 0, 0, 0};
         // a lane's four rows are adjacent: sums of the lanes below
         int g = 0, e = 0;
@@ -239,14 +242,14 @@ __global__ void __launch_bounds__(kSThreads) mfa_kv8_select_kernel(E8Args a) {
         }
         const int both = g | e << 16, inc = scan64(both), last = __builtin_amdgcn_readlane(inc, 63);
         int at_g = base_gt + ((inc - both) & 0xffff), at_e = base_eq + ((inc - both) >> 16);
-        const Place8 p = both ? place8(a, bt, j + 4 * lane) : Place8{-1, 0};  // (of all four)
+        const Place8 p = both ? place8(a, bt, (int)(j + 4 * lane)) : Place8{-1, 0};  // (of all four)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int row = j + 4 * lane + i;
+            const uint32_t row = j + 4 * lane + i;
             const bool is_gt = k[i] > t, is_eq = k[i] == t;
             if (is_gt || (is_eq && at_e < spare)) {
                 idx[at_g + min(at_e, spare)] = packed8(a, Place8{p.id, p.row + i});
-                low += row < a.safe;
+                low += row < (uint32_t)a.safe;
             } else {
                 gone = min(gone, row);
             }
@@ -258,11 +261,11 @@ __global__ void __launch_bounds__(kSThreads) mfa_kv8_select_kernel(E8Args a) {
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        gone = min(gone, __shfl_xor(gone, o));
+        gone = min(gone, (uint32_t)__shfl_xor((int)gone, o));
         low += __shfl_xor(low, o);
     }
     if (lane == 0) {
-        if (gone < m) atomicMin(&first_s, gone);
+        if (gone < rows) atomicMin(&first_s, (int)gone);
         atomicAdd(&low_s, low);
     }
     for (int r = tid; r < tail; r += kSThreads) idx[need + r] = packed8(a, place8(a, bt, m + r));
@@ -551,7 +554,7 @@ int e8_plan(const mfa_kv8_evict_params* p, E8Args* out, int64_t* bytes) {
     if (p->weight_row_stride < 0 || p->weight_head_stride < 0)
         return e8err(MFA_ERR_INVALID, "%s: row and head strides must be >= 0", who);
     const int64_t cap = (int64_t)p->cache.max_pages * p->cache.page_block_size;
-    a.max_k = (int32_t)std::min<int64_t>(p->max_seqlen_k ? p->max_seqlen_k : cap, std::min<int64_t>(cap, 0x7fffff00));
+    a.max_k = (int32_t)std::min<int64_t>(p->max_seqlen_k ? p->max_seqlen_k : cap, cap);  // (below 2^31: checked)
     a.pool[0] = kv4_pool(p->cache.k);
     a.pool[1] = kv4_pool(p->cache.v);
     a.w = p->weights;
