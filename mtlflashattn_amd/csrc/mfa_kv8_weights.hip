@@ -302,7 +302,8 @@ mfa_kv8_weights_many_kernel(K4Args) {
         // fewer than wavefronts, two or four share one and take every second or fourth 32
         // columns
         const int keys = wk.parts > 1 ? kChunk4 / 2 : kWChunks * kChunk4;
-        const int j0 = c0 * kChunk4 + wk.part * keys, jend = min(min(ch.end * kChunk4, j0 + keys), Lk);
+        // (as differences: j0 + keys may pass 31 bits)
+        const int j0 = c0 * kChunk4 + wk.part * keys, jend = j0 + min(min(ch.end * kChunk4, Lk) - j0, keys);
         if (j0 >= jend) break;
         const int nb = (jend - j0 + 31) / 32, cw = nb <= kWaves / 4 ? 4 : nb <= kWaves / 2 ? 2 : 1, kw = kWaves / cw;
         const int cg = wave / kw, b0 = wave - cg * kw;

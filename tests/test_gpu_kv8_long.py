@@ -55,3 +55,22 @@ def test_evict(n):
     keep = wd.cpu()
     keep[2, :budget] = w[2, :budget]
     assert torch.equal(keep, w)
+
+
+@pytest.mark.parametrize("lq,left", [(1, -1), (40, -1), (40, 1000), (300, 1000)])
+@pytest.mark.parametrize("n", [(1 << 31) - 300, (1 << 31) - 700])
+def test_key_weights(n, lq, left):
+    """Keys of zeros and log-sum-exps of 0: a key gains the number of rows that see it, exactly."""
+    kc = mfa.kv8_cache(3, PAGE, 1, 32)
+    last = (n - 1) // PAGE
+    table = long_table({0: 2, last: 1}.items())
+    q = torch.randn(1, lq, 1, 32, device=DEV, dtype=torch.bfloat16)
+    w = torch.ones(3, PAGE, 1, device=DEV)
+    mfa.kv8_key_weights(q, kc, torch.zeros(1, 1, lq, device=DEV), w, i32(n), table, causal=True, window_size=(left, -1))
+    want = torch.ones(3, PAGE)
+    for page, col in ((2, 0), (1, last)):
+        j = col * PAGE + torch.arange(PAGE)
+        i = n - lq + torch.arange(lq)[:, None]
+        seen = (j <= i) & ((j >= i - left) | (left < 0))
+        want[page] = torch.where(j < n, torch.where(j < n - lq, 1.0, 0.0) + seen.sum(0), 1.0)
+    assert torch.equal(w[..., 0].cpu(), want)
