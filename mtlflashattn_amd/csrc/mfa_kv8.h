@@ -20,12 +20,12 @@ constexpr int kKv8Block = MFA_KV8_BLOCK;  // rows per scale
 
 __device__ __forceinline__ float kv8_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// K's scale as a factor of scores in log2 units before their mask is applied: not below
-// 2^-60, as a factor of 0 (byte 0, which a page outside the pool reads as) times a masked
-// score, -inf, would be NaN.  Scores of smaller scales are 0 to fp32 sums either way
-// (products of |q| < 2^24 with codes stay below 2^-20).
-constexpr float kKv8LeastScale = 0x1p-60f;
-__device__ __forceinline__ float kv8_k_scale(uint32_t byte) { return fmaxf(kv8_scale(byte), kKv8LeastScale); }
+// K's scale as a factor of scores in log2 units before their mask is applied: that of byte 1
+// for byte 0 (which a page outside the pool reads as), as a factor of 0 times a masked
+// score, -inf, would be NaN.  Softmax scales up to 2^-24, whose product with it is 0 in
+// fp32, take the path that masks behind the scaling.
+constexpr float kKv8LeastScale = 0x1p-24f;
+__device__ __forceinline__ float kv8_k_scale(uint32_t byte) { return kv8_scale(max(byte, 1u)); }
 
 // Eight codes (two dwords) as eight bf16: exact while code * s is a normal bf16.
 __device__ __forceinline__ u32x4_t kv8_bf16x8(uint32_t w0, uint32_t w1, float s) {
