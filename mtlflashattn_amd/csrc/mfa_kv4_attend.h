@@ -11,6 +11,7 @@ typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4_t;
 
 constexpr int kThreads4 = 256;
 constexpr int kChunk4 = 128;  // keys per chunk, the unit of dealt work
+constexpr int kAllCols4 = 0x3fffffff;  // columns per unit: all of a sequence
 constexpr float kLn2f = 0.6931471805599453f;
 
 // What the merge kernel adds for workgroup w: the parts of workgroups w - 1 to w1
@@ -101,7 +102,8 @@ __device__ __forceinline__ Seq4 seq4(K4Const& a, int b) {
     // row without keys is stored too)
     int n = (s.Lk + kChunk4 - 1) / kChunk4;
     if (a.wl >= 0 && (a.causal || a.wr >= 0)) {
-        const int64_t span = (int64_t)a.wl + (a.causal ? 0 : a.wr) + (a.cols - 1) / a.R + 1;
+        const int rows = a.cols == kAllCols4 ? s.Lq : (a.cols - 1) / a.R + 1;
+        const int64_t span = (int64_t)a.wl + (a.causal ? 0 : a.wr) + rows;
         n = (int)min((int64_t)n, (span + kChunk4 - 1) / kChunk4 + 1);
     }
     s.chunks = max(n, 1);

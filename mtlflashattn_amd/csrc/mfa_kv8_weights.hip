@@ -496,7 +496,7 @@ int mfa_kv8_weights(const mfa_kv8_weights_params* p, void* stream) {
     const int nt = mean > 16 && mean <= 32 ? 2 : 1;
     for (int few = nt; few >= 0; few -= nt) {
         if (few ? !varlen && cols > 16 * nt : cols <= 16 * nt) continue;
-        a.cols = few ? 16 * few : 0x3fffffff;  // (one unit per sequence and K/V head)
+        a.cols = few ? 16 * few : kAllCols4;  // (one unit per sequence and K/V head)
         a.min_cols = few ? 1 : 16 * nt + 1;
         a.max_cols = few ? 16 * few : 0x7fffffff;
         const int64_t most = units * chunks * (few ? 1 : 2);  // (halves of chunks)
