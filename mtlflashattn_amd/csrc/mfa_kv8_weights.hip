@@ -223,7 +223,8 @@ struct Piece4 {
         Seq4 s = seq(0);
         int all = __builtin_amdgcn_readlane(scan64(s.items(H)), 63);
         for (int b0 = 64; b0 < B; b0 += 64) all += __builtin_amdgcn_readlane(scan64(seq(b0).items(H)), 63);
-        const int most = max((all + a.G - 1) / a.G, 1);
+        if (all == 0) return false;
+        const int most = (all + a.G - 1) / a.G;
         const bool half = all <= a.G / 2;
         auto of = [&](const Seq4& y) { return y.tiles * H * pieces(y, most) * parts_of(y, a.R, half); };
         int n = of(s), inc = scan64(n), total = __builtin_amdgcn_readlane(inc, 63);
@@ -499,10 +500,12 @@ int mfa_kv8_weights(const mfa_kv8_weights_params* p, void* stream) {
         a.cols = few ? 16 * few : kAllCols4;  // (one unit per sequence and K/V head)
         a.min_cols = few ? 1 : 16 * nt + 1;
         a.max_cols = few ? 16 * few : 0x7fffffff;
-        const int64_t most = units * chunks * (few ? 1 : 2);  // (halves of chunks)
+        // (of a varlen call's sequences no more than its rows allow have the columns for it)
+        const int64_t mine = few || !varlen ? units : std::min<int64_t>(units, cols / a.min_cols * a.Hkv);
+        const int64_t most = mine * chunks * (few ? 1 : 2);  // (halves of chunks)
         a.G = (int32_t)std::min<int64_t>(most, (int64_t)cus * (few ? few_wgs(few) : kManyWgs));
         // (pieces: at most one more of each unit than its share)
-        int64_t grid = few ? a.G : std::min<int64_t>(most, a.G + units);
+        int64_t grid = few ? a.G : std::min<int64_t>(most, a.G + mine);
         if (!few) grid = (grid + 7) / 8 * 8;
         a.xcds = 1;
         const bool bias = a.bias != 0;

@@ -53,3 +53,39 @@ def test_a_window_over_a_long_cache(batch, lq, left, n):
         assert float(w.double().sum()) == batch * 32 * sum(min(i + L - lq, left) + 1 for i in range(lq))
         times.append(time_of(call))
     assert times[0] <= 2 * times[1]
+
+
+@pytest.mark.parametrize("batch,n", [(1024, 512), (2048, 256)])
+def test_single_rows_of_a_varlen_call(batch, n):
+    """The launch for sequences of more columns, of which there are none, costs little beside the
+    work: a fifth, and half (it was 1.4 and 4 times the work)."""
+    times, sums = [], []
+    for varlen in (False, True):
+        call, w = step([n] * batch, 1, 32, 8, 128, varlen=varlen)
+        call()
+        sums.append(w)
+        assert bool((w == 4).all())
+        times.append(time_of(call))
+    assert torch.equal(*sums)
+    assert times[1] <= (1.6 if batch == 1024 else 2.2) * times[0]
+
+
+@pytest.mark.parametrize("lq", [[17] + [0] * 70 + [18, 1, 40], [1] * 130 + [17], [5] * 64 + [9, 17, 33], [300], [33] * 9])
+def test_few_sequences_with_many_columns(lq):
+    """All of them are found where rows leave room for no more."""
+    lens = [n + 200 for n in lq]
+    Hkv, D, page = 2, 32, 64
+    for R in (1, 4):
+        kc = mfa.kv8_cache(sum(-(-n // page) for n in lens), page, Hkv, D)
+        table, at = torch.full((len(lens), 8), -1, dtype=torch.int32), 0
+        for b, n in enumerate(lens):
+            for i in range(-(-n // page)):
+                table[b, i] = at
+                at += 1
+        q = torch.randn(sum(lq), R * Hkv, D, device=DEV, dtype=torch.bfloat16)
+        w = torch.ones(at, page, Hkv, device=DEV)
+        mfa.kv8_key_weights(q, kc, torch.zeros(R * Hkv, sum(lq), device=DEV), w, i32(*lens), table.to(DEV), cu_of(lq))
+        for b, (n, L) in enumerate(zip(lq, lens)):
+            got = w[table[b, :-(-L // page)].long()].flatten(0, 1)[:L].cpu()
+            want = torch.where(torch.arange(L) < L - n, 1.0, 0.0) + R * n
+            assert torch.equal(got, want[:, None].expand(-1, Hkv)), (R, b)
