@@ -431,8 +431,8 @@ int mfa_kv4_append_params_size(void);
 /*
  * Attention over the cache: the forward of mfa_fwd (masks, soft-cap, ALiBi,
  * grouped-query heads and softmax_lse as there) with K and V from the cache.
- * Sequence b has min(cache_seqlens[b], max_seqlen_k, what the table can name)
- * keys, read on the device; max_seqlen_k 0 leaves the bound out.  Queries: q
+ * Sequence b has min(cache_seqlens[b], max_seqlen_k, what the table can name, 2^31 -
+ * 256) keys, read on the device; max_seqlen_k 0 leaves the bound out.  Queries: q
  * [batch, seqlen_q, heads_q, head_dim], or with cu_seqlens_q q [total_q, heads_q,
  * head_dim], sequence b owning tokens [cu_seqlens_q[b], cu_seqlens_q[b + 1])
  * (tokens of no sequence get 0, lse -inf).  The query rows are the last
@@ -443,7 +443,8 @@ int mfa_kv4_append_params_size(void);
  * The columns of a sequence are its query positions times the query heads per K/V
  * head.  Sequences of more than 32 columns, and in a varlen call of more than 32
  * columns in total those of more than 16, run on tiles of 128 columns: there a
- * probability is rounded to one 16-bit term (elsewhere to two bf16 terms), and with
+ * probability is rounded to one 16-bit term (elsewhere to two bf16 terms; softmax_lse is
+ * that of the probabilities before, on either), and with
  * fp16 queries K and V are rounded to fp16, so that elements beyond +/-65504 saturate
  * and those of groups with scales below 2^-23 lose bits (elsewhere both are exact).
  * Enqueues up to three kernels; never synchronizes, never allocates.  The results
@@ -526,13 +527,15 @@ int mfa_kv8_fwd_params_size(void);
  *   weight[j, hkv] = (j < Lk - Lq ? weight[j, hkv] : 0)
  *                  + sum over query rows i and query heads h of hkv of exp(score_ihj - lse_ih)
  * for the keys j < Lk of every sequence with queries, Lq of them: keys before the
- * queries' own rows add to what they had, the queries' own start from 0.  What a row's
- * mask leaves out, and rows whose lse is -inf, add nothing.  Sequences with queries must
+ * queries' own rows add to what they had, the queries' own start from 0.  (So a pool needs
+ * no clearing where every row passes through a call as a query's own; rows that do not, as
+ * those of a prompt whose last rows alone are given, keep what their page held, from
+ * another sequence too, and the caller clears them first.)  What a row's mask leaves out, and rows whose lse is -inf, add nothing.  Sequences with queries must
  * not share pages.  weights: fp32
  * [num_pages, page_block_size, heads_kv] by element strides (row and head strides >= 0),
  * addressed with the cache's block table; a page id outside the pool drops what is
- * written.  Sums in fp32, in an order that sizes alone decide; every key has one
- * owner.  One or two kernels; never synchronizes, never allocates.
+ * written.  Sums in fp32, in an order that sizes and lengths alone decide; every key has
+ * one owner.  The soft-cap is off by up to softcap 2^-21.  One or two kernels; never synchronizes, never allocates.
  */
 typedef struct mfa_kv8_weights_params {
     mfa_kv8_fwd_params fwd;

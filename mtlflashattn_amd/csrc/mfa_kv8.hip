@@ -25,13 +25,16 @@
 
 namespace {
 
-
 // A block is one wavefront's where a call has at most this many new rows per sequence on
-// average, and at least this many heads of sequences: fewer are on their way at once in
-// either form, and a full block takes a wavefront 12 us.
-// (8 K/V heads of 128, bf16, 256 sequences of 1, 16, 32 rows: 7.5, 13.1, 23.9 us against
-// 12.0, 21.5, 29.2; 64 sequences of 1 and 5: 4.9 and 5.2 against 5.5 and 7.0; 31 single
-// rows beside 400: 12.5 against 6.3, 255 beside 3000: 19.1 against 19.9.)
+// average, and at least this many heads of sequences.  Which sequence has many rows is known
+// on the device only, and a full block takes a wavefront 12 us and a workgroup 5: calls of
+// fewer heads, whose blocks all run at once, lose more by it where they are ragged than they
+// gain where they are not.
+// (us as wavefronts / as workgroups, bf16 heads of 128.  8 of them, 256 sequences of 1, 5,
+// 16, 32 rows: 8.0 / 12.7, 9.4 / 15.9, 12.0 / 18.4, 20.4 / 24.0; 255 single rows beside 400:
+// 16.7 / 15.8, beside 3000: 18.2 / 18.8.  64 sequences of 1, 5, 16, 32: 5.0 / 5.7, 5.8 / 6.1,
+// 6.7 / 6.4, 10.3 / 7.7; 63 single rows beside 900: 12.7 / 7.2.  32 heads, 64 single rows:
+// 6.5 / 10.6; 63 beside 900: 16.7 / 15.8.)
 constexpr int kStepRows = 16, kStepHeads = 2048;
 
 struct A8Args {

@@ -8,8 +8,10 @@
 namespace {
 
 // The codes of two 16-key tiles, and their scale, which the whole block shares (32 keys
-// from a multiple of 32 on lie in one block of 64 rows).  Loads are non-temporal, as a
-// byte of the cache is read once a call.
+// from a multiple of 32 on lie in one block of 64 rows).  Loads are non-temporal: the kernels
+// for few columns read a byte of the cache once a call.  (The key weights of many columns
+// read a block again for every 128 of them where a workgroup has more blocks than
+// wavefronts.)
 //
 // The four lanes of a key's row take 16 adjacent bytes each of 64, so that a load
 // covers whole 64-byte pieces: piece p of a row gives lane group g elements 64 p + 16 g

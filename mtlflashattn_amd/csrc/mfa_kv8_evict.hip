@@ -19,8 +19,9 @@
 //    writes them with a new scale.
 // One sequence (2048 of 2176 rows stay, 8 heads of 128) takes 19 us, of which select, save
 // and gather have 8.6, 5.2 and 6.0: the latency of a few dependent passes each.  Sixteen
-// sequences (4001 of 4096 to 16384 rows stay) take 98 us, select 22 of them and the rest
-// the bytes and the conversions of the walk (save and gather: 111).  Selecting by 32 passes
+// sequences (4001 of 4096 to 16384 rows stay) take 81 us over data that the last-level cache
+// holds, select 22 of them and the rest the bytes and the conversions of the walk, and 98 us
+// over data outside of it (save and gather: 111).  Selecting by 32 passes
 // over one bit took 41 us, and save and gather by 512 threads instead of 256 18 us more.
 #include <stdarg.h>
 #include <stdio.h>
@@ -37,7 +38,10 @@ constexpr int kSThreads = 1024, kSWaves = kSThreads / 64;
 constexpr int kEThreads = 256;
 // Sequences times heads from which on one workgroup moves all rows of a head.  (64 heads of
 // 128, 2067 of 2176 rows: 47 us against 53 by save and gather; 32 heads 41 against 37, 128
-// heads 55 against 81, 8 heads 39 against 24.  128 heads, 4275 of 9500: 98 against 128.)
+// heads 55 against 81, 8 heads 39 against 24.  128 heads, 4275 of 9500: 98 against 128.
+// How many of them are over the budget is known on the device only: one sequence of 8 heads
+// that keeps 4275 of 9500 rows takes 66 us beside 63 that stay as they are, 26 alone, and one
+// of 2048 of 2176 33 and 16.)
 constexpr int kWalk = 64;
 constexpr int walk_threads(int d) { return d == 96 ? 768 : 1024; }  // (whole blocks per step)
 constexpr int kStay = 0x7fffffff;

@@ -14,8 +14,10 @@
 //  * at most 32: bound by the stream of K and the weights (136 bytes per key and head
 //    at head dim 128).  A wavefront takes every fourth 32-key block, the next one on
 //    its way into registers, and multiplies one or two tiles of 16 columns;
-//  * more: bound by the exponentials (24 cycles of a SIMD per 64 scores, against 16 of
-//    the products at head dim 128).  A wavefront holds 32 keys as operands and goes over
+//  * more: bound by vector instructions, nine per 64 scores beside the product's one, of
+//    which the exponential takes four slots (1024 rows over 8192 keys, D=128, 120 us: vector
+//    units active 69 % of the cycles, matrix pipe 25 %).  A wavefront holds 32 keys as
+//    operands and goes over
 //    the columns, 128 of which stand in LDS while the next are loaded straight into it;
 //    eight wavefronts share them.  64 rows over two prompts of 12000 to 16384 keys, Hq=32
 //    Hkv=8 D=128: 32 us, of which about 10 pass before the first product (the dealing,

@@ -40,7 +40,8 @@ __device__ __forceinline__ int vswz4(int r) {
 // LSE: the log-sum-exp is asked for.  Its sum is of the probabilities before they are
 // rounded, beside that of the rounded ones, which the result is divided by: what the
 // roundings of a row's weights have in common cancels there, but would leave the
-// log-sum-exp off by up to 2^-8 in bf16 and 2^-11 in fp16.
+// log-sum-exp off by up to 2^-8 in bf16 and 2^-11 in fp16.  (The 8-bit cache, 1024 rows over
+// 16384 keys, Hq=32 Hkv=8 D=128: 326 us for 316, 348 for 331 in fp16.)
 template <class Stage, bool BIAS, bool LSE>
 __global__ void __launch_bounds__(kThreads4) __attribute__((amdgpu_waves_per_eu(2)))
 mfa_kv_tile_kernel(K4Args) {

@@ -280,8 +280,9 @@ def flash_attn_kv4_func(q, k_cache, v_cache, cache_seqlens, block_table, softmax
     the workspace and the grid small.  Sequences of more than 32 columns (query
     positions times heads per K/V head) run on tiles of 128 columns, whose
     probabilities are rounded once to q.dtype (bf16: an error of 1.4 times the output's
-    rounding alone) and which, for fp16 queries, round K and V to fp16 (beyond 65504
-    they saturate); fewer columns keep two terms and exact K and V.  A page id outside the pool reads as zeros and
+    rounding alone; the log-sum-exp is that of the probabilities before) and which, for
+    fp16 queries, round K and V to fp16 (beyond 65504 they saturate); fewer columns keep
+    two terms and exact K and V.  A page id outside the pool reads as zeros and
     its keys are not masked; MTLFLASHATTN_CHECK_PAGES=1 checks the ids on the host.
     Forward only: a query that requires grad raises.
     """

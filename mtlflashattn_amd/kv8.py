@@ -71,8 +71,8 @@ def flash_attn_kv8_func(q, k_cache, v_cache, cache_seqlens, block_table, softmax
     K is exact; so is V, except on the tiles of 128 columns (sequences of more than 32
     columns; in a varlen call of more than 32 in total, of more than 16, but not where its
     sequences have 17 to 32 on average) with fp16 queries, where it is rounded to fp16 (beyond 65504 it saturates;
-    scales below 2^-15 may lose bits).  NaN elements reach only the rows whose mask
-    holds their key.
+    scales below 2^-15 may lose bits).  The log-sum-exps are those of the probabilities before
+    they are rounded.  NaN elements reach only the rows whose mask holds their key.
     """
     if torch.is_tensor(q) and q.dim() != 4:
         raise ValueError(f"mtlflashattn_amd: expected q [B,Lq,H,D], got {q.dim()}-D")
@@ -120,12 +120,15 @@ def kv8_key_weights(q, k_cache, softmax_lse, weights, cache_seqlens, block_table
       weights = (j < Lk - Lq ? weights : 0) + sum of softmax(...)[i, j] over the sequence's
                 query rows i and the query heads of h,
     so keys before the queries' own rows add to what they had and the queries' own, new
-    in this step, start from 0: the pool needs no clearing.  What a row's mask leaves out
-    adds nothing, and sequences without queries keep their weights.  Sequences with queries
-    must not share pages (a fork's weights need pages of their own).  The weights that the
-    last rows of a prompt alone give come from a call with those rows and their
-    log-sum-exps: then only those rows' own keys start from 0.
+    in this step, start from 0: where every row of a sequence has been a query of some call
+    the pool needs no clearing.  What a row's mask leaves out adds nothing, and sequences
+    without queries keep their weights.  Sequences with queries must not share pages (a
+    fork's weights need pages of their own).  The weights that the last rows of a prompt
+    alone give come from a call with those rows and their log-sum-exps: then only those
+    rows' own keys start from 0, and the others add to what their pages held, from other
+    sequences too, so clear the pages of such a prompt first (weights[pages] = 0).
 
+    A weight is as exact as the log-sum-exps are (those of the attention calls: 1e-4).
     Sums in fp32, every key by one owner in an order that sizes and lengths alone
     decide; no synchronisation.  Any strides; each head's rows of a page side by side are
     read fastest.  Not differentiable: tensors that require grad raise.
